@@ -250,6 +250,104 @@ ZJAI_API int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv, 
                                                 const float* temperature, int32_t precision,
                                                 void* out);
 
+/* ------------------------------------------------ causal context: decayed linear attention */
+
+/* Linear attention with a decay for each head. Over the positions t = 0, 1, .. of a sequence every
+ * head keeps a state S [key_dim][value_dim], which starts at zero or at state_in:
+ *     S_t = decay * S_(t-1) + k_t^T v_t          out_t = scale * q_t S_t
+ * (q, k: key_dim channels, v and out: value_dim). Position t is reached by positions 0..t only: a
+ * context model of this form can be evaluated over a whole map of known latents at once (the
+ * encoder) or position by position as they are decoded, with the same result up to rounding. It has
+ * no counterpart in the reference, whose channel attention (src/nn/fast/math.rs:512) has the same
+ * cost, linear in the positions, but is not causal. Products and sums are f32 whatever the
+ * precision, states are f32 arrays. A non-finite q, k or v reaches the outputs of its own position
+ * and later ones only (infinities may arrive there as NaN), a non-finite state_in every output of its
+ * head.
+ *
+ * zjai_linear_attention takes a map of packed channels, [q | k | v] of heads * key_dim, heads *
+ * key_dim and heads * value_dim channels, the heads one after another in each (value_dim is what the
+ * channel count leaves): with rows = 0 its positions are one sequence in raster order, with rows = 1
+ * every row is a sequence. decay: `heads` floats in [0, 1]. -> heads * value_dim channels. */
+ZJAI_API int32_t zjai_linear_attention(zjai_ctx* ctx, const zjai_tensor* qkv, int32_t heads,
+                                       int32_t key_dim, const float* decay, float scale, int32_t rows,
+                                       zjai_tensor** out);
+
+/* The same on the caller's device buffers, for callers that cannot allocate (serving loops) or that
+ * carry states from call to call. Element strides; q, k, v of a position are
+ * [heads][key_dim or value_dim], dense, so that packed channels (one buffer, q, k and v pointing into
+ * it) and separate buffers both work. `out` shares no element with q, k, v. Pointers are aligned to
+ * their element; 16-byte aligned buffers, strides and head sizes of whole 16 bytes run fastest. */
+typedef struct zjai_linear_attention_desc {
+    int32_t precision, heads, key_dim, value_dim; /* key_dim 1..128, value_dim 1..1024 */
+    int32_t sequences, length;                    /* length: the positions a sequence has room for */
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_position, k_position, v_position, out_position; /* from one position to the next */
+    int64_t q_sequence, k_sequence, v_sequence, out_sequence; /* from one sequence to the next */
+    const float* decay;     /* device, [heads], in [0, 1] */
+    float scale;
+    int32_t num_slots;      /* step: states in state_in / state_out (0: as many as sequences) */
+    const int32_t* lengths; /* device, [sequences], or NULL (all of `length`): positions a sequence
+                               has, taken into 0..length; outputs past them stay as they were */
+    const int32_t* slots;   /* step: device, [sequences], or NULL (sequence i has state i) */
+    const float* state_in;  /* device, [sequences][heads][key_dim][value_dim], or NULL (zeros) */
+    float* state_out;       /* the states after the last position, or NULL; may be state_in, and
+                               overlaps it in no other way */
+} zjai_linear_attention_desc;
+
+/* Whole sequences. desc->slots must be NULL. Enqueued on the context's stream (zjai_sync waits for
+ * it); works in the context's scratch, as zjai_channel_attention_noalloc, and allocates nothing. */
+ZJAI_API int32_t zjai_linear_attention_noalloc(zjai_ctx* ctx, const zjai_linear_attention_desc* desc);
+/* The recurrent form: one position of each sequence (length 1, lengths NULL, both states given).
+ * Sequence i reads state_in[slots[i]] and writes state_out[slots[i]]; states of other slots stay as
+ * they were. A slot outside 0..num_slots-1 marks an idle sequence, whose output stays as it was.
+ * Sequences with the same slot follow one another in their order, as consecutive positions. */
+ZJAI_API int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_attention_desc* desc);
+
+/* ---------------------------------------------- the join of two blocks: norms, gate, residual */
+
+#define ZJAI_NORM_NONE 0
+#define ZJAI_NORM_LAYER 1 /* (v - mean) / sqrt(var + eps) */
+#define ZJAI_NORM_RMS 2   /* v / sqrt(mean(v^2) + eps) */
+#define ZJAI_GATE_LINEAR 0  /* g */
+#define ZJAI_GATE_SIGMOID 1 /* 1 / (1 + exp(-g)) */
+#define ZJAI_GATE_SILU 2    /* g / (1 + exp(-g)) */
+
+/* The end of a residual block and the start of the next in one pass over the positions: the norm
+ * after the block, its gate and residual scale, the residual sum, and the norm before the next block:
+ *     x_out = x + residual_scale * (post_norm(y) * gate_act(gate))
+ *     h     = pre_norm(x_out)
+ * over the channels of each position; post_norm works in post_groups groups of channels (the heads
+ * of an attention), pre_norm over all of them; norms are followed by `* weight + bias`. Statistics
+ * and intermediate values are f32, x_out and h are rounded once each (h from the unrounded
+ * x_out). Stands for zjai_layer_norm_channels, zjai_sigmoid, zjai_mul_assign, zjai_add_assign and
+ * another norm. Absent parts are NULL: gate (1), residual_scale (1), weights (1) and biases (0); a norm of
+ * ZJAI_NORM_NONE takes neither weight nor bias.
+ *
+ * Tensor form: x, y, gate of one shape, weights on the host; new tensors x_out and (unless pre_norm
+ * is ZJAI_NORM_NONE, when out_h may be NULL) h. */
+ZJAI_API int32_t zjai_norm_gate_residual(zjai_ctx* ctx, const zjai_tensor* x, const zjai_tensor* y,
+                                         const zjai_tensor* gate, int32_t gate_act, int32_t post_norm,
+                                         int32_t post_groups, float post_eps, const float* post_weight,
+                                         const float* post_bias, const float* residual_scale,
+                                         int32_t pre_norm, float pre_eps, const float* pre_weight,
+                                         const float* pre_bias, zjai_tensor** out_x, zjai_tensor** out_h);
+
+/* On the caller's device buffers: [positions][channels] with a stride (in elements) from one position to the
+ * next. x_out may be x, and h may be y, gate or x, with that buffer's stride; buffers overlap in no other
+ * way. Weights are device arrays of `channels` floats. Enqueued on the context's stream. */
+typedef struct zjai_norm_gate_residual_desc {
+    int32_t precision, channels; /* channels 1..16384 */
+    int64_t positions;
+    const void *x, *y, *gate;
+    void *x_out, *h;             /* h: NULL with ZJAI_NORM_NONE */
+    int64_t x_stride, y_stride, gate_stride, x_out_stride, h_stride;
+    int32_t gate_act, post_norm, post_groups, pre_norm;
+    float post_eps, pre_eps;     /* > 0 where the norm is used */
+    const float *post_weight, *post_bias, *residual_scale, *pre_weight, *pre_bias;
+} zjai_norm_gate_residual_desc;
+ZJAI_API int32_t zjai_norm_gate_residual_noalloc(zjai_ctx* ctx, const zjai_norm_gate_residual_desc* desc);
+
 /* ------------------------------------------------------------------------ synthesis nets */
 
 /* `SynthesisPrimary::load` / `SynthesisSecondary::load` (src/model/synthesis.rs:242, :972) from

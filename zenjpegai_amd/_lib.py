@@ -41,6 +41,8 @@ CTX_COUNT_F16_RANGE = 0x10
 CTX_VALU_NARROW_CONVT = 0x20
 FAIL_NONE, FAIL_ALLOC, FAIL_LAUNCH = 0, 1, 2  # zjai_inject_failure kinds
 RESIZE_BICUBIC, RESIZE_BILINEAR = 0, 1
+NORMS = {"none": 0, "layer": 1, "rms": 2}  # ZJAI_NORM_*
+GATES = {"linear": 0, "sigmoid": 1, "silu": 2}  # ZJAI_GATE_*
 PLANE_LATENT, PLANE_PSI, PLANE_HYPER_LATENT, PLANE_IMAGE = 0, 1, 2, 3
 
 
@@ -68,6 +70,26 @@ class ZjaiStats(ctypes.Structure):
 class ZjaiMemoryEstimate(ctypes.Structure):
     _fields_ = [("picture_bytes", ctypes.c_uint64), ("live_bytes", ctypes.c_uint64),
                 ("pool_bytes", ctypes.c_uint64)]
+
+
+class ZjaiLinearAttentionDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("precision", "heads", "key_dim", "value_dim", "sequences", "length")]
+                + [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out")]
+                + [(n, ctypes.c_int64) for n in (
+                    "q_position", "k_position", "v_position", "out_position",
+                    "q_sequence", "k_sequence", "v_sequence", "out_sequence")]
+                + [("decay", ctypes.c_void_p), ("scale", ctypes.c_float), ("num_slots", ctypes.c_int32)]
+                + [(n, ctypes.c_void_p) for n in ("lengths", "slots", "state_in", "state_out")])
+
+
+class ZjaiNormGateResidualDesc(ctypes.Structure):
+    _fields_ = ([("precision", ctypes.c_int32), ("channels", ctypes.c_int32), ("positions", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("x", "y", "gate", "x_out", "h")]
+                + [(n, ctypes.c_int64) for n in ("x_stride", "y_stride", "gate_stride", "x_out_stride", "h_stride")]
+                + [(n, ctypes.c_int32) for n in ("gate_act", "post_norm", "post_groups", "pre_norm")]
+                + [("post_eps", ctypes.c_float), ("pre_eps", ctypes.c_float)]
+                + [(n, ctypes.c_void_p) for n in (
+                    "post_weight", "post_bias", "residual_scale", "pre_weight", "pre_bias")])
 
 
 class ZjaiProfRecord(ctypes.Structure):
@@ -120,6 +142,12 @@ PROTOTYPES = {
     "zjai_layer_norm_channels": [_vp, _vp, _f32p, _f32p, _pp],
     "zjai_channel_attention": [_vp, _vp, _i32, _f32p, _pp],
     "zjai_channel_attention_noalloc": [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp],
+    "zjai_linear_attention": [_vp, _vp, _i32, _i32, _f32p, ctypes.c_float, _i32, _pp],
+    "zjai_linear_attention_noalloc": [_vp, ctypes.POINTER(ZjaiLinearAttentionDesc)],
+    "zjai_linear_attention_step": [_vp, ctypes.POINTER(ZjaiLinearAttentionDesc)],
+    "zjai_norm_gate_residual": [_vp, _vp, _vp, _vp, _i32, _i32, _i32, ctypes.c_float, _f32p, _f32p, _f32p,
+                                _i32, ctypes.c_float, _f32p, _f32p, _pp, _pp],
+    "zjai_norm_gate_residual_noalloc": [_vp, ctypes.POINTER(ZjaiNormGateResidualDesc)],
     "zjai_net_create": [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(ctypes.c_char_p), _i32p,
                         _i32p, ctypes.POINTER(_f32p), _pp],
     "zjai_net_destroy": [_vp],

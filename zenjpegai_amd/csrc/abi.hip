@@ -533,6 +533,300 @@ extern "C" int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv
     });
 }
 
+// ------------------------------------------------------- causal context: decayed linear attention
+namespace {
+
+// Makes the context's device current for a call on the caller's buffers and restores the caller's.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int d = -1;
+        ZJAI_HIP(hipGetDevice(&d));
+        if (d == device) return;
+        ZJAI_HIP(hipSetDevice(device));
+        before = d;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
+void need_aligned(const void* p, int bytes, const char* msg) { need(((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0, msg); }
+
+void check_linear_dims(int heads, int dk, int dv) {
+    need(heads > 0 && dk > 0 && dv > 0, "linear attention: head count and sizes");
+    if (dk > LIN_MAX_KEY || dv > LIN_MAX_VALUE)
+        throw Error(ZJAI_E_UNSUPPORTED, "linear attention: more than 128 key or 1024 value channels per head");
+}
+
+void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype) {
+    const double n = (double)a.seqs * a.length, hs = (double)a.heads * a.dk * a.dv;
+    const double bytes = n * a.heads * dtype_size(dtype) * (2.0 * a.dk + 2.0 * a.dv) +
+                         4.0 * a.seqs * hs * ((a.s_in != nullptr) + (a.s_out != nullptr));
+    if (linear_recurrent_groups(a) > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
+    LaunchScope sc(C, linear_recurrent_name(a, dtype), 4.0 * n * hs, bytes);
+    ZJAI_HIP(launch_linear_recurrent(a, dtype, C.stream));
+}
+
+// The descriptor's buffers; `step`: the recurrent form's rules.
+LinAttnArgs linear_args(const zjai_linear_attention_desc& d, bool step) {
+    need(d.precision >= DT_F32 && d.precision <= DT_BF16, "precision");
+    check_linear_dims(d.heads, d.key_dim, d.value_dim);
+    need(d.sequences >= 0 && d.length >= 0, "linear attention: negative count");
+    need(std::isfinite(d.scale), "linear attention: scale");
+    need(d.decay != nullptr, "linear attention: null decay");
+    need_aligned(d.decay, 4, "linear attention: decay not aligned");
+    need_aligned(d.state_in, 4, "linear attention: states not aligned");
+    need_aligned(d.state_out, 4, "linear attention: states not aligned");
+    need_aligned(d.lengths, 4, "linear attention: lengths not aligned");
+    need_aligned(d.slots, 4, "linear attention: slots not aligned");
+    const int es = dtype_size(d.precision);
+    if (d.sequences > 0 && d.length > 0) {
+        need(d.q && d.k && d.v && d.out, "linear attention: null buffer");
+        for (const void* p : {d.q, d.k, d.v, (const void*)d.out}) need_aligned(p, es, "linear attention: buffers not aligned to their element");
+        need(d.out != d.q && d.out != d.k && d.out != d.v, "linear attention: out is an input");
+    }
+    need(d.q_position >= 0 && d.k_position >= 0 && d.v_position >= 0 && d.q_sequence >= 0 && d.k_sequence >= 0 &&
+             d.v_sequence >= 0 && d.out_position >= 0 && d.out_sequence >= 0,
+         "linear attention: negative stride");
+    // Outputs of two positions must not share elements: sequence after sequence, or position after position.
+    const int64_t ow = (int64_t)d.heads * d.value_dim;
+    if (d.sequences > 0 && d.length > 0) {
+        need(d.length == 1 || d.out_position >= ow, "linear attention: output positions overlap");
+        need(d.sequences == 1 || d.out_sequence >= ow, "linear attention: output sequences overlap");
+        const __int128 along = (__int128)(d.length - 1) * d.out_position + ow, across = (__int128)(d.sequences - 1) * d.out_sequence + ow;
+        need(d.sequences == 1 || d.length == 1 || d.out_sequence >= along || d.out_position >= across, "linear attention: output sequences overlap");
+    }
+    if (step) {
+        need(d.length == 1 && !d.lengths, "linear attention step: one position a sequence, no lengths");
+        need(d.state_in && d.state_out, "linear attention step: null states");
+        need(d.num_slots >= 0 && (d.slots || d.num_slots == 0 || d.num_slots >= d.sequences), "linear attention step: slots");
+        need(!d.slots || d.num_slots > 0 || d.sequences == 0, "linear attention step: slots without their number");
+    } else {
+        need(!d.slots && d.num_slots == 0, "linear attention: slots are the recurrent form's");
+    }
+    const int64_t states = step && d.slots ? d.num_slots : d.sequences;
+    if (d.state_in && d.state_out && d.state_in != d.state_out) {
+        const uintptr_t a = (uintptr_t)d.state_in, b = (uintptr_t)d.state_out;
+        const uintptr_t n = (uintptr_t)states * d.heads * d.key_dim * d.value_dim * 4;
+        need(a + n <= b || b + n <= a, "linear attention: states overlap");
+    }
+    LinAttnArgs a{};
+    a.q = LinRows{d.q, d.q_sequence, 0, d.q_position};
+    a.k = LinRows{d.k, d.k_sequence, 0, d.k_position};
+    a.v = LinRows{d.v, d.v_sequence, 0, d.v_position};
+    a.o = LinRows{d.out, d.out_sequence, 0, d.out_position};
+    a.seqs = d.sequences;
+    a.length = d.length;
+    a.heads = d.heads;
+    a.dk = d.key_dim;
+    a.dv = d.value_dim;
+    a.decay = d.decay;
+    a.scale = d.scale;
+    a.lengths = d.lengths;
+    a.slots = d.slots;
+    a.num_slots = d.num_slots;
+    a.s_in = d.state_in;
+    a.s_out = d.state_out;
+    return a;
+}
+
+}  // namespace
+
+extern "C" int32_t zjai_linear_attention(zjai_ctx* ctx, const zjai_tensor* qkv, int32_t heads, int32_t key_dim,
+                                         const float* decay, float scale, int32_t rows, zjai_tensor** out) {
+    if (!ctx || !qkv || !decay || !out) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const Tensor& x = *qkv->t;
+        need(x.n == 1, "linear attention: one map");
+        need(heads > 0 && key_dim > 0 && x.c % heads == 0 && (long long)x.c / heads > 2LL * key_dim, "linear attention: channel / head counts");
+        const int dv = x.c / heads - 2 * key_dim;
+        check_linear_dims(heads, key_dim, dv);
+        need(std::isfinite(scale), "linear attention: scale");
+        need(rows == 0 || rows == 1, "linear attention: rows");
+        need(rows || (long long)x.h * x.w <= INT32_MAX, "linear attention: too many positions");
+        for (int h = 0; h < heads; ++h) need(decay[h] >= 0.0f && decay[h] <= 1.0f, "linear attention: decay outside [0, 1]");
+        TensorP y = ctx->c.alloc(x.n, heads * dv, x.h, x.w, x.dtype);
+        if (x.h > 0 && x.w > 0) {
+            float* d = (float*)ctx->c.pool.alloc(sizeof(float) * heads);
+            std::shared_ptr<void> keep(d, [ctx](void* q) { ctx->c.pool.release(q); });
+            ZJAI_HIP(hipMemcpyAsync(d, decay, sizeof(float) * heads, hipMemcpyHostToDevice, ctx->c.stream));
+            const int es = dtype_size(x.dtype);
+            const auto part = [&](const View& v, int c0) {
+                char* p = (char*)v.p + (size_t)(v.c_off + c0) * es;
+                return LinRows{p, rows ? v.row : v.bstride, rows ? 0 : v.row, v.cs};
+            };
+            LinAttnArgs a{};
+            a.q = part(x.v, 0);
+            a.k = part(x.v, heads * key_dim);
+            a.v = part(x.v, 2 * heads * key_dim);
+            a.o = part(y->v, 0);
+            // Rows that follow one another without a gap are one run of positions.
+            a.width = rows || (x.v.row == (long long)x.w * x.v.cs) ? 0 : x.w;
+            a.seqs = rows ? x.h : x.n;
+            a.length = rows ? x.w : x.h * x.w;
+            a.heads = heads;
+            a.dk = key_dim;
+            a.dv = dv;
+            a.decay = d;
+            a.scale = scale;
+            run_linear_attention(ctx->c, a, x.dtype);
+            count_f16_range(ctx->c, *y);
+            ZJAI_HIP(hipStreamSynchronize(ctx->c.stream));
+        }
+        *out = new zjai_tensor{y};
+    });
+}
+
+extern "C" int32_t zjai_linear_attention_noalloc(zjai_ctx* ctx, const zjai_linear_attention_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const LinAttnArgs a = linear_args(*desc, false);
+        if (a.seqs > 0 && (a.length > 0 || a.s_out)) run_linear_attention(ctx->c, a, desc->precision);
+    });
+}
+
+extern "C" int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_attention_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const LinAttnArgs a = linear_args(*desc, true);
+        if (a.seqs > 0) run_linear_attention(ctx->c, a, desc->precision);
+    });
+}
+
+// --------------------------------------------------- the join of two blocks: norms, gate, residual
+namespace {
+
+void check_join(int channels, int gate, int gate_act, int post, int groups, float post_eps, bool post_vec, int pre, float pre_eps,
+                bool pre_vec, bool h) {
+    need(channels > 0, "norm / gate / residual: channel count");
+    if (channels > JOIN_MAX_CHANNELS) throw Error(ZJAI_E_UNSUPPORTED, "norm / gate / residual: more than 16384 channels");
+    need(gate_act >= GATE_LINEAR && gate_act <= GATE_SILU && (gate || gate_act == GATE_LINEAR), "norm / gate / residual: gate_act");
+    need(post >= NORM_NONE && post <= NORM_RMS && pre >= NORM_NONE && pre <= NORM_RMS, "norm / gate / residual: norm");
+    need(groups > 0 && channels % groups == 0, "norm / gate / residual: channels not divisible by post_groups");
+    need(post == NORM_NONE ? !post_vec : std::isfinite(post_eps) && post_eps > 0.0f, "norm / gate / residual: post_norm's eps or weights");
+    need(pre == NORM_NONE ? !pre_vec : std::isfinite(pre_eps) && pre_eps > 0.0f, "norm / gate / residual: pre_norm's eps or weights");
+    need(h == (pre != NORM_NONE), "norm / gate / residual: h goes with pre_norm");
+}
+
+void run_join(Context& C, const JoinArgs& a, int dtype) {
+    const double n = (double)a.positions * a.channels, arrays = 3.0 + (a.g.p != nullptr) + (a.h.p != nullptr);
+    LaunchScope sc(C, join_name(a, dtype), 20.0 * n, n * arrays * dtype_size(dtype));
+    ZJAI_HIP(launch_join(a, dtype, C.stream));
+}
+
+}  // namespace
+
+extern "C" int32_t zjai_norm_gate_residual(zjai_ctx* ctx, const zjai_tensor* x, const zjai_tensor* y, const zjai_tensor* gate,
+                                           int32_t gate_act, int32_t post_norm, int32_t post_groups, float post_eps,
+                                           const float* post_weight, const float* post_bias, const float* residual_scale,
+                                           int32_t pre_norm, float pre_eps, const float* pre_weight, const float* pre_bias,
+                                           zjai_tensor** out_x, zjai_tensor** out_h) {
+    if (!ctx || !x || !y || !out_x) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const Tensor& a = *x->t;
+        for (const zjai_tensor* t : {y, gate})
+            need(!t || (t->t->n == a.n && t->t->c == a.c && t->t->h == a.h && t->t->w == a.w && t->t->dtype == a.dtype), "shapes differ");
+        need(a.n == 1, "norm / gate / residual: one map");
+        check_join(a.c, gate != nullptr, gate_act, post_norm, post_groups, post_eps, post_weight || post_bias, pre_norm, pre_eps,
+                   pre_weight || pre_bias, pre_norm != NORM_NONE && out_h);
+        TensorP xo = ctx->c.alloc(1, a.c, a.h, a.w, a.dtype), h;
+        if (pre_norm != NORM_NONE) h = ctx->c.alloc(1, a.c, a.h, a.w, a.dtype);
+        if (a.h > 0 && a.w > 0) {
+            const float* host[5] = {post_weight, post_bias, residual_scale, pre_weight, pre_bias};
+            float* d = (float*)ctx->c.pool.alloc(sizeof(float) * 5 * a.c);
+            std::shared_ptr<void> keep(d, [ctx](void* q) { ctx->c.pool.release(q); });
+            const float* dev[5] = {};
+            for (int i = 0; i < 5; ++i)
+                if (host[i]) {
+                    ZJAI_HIP(hipMemcpyAsync(d + (size_t)i * a.c, host[i], sizeof(float) * a.c, hipMemcpyHostToDevice, ctx->c.stream));
+                    dev[i] = d + (size_t)i * a.c;
+                }
+            const int es = dtype_size(a.dtype);
+            const auto rows = [&](const View& v) { return JoinRows{(char*)v.p + (size_t)v.c_off * es, v.row, v.cs}; };
+            JoinArgs j{};
+            j.x = rows(a.v);
+            j.y = rows(y->t->v);
+            if (gate) j.g = rows(gate->t->v);
+            j.xo = rows(xo->v);
+            if (h) j.h = rows(h->v);
+            j.positions = (long long)a.h * a.w;
+            j.width = a.w;
+            j.channels = a.c;
+            j.gate = gate_act;
+            j.post = post_norm;
+            j.groups = post_groups;
+            j.pre = pre_norm;
+            j.post_eps = post_eps;
+            j.pre_eps = pre_eps;
+            j.post_w = dev[0];
+            j.post_b = dev[1];
+            j.scale = dev[2];
+            j.pre_w = dev[3];
+            j.pre_b = dev[4];
+            run_join(ctx->c, j, a.dtype);
+            count_f16_range(ctx->c, *xo);
+            if (h) count_f16_range(ctx->c, *h);
+            ZJAI_HIP(hipStreamSynchronize(ctx->c.stream));
+        }
+        std::unique_ptr<zjai_tensor> tx(new zjai_tensor{xo});
+        if (out_h) *out_h = h ? new zjai_tensor{h} : nullptr;
+        *out_x = tx.release();
+    });
+}
+
+extern "C" int32_t zjai_norm_gate_residual_noalloc(zjai_ctx* ctx, const zjai_norm_gate_residual_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const zjai_norm_gate_residual_desc& d = *desc;
+        need(d.precision >= DT_F32 && d.precision <= DT_BF16, "precision");
+        need(d.positions >= 0, "norm / gate / residual: positions");
+        check_join(d.channels, d.gate != nullptr, d.gate_act, d.post_norm, d.post_groups, d.post_eps, d.post_weight || d.post_bias,
+                   d.pre_norm, d.pre_eps, d.pre_weight || d.pre_bias, d.h != nullptr);
+        const int es = dtype_size(d.precision);
+        need(d.positions == 0 || (d.x && d.y && d.x_out), "norm / gate / residual: null buffer");
+        for (const void* p : {d.x, d.y, d.gate, (const void*)d.x_out, (const void*)d.h})
+            need_aligned(p, es, "norm / gate / residual: buffers not aligned to their element");
+        for (const float* p : {d.post_weight, d.post_bias, d.residual_scale, d.pre_weight, d.pre_bias})
+            need_aligned(p, 4, "norm / gate / residual: weights not aligned");
+        need(d.x_stride >= 0 && d.y_stride >= 0 && d.gate_stride >= 0, "norm / gate / residual: negative stride");
+        need(d.positions <= 1 || (d.x_out_stride >= d.channels && (!d.h || d.h_stride >= d.channels)), "norm / gate / residual: output positions overlap");
+        need(d.x_out != d.h || !d.h || d.positions == 0, "norm / gate / residual: x_out and h are one buffer");
+        need(d.positions <= 1 || ((d.x_out != d.x || d.x_out_stride == d.x_stride) && (d.h != d.y || d.h_stride == d.y_stride) &&
+                                  (d.h != d.gate || !d.h || d.h_stride == d.gate_stride) && (d.h != d.x || d.h_stride == d.x_stride)),
+             "norm / gate / residual: in place with another stride");
+        need(d.x_out != d.y && (!d.gate || d.x_out != d.gate), "norm / gate / residual: x_out is y or gate");
+        if (d.positions == 0) return;
+        JoinArgs j{};
+        j.x = JoinRows{const_cast<void*>(d.x), 0, d.x_stride};
+        j.y = JoinRows{const_cast<void*>(d.y), 0, d.y_stride};
+        j.g = JoinRows{const_cast<void*>(d.gate), 0, d.gate_stride};
+        j.xo = JoinRows{d.x_out, 0, d.x_out_stride};
+        j.h = JoinRows{d.h, 0, d.h_stride};
+        j.positions = d.positions;
+        j.channels = d.channels;
+        j.gate = d.gate_act;
+        j.post = d.post_norm;
+        j.groups = d.post_groups;
+        j.pre = d.pre_norm;
+        j.post_eps = d.post_eps;
+        j.pre_eps = d.pre_eps;
+        j.post_w = d.post_weight;
+        j.post_b = d.post_bias;
+        j.scale = d.residual_scale;
+        j.pre_w = d.pre_weight;
+        j.pre_b = d.pre_bias;
+        run_join(ctx->c, j, d.precision);
+    });
+}
+
 // ----------------------------------------------------------------------------------- nets
 static std::map<std::string, Param> params_of(int32_t n_tensors, const char* const* names, const int32_t* ndims,
                                               const int32_t* dims, const float* const* data) {

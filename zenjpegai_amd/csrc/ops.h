@@ -128,6 +128,49 @@ hipError_t launch_attention_softmax(const float* partial, int N, int nchunk, int
 hipError_t launch_attention_fold(const float* proj, const float* attn, int N, int dim, int heads,
                                  int dtype, int nblk, void* wpk, long long w_bstride,
                                  hipStream_t s);
+// Linear attention with a decay for each head (zjai_linear_attention): buffers as the descriptor of the
+// C-ABI. Position t of sequence s lies at s * seq + t * pos or, with width > 0 (rows of `width` positions),
+// at s * seq + (t / width) * row + (t % width) * pos.
+struct LinRows {
+    const void* p;
+    long long seq, row, pos;
+};
+struct LinAttnArgs {
+    LinRows q, k, v, o;
+    int width;  // 0: no rows
+    int seqs, length, heads, dk, dv;
+    const float* decay;
+    float scale;
+    const int* lengths;
+    const int* slots;
+    int num_slots;
+    const float* s_in;
+    float* s_out;
+};
+constexpr int LIN_MAX_KEY = 128, LIN_MAX_VALUE = 1024;
+// The recurrent form: a workgroup keeps its part of a state in registers over the positions.
+long long linear_recurrent_groups(const LinAttnArgs& a);
+std::string linear_recurrent_name(const LinAttnArgs& a, int dtype);
+hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t s);
+// Norm, gate, residual scale, residual sum and norm of each position (zjai_norm_gate_residual): views of
+// N x [h][w][C] (x_out may be x; h may be y, g or x).
+enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
+enum GateAct : int { GATE_LINEAR = 0, GATE_SIGMOID = 1, GATE_SILU = 2 };
+struct JoinRows {
+    void* p;
+    long long row, pos;  // position i at (i / width) * row + (i % width) * pos
+};
+struct JoinArgs {
+    JoinRows x, y, g, xo, h;  // g.p / h.p may be null
+    long long positions;
+    int width, channels;
+    int gate, post, groups, pre;
+    float post_eps, pre_eps;
+    const float *post_w, *post_b, *scale, *pre_w, *pre_b;  // each may be null
+};
+constexpr int JOIN_MAX_CHANNELS = 16384;
+std::string join_name(const JoinArgs& a, int dtype);
+hipError_t launch_join(const JoinArgs& a, int dtype, hipStream_t s);
 // Zero `bytes` (a multiple of 4, 4-byte aligned) at p with a kernel.
 hipError_t launch_zero(void* p, size_t bytes, hipStream_t s);
 // Adds the non-finite f16 samples of an N x [h][w][C] view to slots[0 .. nslots) (nslots

@@ -340,3 +340,101 @@ def channel_attention(eng: Engine, qkv: BTensor, heads: int, temperature) -> BTe
     check(lib().zjai_channel_attention(eng.handle, qkv._h, heads, _fp(t), ctypes.byref(out)),
           eng.handle)
     return BTensor(eng, out)
+
+
+# ------------------------------------------------- causal context: decayed linear attention
+def linear_attention(eng: Engine, qkv: BTensor, heads: int, key_dim: int, decay, scale: float = 1.0,
+                     rows: bool = False) -> BTensor:
+    """Linear attention with a decay for each head over a map of packed channels
+    ``[q | k | v]``, in raster order or (``rows``) row by row (``zjai_linear_attention``)."""
+    out = ctypes.c_void_p()
+    d = _f32(np.ravel(decay))
+    if d.size != heads:
+        raise HipError(_lib.E_INVALID_ARGUMENT, "linear attention: one decay for each head")
+    check(lib().zjai_linear_attention(eng.handle, qkv._h, heads, key_dim, _fp(d), scale, int(rows),
+                                      ctypes.byref(out)), eng.handle)
+    return BTensor(eng, out)
+
+
+def _address(a):
+    """The device address of a buffer: None, a number, or anything with ``data_ptr()``."""
+    return a.data_ptr() if hasattr(a, "data_ptr") else a
+
+
+def linear_attention_desc(precision: str, qkv, out, *, heads: int, key_dim: int, value_dim: int,
+                          sequences: int, length: int, decay, scale: float = 1.0, lengths=None,
+                          slots=None, num_slots: int = 0, state_in=None, state_out=None,
+                          **strides) -> _lib.ZjaiLinearAttentionDesc:
+    """A descriptor for ``linear_attention_noalloc`` / ``linear_attention_step`` over device buffers
+    (addresses, or objects with ``data_ptr()``, which the caller keeps alive). ``qkv`` is one
+    buffer of packed channels, dense over positions and sequences, or a tuple ``(q, k, v)`` of
+    dense buffers; ``strides`` (``q_position=...``, ``out_sequence=...``) replaces single ones."""
+    kc, vc = heads * key_dim, heads * value_dim
+    if isinstance(qkv, (tuple, list)):
+        q, k, v = (_address(a) for a in qkv)
+        pos = {"q": kc, "k": kc, "v": vc}
+    else:
+        es = 4 if precision == "f32" else 2
+        q = _address(qkv)
+        k, v = q + kc * es, q + 2 * kc * es
+        pos = dict.fromkeys("qkv", 2 * kc + vc)
+    pos["out"] = vc
+    st = {n + "_position": p for n, p in pos.items()}
+    st.update({n + "_sequence": p * length for n, p in pos.items()})
+    st.update(strides)
+    return _lib.ZjaiLinearAttentionDesc(
+        precision=_lib.PRECISIONS[precision], heads=heads, key_dim=key_dim, value_dim=value_dim,
+        sequences=sequences, length=length, q=q, k=k, v=v, out=_address(out), decay=_address(decay), scale=scale,
+        num_slots=num_slots if slots is not None else 0, lengths=_address(lengths), slots=_address(slots),
+        state_in=_address(state_in), state_out=_address(state_out), **st)
+
+
+def linear_attention_noalloc(eng: Engine, desc: _lib.ZjaiLinearAttentionDesc) -> None:
+    """``zjai_linear_attention_noalloc``: enqueued on the engine's stream."""
+    check(lib().zjai_linear_attention_noalloc(eng.handle, desc), eng.handle)
+
+
+def linear_attention_step(eng: Engine, desc: _lib.ZjaiLinearAttentionDesc) -> None:
+    """``zjai_linear_attention_step``: enqueued on the engine's stream."""
+    check(lib().zjai_linear_attention_step(eng.handle, desc), eng.handle)
+
+
+# ---------------------------------------------- the join of two blocks: norms, gate, residual
+def norm_gate_residual(eng: Engine, x: BTensor, y: BTensor, gate: BTensor | None = None, *,
+                       gate_act: str = "linear", post_norm: str = "none", post_groups: int = 1,
+                       post_eps: float = 1e-5, post_weight=None, post_bias=None, residual_scale=None,
+                       pre_norm: str = "none", pre_eps: float = 1e-5, pre_weight=None, pre_bias=None):
+    """``x + residual_scale * (post_norm(y) * gate_act(gate))`` and ``pre_norm`` of it
+    (``zjai_norm_gate_residual``): returns ``(x_out, h)``, h None without a pre_norm."""
+    ox, oh = ctypes.c_void_p(), ctypes.c_void_p()
+    vec = [_f32(a) for a in (post_weight, post_bias, residual_scale, pre_weight, pre_bias)]
+    if any(a is not None and a.shape != (x.c,) for a in vec):
+        raise HipError(_lib.E_INVALID_ARGUMENT, "norm / gate / residual: weights of other than the channels' size")
+    check(lib().zjai_norm_gate_residual(
+        eng.handle, x._h, y._h, gate._h if gate else None, _lib.GATES[gate_act], _lib.NORMS[post_norm],
+        post_groups, post_eps, _fp(vec[0]), _fp(vec[1]), _fp(vec[2]), _lib.NORMS[pre_norm], pre_eps,
+        _fp(vec[3]), _fp(vec[4]), ctypes.byref(ox), ctypes.byref(oh)), eng.handle)
+    return BTensor(eng, ox), BTensor(eng, oh) if oh else None
+
+
+def norm_gate_residual_desc(precision: str, x, y, gate, x_out, h, *, positions: int, channels: int,
+                            gate_act: str = "linear", post_norm: str = "none", post_groups: int = 1,
+                            post_eps: float = 1e-5, post_weight=None, post_bias=None, residual_scale=None,
+                            pre_norm: str = "none", pre_eps: float = 1e-5, pre_weight=None, pre_bias=None,
+                            **strides) -> _lib.ZjaiNormGateResidualDesc:
+    """A descriptor for ``norm_gate_residual_noalloc`` over device buffers (addresses, or objects
+    with ``data_ptr()``, which the caller keeps alive), dense unless ``strides`` (``x_stride=...``)
+    says otherwise."""
+    st = {n + "_stride": channels for n in ("x", "y", "gate", "x_out", "h")}
+    st.update(strides)
+    return _lib.ZjaiNormGateResidualDesc(
+        precision=_lib.PRECISIONS[precision], channels=channels, positions=positions, x=_address(x), y=_address(y),
+        gate=_address(gate), x_out=_address(x_out), h=_address(h), gate_act=_lib.GATES[gate_act],
+        post_norm=_lib.NORMS[post_norm], post_groups=post_groups, pre_norm=_lib.NORMS[pre_norm],
+        post_eps=post_eps, pre_eps=pre_eps, post_weight=_address(post_weight), post_bias=_address(post_bias),
+        residual_scale=_address(residual_scale), pre_weight=_address(pre_weight), pre_bias=_address(pre_bias), **st)
+
+
+def norm_gate_residual_noalloc(eng: Engine, desc: _lib.ZjaiNormGateResidualDesc) -> None:
+    """``zjai_norm_gate_residual_noalloc``: enqueued on the engine's stream."""
+    check(lib().zjai_norm_gate_residual_noalloc(eng.handle, desc), eng.handle)
