@@ -561,13 +561,31 @@ void check_linear_dims(int heads, int dk, int dv) {
         throw Error(ZJAI_E_UNSUPPORTED, "linear attention: more than 128 key or 1024 value channels per head");
 }
 
-void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype) {
+void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype, bool recurrent = false) {
     const double n = (double)a.seqs * a.length, hs = (double)a.heads * a.dk * a.dv;
     const double bytes = n * a.heads * dtype_size(dtype) * (2.0 * a.dk + 2.0 * a.dv) +
                          4.0 * a.seqs * hs * ((a.s_in != nullptr) + (a.s_out != nullptr));
-    if (linear_recurrent_groups(a) > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
-    LaunchScope sc(C, linear_recurrent_name(a, dtype), 4.0 * n * hs, bytes);
-    ZJAI_HIP(launch_linear_recurrent(a, dtype, C.stream));
+    const double flops = 4.0 * n * hs;
+    if (recurrent || linear_prefers_recurrent(a)) {
+        if (linear_recurrent_groups(a) > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
+        LaunchScope sc(C, linear_recurrent_name(a, dtype), flops, bytes);
+        ZJAI_HIP(launch_linear_recurrent(a, dtype, C.stream));
+        return;
+    }
+    const LinChunkPlan p = linear_chunk_plan(a, ZJAI_NOALLOC_SCRATCH_BYTES);
+    if ((double)a.seqs * p.segments * p.groups > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
+    float* scratch = (float*)C.top().scratch;
+    const double states = 4.0 * a.seqs * (p.segments - 1) * p.units * p.width * p.width;
+    if (p.segments > 1) {
+        LaunchScope sc(C, linear_chunk_name(p, dtype, false), 2.0 * n * hs, n * a.heads * dtype_size(dtype) * (a.dk + a.dv) + states);
+        ZJAI_HIP(launch_linear_sums(a, p, dtype, scratch, C.stream));
+    }
+    if (p.segments > 2) {
+        LaunchScope sc(C, "k_linear_scan", 2.0 * states / 4, 2.0 * states);
+        ZJAI_HIP(launch_linear_scan(a, p, scratch, C.stream));
+    }
+    LaunchScope sc(C, linear_chunk_name(p, dtype, true), flops, bytes + states);
+    ZJAI_HIP(launch_linear_outputs(a, p, dtype, scratch, C.stream));
 }
 
 // The descriptor's buffers; `step`: the recurrent form's rules.
@@ -695,7 +713,7 @@ extern "C" int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_a
     return guard(ctx, [&] {
         const OnDevice on(ctx->c.device);
         const LinAttnArgs a = linear_args(*desc, true);
-        if (a.seqs > 0) run_linear_attention(ctx->c, a, desc->precision);
+        if (a.seqs > 0) run_linear_attention(ctx->c, a, desc->precision, true);
     });
 }
 

@@ -148,6 +148,19 @@ struct LinAttnArgs {
     float* s_out;
 };
 constexpr int LIN_MAX_KEY = 128, LIN_MAX_VALUE = 1024;
+// The chunked form: `segments` stretches of each sequence (a multiple of 32 positions each, the last one shorter)
+// run side by side; with more than one, `scratch` holds linear_scratch_bytes.
+struct LinChunkPlan {
+    int segments = 1, seg_len = 0;
+    int width = 32;        // key and value channels of a unit: 32, 64 or 128
+    int units = 0, groups = 0;  // units of a sequence, workgroups that hold them
+};
+LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes);
+bool linear_prefers_recurrent(const LinAttnArgs& a);
+std::string linear_chunk_name(const LinChunkPlan& p, int dtype, bool outputs);
+hipError_t launch_linear_sums(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, float* scratch, hipStream_t s);
+hipError_t launch_linear_scan(const LinAttnArgs& a, const LinChunkPlan& p, float* scratch, hipStream_t s);
+hipError_t launch_linear_outputs(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, const float* scratch, hipStream_t s);
 // The recurrent form: a workgroup keeps its part of a state in registers over the positions.
 long long linear_recurrent_groups(const LinAttnArgs& a);
 std::string linear_recurrent_name(const LinAttnArgs& a, int dtype);
