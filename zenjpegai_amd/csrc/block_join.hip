@@ -1,6 +1,13 @@
 // The join of two residual blocks (gfx950 / CDNA4, wave64), position by position:
 //   x_out = x + scale * (post_norm(y) * act(gate)),   h = pre_norm(x_out),
 // post_norm in groups of channels, statistics and intermediate values in f32, one rounding each.
+//
+// HBM bound: five arrays pass once (x, y, gate in, x_out, h out). A position belongs to a team of TP lanes
+// (a power of two), a lane to the vectors lane + TP i of its channels, so the five weight vectors
+// are loaded once and stay in registers over the positions a team walks through; a position's whole
+// arithmetic runs on registers. The next position's loads are issued before this one's sums.
+
+#include <algorithm>
 
 #include "ops.h"
 
@@ -14,94 +21,284 @@ __device__ __forceinline__ long long join_at(const JoinRows& r, int width, long 
     return y * r.row + (i - y * width) * r.pos;
 }
 
+// exp(-g) by the hardware's 2^x: relative error (|g| + 2) 2^-24, as the rounding of g log2 e leaves any.
 __device__ __forceinline__ float gate_value(float g, int act) {
     if (act == GATE_LINEAR) return g;
-    const float d = 1.0f + expf(-g);
-    return act == GATE_SIGMOID ? 1.0f / d : g / d;
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f));
+    return act == GATE_SIGMOID ? s : g * s;
 }
 
-// Sum over the workgroup's 256 threads.
-__device__ __forceinline__ float block_sum(float v, float* s_red) {
+// How a team sums over groups of channels: all of a position; groups of 2^k lanes; or, for every other
+// size, lane exchanges over the 2^k lanes that divide a group and LDS for the rest.
+enum SumMode : int { SUM_ALL = 0, SUM_LANES = 1, SUM_LDS = 2 };
+
+struct JoinPlan {
+    int tp, threads, mode, group_vecs, lanes;  // group_vecs: vectors of a group; lanes: 2^k of SUM_LANES / SUM_LDS
+};
+
+template <int NV>
+struct TeamSum {
+    int tid, lane, tp, threads, team0;  // team0: the team's first thread
+    float* s_red;
+
+    // Of the whole team's values; every lane gets it.
+    __device__ __forceinline__ float all(const float (&v)[NV]) const {
+        float s = v[0];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-}
-
-// Mean (0 for RMS) and 1 / sqrt(variance + eps) of the n values at s.
-__device__ __forceinline__ void norm_stats(const float* s, int n, int kind, float eps, float* s_red, float* mean, float* inv) {
-    float m = 0.0f;
-    if (kind == NORM_LAYER) {
-        for (int c = threadIdx.x; c < n; c += 256) m += s[c];
-        m = block_sum(m, s_red) / (float)n;
+        for (int i = 1; i < NV; ++i) s += v[i];
+        const int in_wave = min(tp, 64);
+        for (int off = 1; off < in_wave; off <<= 1) s += __shfl_xor(s, off);
+        if (tp > 64) {
+            __syncthreads();
+            if ((tid & 63) == 0) s_red[tid >> 6] = s;
+            __syncthreads();
+            s = 0.0f;
+            for (int w = team0 >> 6; w < (team0 + tp) >> 6; ++w) s += s_red[w];
+        }
+        return s;
     }
-    float q = 0.0f;
-    for (int c = threadIdx.x; c < n; c += 256) q = fmaf(s[c] - m, s[c] - m, q);
-    *mean = m;
-    *inv = 1.0f / sqrtf(block_sum(q, s_red) / (float)n + eps);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) k_join(JoinArgs a) {
-    extern __shared__ float s_v[];
-    __shared__ float s_red[4];
-    const long long i = blockIdx.x;
-    const int C = a.channels, tid = threadIdx.x;
-    const T* x = (const T*)a.x.p + join_at(a.x, a.width, i);
-    const T* y = (const T*)a.y.p + join_at(a.y, a.width, i);
-    const T* g = a.g.p ? (const T*)a.g.p + join_at(a.g, a.width, i) : nullptr;
-    T* xo = (T*)a.xo.p + join_at(a.xo, a.width, i);
-    T* h = a.h.p ? (T*)a.h.p + join_at(a.h, a.width, i) : nullptr;
-    for (int c = tid; c < C; c += 256) s_v[c] = to_f32(y[c]);
-    __syncthreads();
-    const int per = C / a.groups;
-    for (int k = 0; k < a.groups; ++k) {
-        float m = 0.0f, inv = 1.0f;
-        if (a.post != NORM_NONE) norm_stats(s_v + k * per, per, a.post, a.post_eps, s_red, &m, &inv);
+    // v[i]: of the group that vector i belongs to.
+    __device__ __forceinline__ void groups(float (&v)[NV], const JoinPlan& p) const {
+        if (p.mode == SUM_ALL) {
+            const float s = all(v);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = s;
+            return;
+        }
+        for (int off = 1; off < p.lanes; off <<= 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], off);
+        if (p.mode == SUM_LANES) return;
         __syncthreads();
-        for (int c = k * per + tid; c < (k + 1) * per; c += 256) {
-            float u = s_v[c];
-            if (a.post != NORM_NONE) u = (u - m) * inv;
-            if (a.post_w) u *= a.post_w[c];
-            if (a.post_b) u += a.post_b[c];
-            if (g) u *= gate_value(to_f32(g[c]), a.gate);
-            if (a.scale) u *= a.scale[c];
-            s_v[c] = to_f32(x[c]) + u;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if ((tid & (p.lanes - 1)) == 0) s_red[i * threads + tid] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int first = (lane + tp * i) / p.group_vecs * p.group_vecs;
+            float s = 0.0f;
+            if (first < tp * NV)
+                for (int k = first; k < min(first + p.group_vecs, tp * NV); k += p.lanes)
+                    s += s_red[k / tp * threads + team0 + (k & (tp - 1))];
+            v[i] = s;
         }
     }
-    __syncthreads();
-    float m = 0.0f, inv = 1.0f;
-    if (h) norm_stats(s_v, C, a.pre, a.pre_eps, s_red, &m, &inv);
-    for (int c = tid; c < C; c += 256) {
-        const float v = s_v[c];
-        xo[c] = from_f32<T>(v);
-        if (h) {
-            float u = (v - m) * inv;
-            if (a.pre_w) u *= a.pre_w[c];
-            if (a.pre_b) u += a.pre_b[c];
-            h[c] = from_f32<T>(u);
+};
+
+template <typename T, int VE> struct alignas(sizeof(T) * VE) JoinVec { T e[VE]; };
+
+// PRE, GATE: whether h and the gate are there.
+template <typename T, int VE, int NV, bool PRE, bool GATE>
+__global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
+    typedef JoinVec<T, VE> V;
+    extern __shared__ float s_red[];
+    const int tid = threadIdx.x, lane = tid & (p.tp - 1), team = tid / p.tp, teams = p.threads / p.tp;
+    const TeamSum<NV> sum{tid, lane, p.tp, p.threads, team * p.tp, s_red};
+    const int C = a.channels;
+    // Eight channels' weights stay in registers; sixteen channels' are read again for each position.
+    constexpr bool KEEP = NV * VE <= 8;
+    bool on[NV];
+    float pw[NV][VE], pb[NV][VE], sc[NV][VE], nw[NV][VE], nb[NV][VE];
+    const auto weight = [&](const float* w, int i, int e, float absent) {
+        return w && on[i] ? w[(lane + p.tp * i) * VE + e] : absent;
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        on[i] = (lane + p.tp * i) * VE < C;
+        if (!KEEP) continue;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            pw[i][e] = weight(a.post_w, i, e, 1.0f);
+            pb[i][e] = weight(a.post_b, i, e, 0.0f);
+            sc[i][e] = weight(a.scale, i, e, 1.0f);
+            nw[i][e] = weight(PRE ? a.pre_w : nullptr, i, e, 1.0f);
+            nb[i][e] = weight(PRE ? a.pre_b : nullptr, i, e, 0.0f);
+        }
+    }
+    const float inv_group = 1.0f / (float)(C / a.groups), inv_all = 1.0f / (float)C;
+
+    V x[NV], y[NV], g[NV];
+    const auto fetch = [&](long long at) {
+        const bool ok = at < a.positions;
+        const T* px = (const T*)a.x.p + (ok ? join_at(a.x, a.width, at) : 0);
+        const T* py = (const T*)a.y.p + (ok ? join_at(a.y, a.width, at) : 0);
+        const T* pg = GATE ? (const T*)a.g.p + (ok ? join_at(a.g, a.width, at) : 0) : nullptr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = on[i] ? (lane + p.tp * i) * VE : 0;  // always a channel that exists
+            x[i] = *(const V*)(px + c);
+            y[i] = *(const V*)(py + c);
+            if (GATE) g[i] = *(const V*)(pg + c);
+        }
+    };
+    const long long step = (long long)gridDim.x * teams;
+    long long base = (long long)blockIdx.x * teams;
+    if (base < a.positions) fetch(base + team);
+    for (; base < a.positions; base += step) {
+        const long long at = base + team;
+        float u[NV][VE], v[NV][VE];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                u[i][e] = to_f32(y[i].e[e]);
+                v[i][e] = to_f32(x[i].e[e]);
+            }
+        if (a.post != NORM_NONE) {
+            float s[NV];
+            if (a.post == NORM_LAYER) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    s[i] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) s[i] += u[i][e];
+                    s[i] = on[i] ? s[i] : 0.0f;
+                }
+                sum.groups(s, p);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) u[i][e] -= s[i] * inv_group;
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                s[i] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) s[i] = fmaf(u[i][e], u[i][e], s[i]);
+                s[i] = on[i] ? s[i] : 0.0f;
+            }
+            sum.groups(s, p);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float inv = 1.0f / sqrtf(s[i] * inv_group + a.post_eps);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) u[i][e] = u[i][e] * inv * (KEEP ? pw[i][e] : weight(a.post_w, i, e, 1.0f)) + (KEEP ? pb[i][e] : weight(a.post_b, i, e, 0.0f));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                if (GATE) u[i][e] *= gate_value(to_f32(g[i].e[e]), a.gate);
+                v[i][e] += u[i][e] * (KEEP ? sc[i][e] : weight(a.scale, i, e, 1.0f));
+            }
+        fetch(at + step);
+        if (at < a.positions) {
+            T* po = (T*)a.xo.p + join_at(a.xo, a.width, at);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                V o;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(v[i][e]);
+                if (on[i]) *(V*)(po + (lane + p.tp * i) * VE) = o;
+            }
+        }
+        if (!PRE) continue;
+        float s[NV], mean = 0.0f;
+        if (a.pre == NORM_LAYER) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                s[i] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) s[i] += v[i][e];
+                s[i] = on[i] ? s[i] : 0.0f;
+            }
+            mean = sum.all(s) * inv_all;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            s[i] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                v[i][e] -= mean;
+                s[i] = fmaf(v[i][e], v[i][e], s[i]);
+            }
+            s[i] = on[i] ? s[i] : 0.0f;
+        }
+        const float inv = 1.0f / sqrtf(sum.all(s) * inv_all + a.pre_eps);
+        if (at < a.positions) {
+            T* ph = (T*)a.h.p + join_at(a.h, a.width, at);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                V o;
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    o.e[e] = from_f32<T>(v[i][e] * inv * (KEEP ? nw[i][e] : weight(a.pre_w, i, e, 1.0f)) +
+                                         (KEEP ? nb[i][e] : weight(a.pre_b, i, e, 0.0f)));
+                if (on[i]) *(V*)(ph + (lane + p.tp * i) * VE) = o;
+            }
         }
     }
 }
 
-template <typename T>
+// Channels a vector holds: the most, up to 16 bytes, that divide the group and keep every row aligned.
+int join_vector(const JoinArgs& a, int es) {
+    int ve = 16 / es;
+    const auto fits = [&](int v) {
+        if (a.channels / a.groups % v) return false;
+        for (const JoinRows* r : {&a.x, &a.y, &a.g, &a.xo, &a.h})
+            if (r->p && (((uintptr_t)r->p % (v * es)) || r->pos % v || r->row % v)) return false;
+        return true;
+    };
+    while (ve > 1 && !fits(ve)) ve /= 2;
+    return ve;
+}
+// Channels a lane holds: eight, or sixteen where 1024 lanes of eight are too few.
+int join_lane_channels(const JoinArgs& a) { return a.channels <= 8192 ? 8 : 16; }
+
+JoinPlan join_plan(const JoinArgs& a, int ve, int per_lane) {
+    JoinPlan p{};
+    p.tp = 1;
+    while (p.tp * per_lane < a.channels) p.tp *= 2;
+    p.threads = std::max(p.tp, 256);
+    p.group_vecs = a.channels / a.groups / ve;
+    p.lanes = 1;
+    while (p.lanes < std::min(p.tp, 64) && p.group_vecs % (2 * p.lanes) == 0) p.lanes *= 2;
+    p.mode = a.groups == 1 ? SUM_ALL : p.group_vecs == p.lanes ? SUM_LANES : SUM_LDS;
+    return p;
+}
+
+template <typename T, int VE, int NV>
 hipError_t join(const JoinArgs& a, hipStream_t s) {
-    k_join<T><<<dim3((unsigned)a.positions), 256, sizeof(float) * a.channels, s>>>(a);
+    const JoinPlan p = join_plan(a, VE, VE * NV);
+    const int teams = p.threads / p.tp;
+    // Four workgroups of 256 lanes to a CU: registers hold four waves to a SIMD.
+    const long long blocks = std::min((a.positions + teams - 1) / teams, (long long)256 * 4 * 256 / p.threads);
+    const dim3 grid((unsigned)blocks), block((unsigned)p.threads);
+    const size_t lds = sizeof(float) * (p.mode == SUM_LDS ? std::max(NV * p.threads, 16) : 16);
+    if (a.h.p && a.g.p) k_join<T, VE, NV, true, true><<<grid, block, lds, s>>>(a, p);
+    else if (a.h.p) k_join<T, VE, NV, true, false><<<grid, block, lds, s>>>(a, p);
+    else if (a.g.p) k_join<T, VE, NV, false, true><<<grid, block, lds, s>>>(a, p);
+    else k_join<T, VE, NV, false, false><<<grid, block, lds, s>>>(a, p);
     return hipGetLastError();
+}
+template <typename T, int VE>
+hipError_t join_lanes(const JoinArgs& a, hipStream_t s) {
+    return join_lane_channels(a) == 8 ? join<T, VE, 8 / VE>(a, s) : join<T, VE, 16 / VE>(a, s);
+}
+template <typename T>
+hipError_t join_of(const JoinArgs& a, hipStream_t s) {
+    const int ve = join_vector(a, sizeof(T));
+    if constexpr (sizeof(T) == 2)
+        if (ve == 8) return join_lanes<T, 8>(a, s);
+    if (ve == 4) return join_lanes<T, 4>(a, s);
+    if (ve == 2) return join_lanes<T, 2>(a, s);
+    return join_lanes<T, 1>(a, s);
 }
 
 }  // namespace
 
 std::string join_name(const JoinArgs& a, int dtype) {
-    return std::string("k_join<") + (dtype == DT_F32 ? "float" : dtype == DT_F16 ? "_Float16" : "__bf16") + ">";
+    const int ve = join_vector(a, dtype == DT_F32 ? 4 : 2);
+    return std::string("k_join<") + (dtype == DT_F32 ? "float" : dtype == DT_F16 ? "_Float16" : "__bf16") + ", " + std::to_string(ve) +
+           ", " + std::to_string(join_lane_channels(a) / ve) + (a.h.p ? ", true" : ", false") + (a.g.p ? ", true>" : ", false>");
 }
 
 hipError_t launch_join(const JoinArgs& a, int dtype, hipStream_t s) {
-    if (dtype == DT_F32) return join<float>(a, s);
-    if (dtype == DT_F16) return join<_Float16>(a, s);
-    return join<__bf16>(a, s);
+    if (dtype == DT_F32) return join_of<float>(a, s);
+    if (dtype == DT_F16) return join_of<_Float16>(a, s);
+    return join_of<__bf16>(a, s);
 }
 
 }  // namespace zjai
