@@ -187,31 +187,26 @@ const char* type_name(int dtype) { return dtype == DT_F32 ? "float" : dtype == D
 // tiles under one another are the K slots {4 g + r, 16 + 4 g + r} of the next product's operand, and
 // the other operand is read in the same order (q stored so, k^T and v through the transposing LDS read).
 //
-// Every value enters the matrix cores as bf16 pieces whose sum it is: one for bf16, two for f16 and three for
-// f32 inputs (exact). What is computed in f32 is split likewise: the weighted values three ways (the
-// state's sums keep f32 accuracy), the query products and the state in front of an output that is
-// rounded to 16 bits two ways (2^-16 of them), with f32 outputs three ways. Products of pieces below
-// 2^-16 (16-bit outputs) or 2^-23 of the whole are left out.
+// f32 runs on the f32 MFMAs (16x16x4; the same slots, one register at a time). The 16-bit types run on
+// 16x16x32 MFMAs, q.k on the stored values themselves. What is computed in f32 enters the matrix cores in pieces:
+//  - the query products and the state, in front of an output that is rounded to 16 bits, as two bf16
+//    pieces (2^-16 of them; bf16 has f32's range, which f16 q.k or states can leave), and so do the f16
+//    values they meet (exactly: 11 bits);
+//  - the weighted values g^(31-j) v_j, which the state's f32 sums are made of, as three bf16 pieces next to
+//    bf16 keys (exactly), and next to f16 keys as two f16 ones, the second times 2^11 in a sum of its own
+//    (2^-23 of them; |g^n v| <= |v| stays in f16's range).
 constexpr int LC = 32;
 
-template <typename T> struct LinPieces;
-template <> struct LinPieces<__bf16> { static constexpr int in = 1, mid = 2; };
-template <> struct LinPieces<_Float16> { static constexpr int in = 2, mid = 2; };
-template <> struct LinPieces<float> { static constexpr int in = 3, mid = 3; };
-
-__device__ u32x4 g_lin_zero[1];  // 16 zero bytes: the source of absent positions and channels
+__device__ u32x4 g_lin_zero[2];  // zeros: the source of absent positions and channels
 
 // g^n for n >= 0, l2 = log2 g (-inf for g = 0).
 __device__ __forceinline__ float lin_pow(float l2, int n) { return n == 0 ? 1.0f : exp2f((float)n * l2); }
 
-// LDS rows of D bf16 in 16-byte units, XORed by row: the 16 rows of a b128 fragment read (q) and the 8
-// rows by 2 units of a transposing read or the 16 rows of a b64 read (k, v) fall on distinct banks.
-template <int D> __device__ __forceinline__ int swz_q(int row) {
-    return D == 128 ? row & 15 : D == 64 ? (row >> 1) & 7 : ((row >> 2) & 1) << 1;
-}
-template <int D> __device__ __forceinline__ int swz_kv(int row) {
-    return (D == 128 ? (row & 7) << 1 : D == 64 ? ((row >> 1) & 3) << 1 : ((row >> 2) & 1) << 1) | ((row >> 3) & 1);
-}
+// LDS rows: 16-bit ones are padded by 32 bytes, which puts the 16 rows of a b128 fragment read (q) and the 8 rows by 2
+// units of a transposing read (k, v) on distinct banks; f32 ones by 16, which does it for rows r and
+// r + 4 of a column read and all but a pair of the rows of a b128 read. (An XOR by row has no conflicts at
+// all, but every address is then an instruction and a register of its own.)
+template <typename T> __host__ __device__ constexpr int lin_row(int d) { return d + (sizeof(T) == 4 ? 4 : 16); }
 
 // The bf16 pieces of eight values: p0 cut off (so that a finite value's is finite), the others rounded.
 template <int N>
@@ -231,42 +226,78 @@ __device__ __forceinline__ void lin_split(const float (&x)[8], u32x4 (&p)[N]) {
     }
 }
 
-// c[i][j] += a[i] b[j] over the products of pieces p + q <= LIM, the small ones first (two tiles of either operand).
-// Inline assembly with the accumulators in place: the compiler renames the builtin's chains back to
-// back. The block carries its own wait states, as split.h's.
-#define LM(i, j, p, q) ZJAI_MF "%[c" #i #j "], %[a" #i #p "], %[b" #j #q "], %[c" #i #j "]\n\t"
-#define LM4(p, q) LM(0, 0, p, q) LM(0, 1, p, q) LM(1, 0, p, q) LM(1, 1, p, q)
+// c[i][j] += a[i] b[j] over the products of pieces p + q <= 1 (up to 2 with three), the small ones first (two
+// tiles of either operand; zero: the sums start here, a constant where this is inlined). Inline
+// assembly with the accumulators in place: the compiler renames the builtin's chains back to back. The
+// block carries its own wait states, as split.h's.
+#define LM(MF, i, j, p, q) MF "%[c" #i #j "], %[a" #i #p "], %[b" #j #q "], %[c" #i #j "]\n\t"
+#define LZ(MF, i, j, p, q) MF "%[c" #i #j "], %[a" #i #p "], %[b" #j #q "], 0\n\t"
+#define LM4(MF, p, q) LM(MF, 0, 0, p, q) LM(MF, 0, 1, p, q) LM(MF, 1, 0, p, q) LM(MF, 1, 1, p, q)
+#define LZ4(MF, p, q) LZ(MF, 0, 0, p, q) LZ(MF, 0, 1, p, q) LZ(MF, 1, 0, p, q) LZ(MF, 1, 1, p, q)
 #define LC4 [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1])
+#define LO4 [c00] "=&v"(c[0][0]), [c01] "=&v"(c[0][1]), [c10] "=&v"(c[1][0]), [c11] "=&v"(c[1][1])
 #define LA(p) [a0##p] "v"(a[0][p]), [a1##p] "v"(a[1][p])
 #define LB(p) [b0##p] "v"(b[0][p]), [b1##p] "v"(b[1][p])
-template <int LIM, int NA, int NB>
-__device__ __forceinline__ void lin_mma(f32x4 (&c)[2][2], const u32x4 (&a)[2][NA], const u32x4 (&b)[2][NB]) {
+#define LIN_ASM(MF, WAIT, P, Q, REST, ...)                                              \
+    if (zero) asm("s_nop 1\n\t" LZ4(MF, P, Q) REST WAIT : LO4 : __VA_ARGS__);            \
+    else asm("s_nop 1\n\t" LM4(MF, P, Q) REST WAIT : LC4 : __VA_ARGS__);
+template <int NA, int NB>
+__device__ __forceinline__ void lin_mma(f32x4 (&c)[2][2], const u32x4 (&a)[2][NA], const u32x4 (&b)[2][NB], bool zero = false) {
     if constexpr (NA == 1 && NB == 1) {
-        asm("s_nop 1\n\t" LM4(0, 0) ZJAI_WAIT : LC4 : LA(0), LB(0));
+        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 0, 0, , LA(0), LB(0))
     } else if constexpr (NA == 1 && NB == 2) {
-        asm("s_nop 1\n\t" LM4(0, 1) LM4(0, 0) ZJAI_WAIT : LC4 : LA(0), LB(0), LB(1));
+        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 0, 1, LM4(ZJAI_MF, 0, 0), LA(0), LB(0), LB(1))
     } else if constexpr (NA == 2 && NB == 1) {
-        asm("s_nop 1\n\t" LM4(1, 0) LM4(0, 0) ZJAI_WAIT : LC4 : LA(0), LA(1), LB(0));
+        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 1, 0, LM4(ZJAI_MF, 0, 0), LA(0), LA(1), LB(0))
     } else if constexpr (NA == 1 && NB == 3) {
-        asm("s_nop 1\n\t" LM4(0, 2) LM4(0, 1) LM4(0, 0) ZJAI_WAIT : LC4 : LA(0), LB(0), LB(1), LB(2));
-    } else if constexpr (NA == 2 && NB == 2 && LIM == 1) {
-        asm("s_nop 1\n\t" LM4(1, 0) LM4(0, 1) LM4(0, 0) ZJAI_WAIT : LC4 : LA(0), LA(1), LB(0), LB(1));
-    } else if constexpr (NA == 2 && NB == 3 && LIM == 2) {
-        asm("s_nop 1\n\t" LM4(1, 1) LM4(0, 2) LM4(1, 0) LM4(0, 1) LM4(0, 0) ZJAI_WAIT : LC4 : LA(0), LA(1), LB(0), LB(1), LB(2));
+        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 0, 2, LM4(ZJAI_MF, 0, 1) LM4(ZJAI_MF, 0, 0), LA(0), LB(0), LB(1), LB(2))
     } else {
-        static_assert(NA == 3 && NB == 3 && LIM == 2, "piece products");
-        asm("s_nop 1\n\t" LM4(2, 0) LM4(1, 1) LM4(0, 2) LM4(1, 0) LM4(0, 1) LM4(0, 0) ZJAI_WAIT
-            : LC4 : LA(0), LA(1), LA(2), LB(0), LB(1), LB(2));
+        static_assert(NA == 2 && NB == 2, "piece products");
+        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 1, 0, LM4(ZJAI_MF, 0, 1) LM4(ZJAI_MF, 0, 0), LA(0), LA(1), LB(0), LB(1))
     }
 }
+#define LIN_F16 "v_mfma_f32_16x16x32_f16 "
+__device__ __forceinline__ void lin_mma_f16(f32x4 (&c)[2][2], const u32x4 (&a)[2][1], const u32x4 (&b)[2][1], bool zero = false) {
+    LIN_ASM(LIN_F16, ZJAI_WAIT, 0, 0, , LA(0), LB(0))
+}
+// The f32 form: sixteen (a tile's four K slots, one register each) or, with TRI, the twelve but c[1][0]'s.
+#define LIN_F32 "v_mfma_f32_16x16x4_f32 "
+#define LIN_F32_WAIT "s_nop 9"
+#define LM3(MF, p, q) LM(MF, 0, 0, p, q) LM(MF, 0, 1, p, q) LM(MF, 1, 1, p, q)
+template <bool TRI>
+__device__ __forceinline__ void lin_mma_f32(f32x4 (&c)[2][2], const f32x4 (&a)[2], const f32x4 (&b)[2], bool zero = false) {
+    if constexpr (TRI) {
+        if (zero) c[0][0] = c[0][1] = c[1][0] = c[1][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        asm("s_nop 1\n\t" LM3(LIN_F32, 0, 0) LM3(LIN_F32, 1, 1) LM3(LIN_F32, 2, 2) LM3(LIN_F32, 3, 3) LIN_F32_WAIT
+            : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c11] "+v"(c[1][1])
+            : LA(0), LA(1), LA(2), LA(3), LB(0), LB(1), LB(2), LB(3));
+    } else {
+        LIN_ASM(LIN_F32, LIN_F32_WAIT, 0, 0, LM4(LIN_F32, 1, 1) LM4(LIN_F32, 2, 2) LM4(LIN_F32, 3, 3), LA(0), LA(1), LA(2), LA(3), LB(0),
+                LB(1), LB(2), LB(3))
+    }
+}
+// c[n] += a[n] b: the values of the later sixteen positions, which only the later sixteen queries see.
+__device__ __forceinline__ void lin_mma_f32_late(f32x4& c0, f32x4& c1, const f32x4 (&a)[2], const f32x4& b) {
+    asm("s_nop 1\n\t" LIN_F32 "%0, %2, %10, %0\n\t" LIN_F32 "%1, %6, %10, %1\n\t" LIN_F32 "%0, %3, %11, %0\n\t" LIN_F32
+        "%1, %7, %11, %1\n\t" LIN_F32 "%0, %4, %12, %0\n\t" LIN_F32 "%1, %8, %12, %1\n\t" LIN_F32 "%0, %5, %13, %0\n\t" LIN_F32
+        "%1, %9, %13, %1\n\t" LIN_F32_WAIT
+        : "+v"(c0), "+v"(c1)
+        : "v"(a[0][0]), "v"(a[0][1]), "v"(a[0][2]), "v"(a[0][3]), "v"(a[1][0]), "v"(a[1][1]), "v"(a[1][2]), "v"(a[1][3]), "v"(b[0]),
+          "v"(b[1]), "v"(b[2]), "v"(b[3]));
+}
+#undef LM3
+#undef LIN_ASM
 #undef LB
 #undef LA
+#undef LO4
 #undef LC4
+#undef LZ4
 #undef LM4
+#undef LZ
 #undef LM
 
 // Eight channels of one position as loaded.
-template <typename T> struct LinUnit { u32x4 v[sizeof(T) / 2]; };
+template <typename T> struct alignas(16) LinUnit { u32x4 v[sizeof(T) / 2]; };
 
 // Channels 8 u .. 8 u + 7 of a head at `p` (d channels), zeros where absent. VEC: whole 16-byte loads.
 template <typename T>
@@ -292,22 +323,21 @@ __device__ __forceinline__ LinUnit<T> lin_load(const T* p, int c0, int d, bool v
     return r;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void lin_pieces(const LinUnit<T>& u, u32x4 (&p)[N]) {
-    if constexpr (N == 1) {
-        p[0] = u.v[0];
-    } else {
-        float x[8];
-        constexpr int E = 16 / sizeof(T);
-        typedef T tE __attribute__((ext_vector_type(E)));
+// An f16 pair of f32 values' halves.
+__device__ __forceinline__ unsigned pack_f16(float a, float b) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    f16x2 r;
+    r[0] = (_Float16)a;
+    r[1] = (_Float16)b;
+    return __builtin_bit_cast(unsigned, r);
+}
+// Eight f16 or bf16 values as f32.
+template <typename T>
+__device__ __forceinline__ void lin_floats(const u32x4& v, float (&x)[8]) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const t8 t = __builtin_bit_cast(t8, v);
 #pragma unroll
-        for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
-            const tE t = __builtin_bit_cast(tE, u.v[h]);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[h * E + e] = (float)t[e];
-        }
-        lin_split<N>(x, p);
-    }
+    for (int e = 0; e < 8; ++e) x[e] = (float)t[e];
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -320,73 +350,49 @@ __device__ __forceinline__ u32x2 lds_tr(const unsigned short* p) {
 struct LinChunkArgs {
     LinAttnArgs a;
     float* scratch;  // sums: the state after each segment; outputs: before each but the first
-    int segments, seg_len, units, groups, tiles;
+    int segments, seg_len, units, groups, teams, tiles;
     int vec_k, vec_v, vec_o;
+    int even;  // vec_k and vec_v, and head sizes of whole units
+    int fold;  // outputs: join the segments' sums in place of a scan
 };
+
+// 16-bit planes of a chunk in LDS: k, v and, for outputs, q (f16's in pieces too).
+template <typename T> __host__ __device__ constexpr int lin_lds_planes(bool out) {
+    return sizeof(T) == 4 ? (out ? 6 : 4) : Elem<T>::dt == DT_F16 ? (out ? 5 : 2) : (out ? 3 : 2);
+}
 
 template <typename T, int WV, bool OUT>
 __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
-    constexpr int D = 32 * WV, TT = 64 * WV, TEAMS = 4 / WV, NP = LinPieces<T>::in, NM = LinPieces<T>::mid;
-    constexpr int LIM = NM - 1;               // products of the outputs
-    constexpr int PLANE = LC * D;             // one piece of q, k or v
+    constexpr bool F32 = sizeof(T) == 4, F16 = Elem<T>::dt == DT_F16;
+    constexpr int D = 32 * WV, TT = 64 * WV;
+    constexpr int ROW = lin_row<T>(D), PLANE = LC * ROW;  // LDS values of a position and of a chunk of q, k or v
     constexpr int MT = D / 16, KS = D / 32;
-    constexpr int NMAT = OUT ? 3 : 2;
-    __shared__ __attribute__((aligned(16))) unsigned short s_lds[TEAMS * NMAT * NP * PLANE];
+    constexpr int QP = F16 ? 2 : 1;           // bf16 pieces of a 16-bit q or v
+    extern __shared__ __attribute__((aligned(16))) unsigned short s_lds[];  // [teams][lin_lds_planes][PLANE]
     const LinAttnArgs& a = c.a;
     const int team = threadIdx.x / TT, t = threadIdx.x % TT, wave = t >> 6, lane = t & 63, l16 = lane & 15, g = lane >> 4;
-    unsigned short* s_k = s_lds + team * NMAT * NP * PLANE;
-    unsigned short* s_v = s_k + NP * PLANE;
-    unsigned short* s_q = s_v + NP * PLANE;
+    unsigned short* s_k = s_lds + team * lin_lds_planes<T>(OUT) * PLANE;
+    unsigned short* s_v = s_k + (F32 ? 2 : 1) * PLANE;
+    unsigned short* s_q = s_v + (F32 ? 2 : 1) * PLANE;  // f16: the values, then their two pieces
+    float *f_k = (float*)s_k, *f_v = (float*)s_v, *f_q = (float*)s_q;
 
+    // Workgroups go round the eight XCDs; neighbours in (sequence, segment, group) share cache lines of the
+    // positions' channels and are put on one XCD.
     const int segs = OUT ? c.segments : c.segments - 1;
-    int b = blockIdx.x;
+    int b = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     const int group = b % c.groups;
     b /= c.groups;
     const int seg = b % segs, seq = b / segs;
+    if (seq >= a.seqs) return;
     const int len = a.lengths ? max(0, min(a.lengths[seq], a.length)) : a.length;
     const int begin = seg * c.seg_len, end = min(len, begin + c.seg_len);
     // Sums are those that a later segment starts from.
     if (OUT ? begin > len || (begin == len && seg > 0) : begin + c.seg_len >= len) return;
-    const int unit = group * TEAMS + team;
+    const int unit = group * c.teams + team;
     const bool live = unit < c.units;
     const int head = live ? unit / c.tiles : 0, col0 = live ? (unit % c.tiles) * D : 0;
     const int colw = col0 + wave * 32;        // the wave's 32 value columns
     const bool work = live && colw < a.dv;
-
-    const float l2 = log2f(a.decay[head]);
-    float w_v[8], w_o[2], w_d[4], w_n[4], g_c = lin_pow(l2, LC);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        w_v[r] = lin_pow(l2, LC - 1 - (4 * g + r));
-        w_v[4 + r] = lin_pow(l2, LC - 1 - (16 + 4 * g + r));
-        const int d = l16 - (4 * g + r);
-        w_d[r] = d >= 0 ? lin_pow(l2, d) : 0.0f;
-        w_n[r] = lin_pow(l2, 16 + d);
-    }
-    w_o[0] = lin_pow(l2, l16 + 1);
-    w_o[1] = lin_pow(l2, l16 + 17);
-
-    // The state before the segment: S[mt][n][r] is key channel 16 mt + 4 g + r of value column 16 n + l16.
-    f32x4 S[MT][2];
-    const long long sbase = ((long long)seq * a.heads + head) * a.dk;
-    const size_t xunit = (size_t)D * D;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (seg == 0) {
-                if (a.s_in && work)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int kk = 16 * m + 4 * g + r, vv = colw + 16 * n + l16;
-                        if (kk < a.dk && vv < a.dv) S[m][n][r] = a.s_in[(sbase + kk) * a.dv + vv];
-                    }
-            } else if (OUT && live) {
-                const float* x = c.scratch + (((size_t)seq * (c.segments - 1) + seg - 1) * c.units + unit) * xunit;
-                S[m][n] = *(const f32x4*)(x + (size_t)(((m * 2 + n) * WV + wave) * 64 + lane) * 4);
-            }
-        }
 
     const T* kp = (const T*)a.k.p + (long long)seq * a.k.seq + (long long)head * a.dk;
     const T* vp = (const T*)a.v.p + (long long)seq * a.v.seq + (long long)head * a.dv + col0;
@@ -398,7 +404,33 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     constexpr int UPR = D / 8;
     const int row0 = t / UPR, u = t % UPR;
     LinUnit<T> rk[2], rv[2], rq[2];
+    // Whole chunks of evenly strided rows: running pointers, those of absent channels on zeros that stay put.
+    const bool even = a.width == 0 && c.even;
+    const bool on_k = live && u * 8 < a.dk, on_v = live && u * 8 < vcols;
+    const T *pk[2], *pv[2], *pq[2];
+    const long long step_k = on_k ? LC * a.k.pos : 0, step_v = on_v ? LC * a.v.pos : 0, step_q = on_k ? LC * a.q.pos : 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const long long p = begin + row0 + i * 16;
+        pk[i] = on_k ? kp + p * a.k.pos + u * 8 : (const T*)g_lin_zero;
+        pv[i] = on_v ? vp + p * a.v.pos + u * 8 : (const T*)g_lin_zero;
+        if (OUT) pq[i] = on_k ? qp + p * a.q.pos + u * 8 : (const T*)g_lin_zero;
+    }
     const auto fetch = [&](int pos) {
+        if (even && pos + LC <= end) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                rk[i] = *(const LinUnit<T>*)pk[i];
+                rv[i] = *(const LinUnit<T>*)pv[i];
+                pk[i] += step_k;
+                pv[i] += step_v;
+                if (OUT) {
+                    rq[i] = *(const LinUnit<T>*)pq[i];
+                    pq[i] += step_q;
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int p = pos + row0 + i * 16;
@@ -409,34 +441,110 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
             if (OUT) rq[i] = lin_load<T>(qp + (y * a.q.row + x * a.q.pos), u * 8, a.dk, ok, c.vec_k);
         }
     };
+    if (begin < end) fetch(begin);
+
+    // The head's powers g^0..g^63, one a lane, then those a lane's rows and columns need.
+    float* s_pow = (float*)(s_lds + c.teams * lin_lds_planes<T>(OUT) * PLANE) + (threadIdx.x >> 6) * 64;
+    s_pow[lane] = lin_pow(log2f(a.decay[head]), lane);
+    __syncthreads();
+    float w_v[8], w_o[2], w_d[4], w_n[4], g_c = s_pow[LC];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        w_v[r] = s_pow[LC - 1 - (4 * g + r)];
+        w_v[4 + r] = s_pow[LC - 1 - (16 + 4 * g + r)];
+        const int d = l16 - (4 * g + r);
+        w_d[r] = s_pow[max(d, 0)] * a.scale;
+        w_n[r] = s_pow[16 + d] * a.scale;
+    }
+    w_o[0] = s_pow[l16 + 1] * a.scale;
+    w_o[1] = s_pow[l16 + 17] * a.scale;
+
+    // The state before the segment: S[mt][n][r] is key channel 16 mt + 4 g + r of value column 16 n + l16.
+    f32x4 S[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const long long sbase = ((long long)seq * a.heads + head) * a.dk;
+    const size_t xunit = (size_t)D * D;
+    float* const x_seq = c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * xunit + (size_t)(wave * 64 + lane) * 4;
+    const size_t x_seg = c.units * xunit;
+    if (seg == 0) {
+        if (a.s_in && work)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int kk = 16 * m + 4 * g + r, vv = colw + 16 * n + l16;
+                        const bool in = kk < a.dk && vv < a.dv;
+                        const float x = a.s_in[in ? (sbase + kk) * a.dv + vv : 0];
+                        S[m][n][r] = in ? x : 0.0f;
+                    }
+    } else if (OUT && live) {
+        if (c.fold) {
+            // Few segments: their sums are joined here, E_(s+1) = g^seg_len E_s + X_s.
+            const float gl = lin_pow(log2f(a.decay[head]), c.seg_len);
+            for (int s = 0; s < seg; ++s)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const f32x4 x = *(const f32x4*)(x_seq + s * x_seg + (size_t)(m * 2 + n) * WV * 256);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) S[m][n][r] = fmaf(gl, S[m][n][r], x[r]);
+                    }
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (size_t)(m * 2 + n) * WV * 256);
+        }
+    }
+
     const auto stage = [&]() {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int row = row0 + i * 16;
-            u32x4 p[NP];
-            const int kv = row * D + ((u ^ swz_kv<D>(row)) * 8);
-            lin_pieces<T, NP>(rk[i], p);
+            if constexpr (F32) {
+                const int at = row * ROW, u0 = u * 8, u1 = u * 8 + 4;
+                *(u32x4*)(f_k + at + u0) = rk[i].v[0];
+                *(u32x4*)(f_k + at + u1) = rk[i].v[1];
+                *(u32x4*)(f_v + at + u0) = rv[i].v[0];
+                *(u32x4*)(f_v + at + u1) = rv[i].v[1];
+                if (OUT) {
+                    *(u32x4*)(f_q + at + u0) = rq[i].v[0];
+                    *(u32x4*)(f_q + at + u1) = rq[i].v[1];
+                }
+            } else {
+                const int kv = row * ROW + u * 8;
+                *(u32x4*)(s_k + kv) = rk[i].v[0];
+                *(u32x4*)(s_v + kv) = rv[i].v[0];
+                if (OUT) {
+                    // Channels 4 x of a 32-channel block go to unit x % 4, half x / 4.
+                    const int unit0 = (u & ~3) + 2 * (u & 1), half = ((u >> 1) & 1) * 4;
+                    unsigned short* q0 = s_q + row * ROW + unit0 * 8 + half;
+                    unsigned short* q1 = q0 + 8;
+                    const u32x4 v = rq[i].v[0];
+                    *(u32x2*)q0 = u32x2{v[0], v[1]};
+                    *(u32x2*)q1 = u32x2{v[2], v[3]};
+                    if constexpr (F16) {
+                        float x[8];
+                        u32x4 p[2];
+                        lin_floats<T>(v, x);
+                        lin_split<2>(x, p);
 #pragma unroll
-            for (int n = 0; n < NP; ++n) *(u32x4*)(s_k + n * PLANE + kv) = p[n];
-            lin_pieces<T, NP>(rv[i], p);
-#pragma unroll
-            for (int n = 0; n < NP; ++n) *(u32x4*)(s_v + n * PLANE + kv) = p[n];
-            if (OUT) {
-                // Channels 4 x of a 32-channel block go to unit x % 4, half x / 4.
-                lin_pieces<T, NP>(rq[i], p);
-                const int unit0 = (u & ~3) + 2 * (u & 1), half = ((u >> 1) & 1) * 4;
-                unsigned short* q0 = s_q + row * D + ((unit0 ^ swz_q<D>(row)) * 8) + half;
-                unsigned short* q1 = s_q + row * D + (((unit0 + 1) ^ swz_q<D>(row)) * 8) + half;
-#pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    *(u32x2*)(q0 + n * PLANE) = u32x2{p[n][0], p[n][1]};
-                    *(u32x2*)(q1 + n * PLANE) = u32x2{p[n][2], p[n][3]};
+                        for (int n = 0; n < 2; ++n) {
+                            *(u32x2*)(q0 + (n + 1) * PLANE) = u32x2{p[n][0], p[n][1]};
+                            *(u32x2*)(q1 + (n + 1) * PLANE) = u32x2{p[n][2], p[n][3]};
+                        }
+                    }
                 }
             }
         }
     };
 
-    if (begin < end) fetch(begin);
     for (int pos = begin; pos < end; pos += LC) {
         __syncthreads();
         stage();
@@ -445,38 +553,49 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
         if (pos + LC < end) fetch(pos + LC);
         if (!work) continue;
 
-        f32x4 O[2][2];  // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
-        u32x4 P[2][NM]; // weighted query products of positions 16 i + l16 with j = {4 g + r, 16 + 4 g + r}
+        f32x4 O[2][2];   // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
+        u32x4 P[2][2];   // P[i]: weighted query products of positions 16 i + l16 with j = {4 g + r, 16 + 4 g + r}, two
+                         // pieces; f32: P[i][t] with j = 16 t + 4 g + r
         if (OUT) {
             f32x4 pt[2][2];  // pt[j][i]: rows are positions j of the keys, columns positions i of the queries
+            if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pt[i >> 1][i & 1] = O[i >> 1][i & 1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int s = 0; s < MT; ++s) {
+                    f32x4 kf[2], qf[2], sf[2];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                u32x4 qf[2][NP], kf[2][NP];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int row = 16 * i + l16;
-                    const unsigned short* qr = s_q + row * D + (((4 * s + g) ^ swz_q<D>(row)) * 8);
-                    const unsigned short* k0 = s_k + row * D + (((4 * s + (g >> 1)) ^ swz_kv<D>(row)) * 8) + (g & 1) * 4;
-                    const unsigned short* k1 = s_k + row * D + (((4 * s + 2 + (g >> 1)) ^ swz_kv<D>(row)) * 8) + (g & 1) * 4;
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        qf[i][n] = *(const u32x4*)(qr + n * PLANE);
-                        const u32x2 lo = *(const u32x2*)(k0 + n * PLANE), hi = *(const u32x2*)(k1 + n * PLANE);
-                        kf[i][n] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = (16 * i + l16) * ROW + (4 * s + g) * 4;
+                        kf[i] = *(const f32x4*)(f_k + at);
+                        qf[i] = *(const f32x4*)(f_q + at);
+                        sf[i] = S[s][i];
                     }
+                    lin_mma_f32<true>(pt, kf, qf, s == 0);
+                    lin_mma_f32<false>(O, sf, qf, s == 0);
                 }
-                lin_mma<LIM>(pt, kf, qf);
-                u32x4 sf[2][NM];
+            } else {
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    float x[8];
+                for (int s = 0; s < KS; ++s) {
+                    u32x4 qf[2][1], qp[2][QP], kf[2][1], sf[2][2];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] = S[2 * s][n][r], x[4 + r] = S[2 * s + 1][n][r];
-                    lin_split<NM>(x, sf[n]);
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = 16 * i + l16;
+                        const unsigned short* qr = s_q + row * ROW + (4 * s + g) * 8;
+                        const unsigned short* k0 = s_k + row * ROW + 32 * s + 4 * g;
+                        const unsigned short* k1 = k0 + 16;
+                        qf[i][0] = *(const u32x4*)qr;
+#pragma unroll
+                        for (int n = 0; n < QP; ++n) qp[i][n] = F16 ? *(const u32x4*)(qr + (n + 1) * PLANE) : qf[i][0];
+                        const u32x2 lo = *(const u32x2*)k0, hi = *(const u32x2*)k1;
+                        kf[i][0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                        float x[8];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[r] = S[2 * s][i][r], x[4 + r] = S[2 * s + 1][i][r];
+                        lin_split<2>(x, sf[i]);
+                    }
+                    if constexpr (F16) lin_mma_f16(pt, kf, qf, s == 0);
+                    else lin_mma(pt, kf, qf, s == 0);
+                    lin_mma(O, sf, qp, s == 0);
                 }
-                lin_mma<LIM>(O, sf, qf);
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n)
@@ -493,69 +612,92 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                 x1[r] = pt[0][1][r] * w_n[r];
                 x1[4 + r] = seen ? pt[1][1][r] * w_d[r] : 0.0f;
             }
-            lin_split<NM>(x0, P[0]);
-            lin_split<NM>(x1, P[1]);
+            if constexpr (F32) {
+                P[0][0] = __builtin_bit_cast(u32x4, f32x4{x0[0], x0[1], x0[2], x0[3]});
+                P[1][0] = __builtin_bit_cast(u32x4, f32x4{x1[0], x1[1], x1[2], x1[3]});
+                P[1][1] = __builtin_bit_cast(u32x4, f32x4{x1[4], x1[5], x1[6], x1[7]});
+            } else {
+                lin_split<2>(x0, P[0]);
+                lin_split<2>(x1, P[1]);
+            }
         }
 
         const bool last = pos + LC >= end;
         const bool update = !OUT || !last || (end == len && a.s_out);
         if (update && nv < LC) {  // the last chunk of a state that is kept: weights from its own end
-            g_c = lin_pow(l2, nv);
+            g_c = s_pow[nv];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                w_v[r] = lin_pow(l2, max(0, nv - 1 - (4 * g + r)));
-                w_v[4 + r] = lin_pow(l2, max(0, nv - 1 - (16 + 4 * g + r)));
+                w_v[r] = s_pow[max(0, nv - 1 - (4 * g + r))];
+                w_v[4 + r] = s_pow[max(0, nv - 1 - (16 + 4 * g + r))];
             }
         }
-        const int trow = 4 * g + (l16 >> 2), tcol = (l16 & 3) >> 1, thalf = (l16 & 1) * 4;
-        u32x4 vf[2][NP], wv[2][3];  // the values, and their weighted values' pieces
-        float big = 0.0f;
+        // Transposing reads of 16-bit rows 4 g + r (and 16 + 4 g + r): the lane's part of the address.
+        const int tbase = (4 * g + (l16 >> 2)) * ROW + (l16 & 3) * 4;
+        const auto column16 = [&](const unsigned short* m, int un) {
+            const unsigned short* p = m + tbase + un * 8;
+            const u32x2 lo = lds_tr(p), hi = lds_tr(p + 16 * ROW);
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
+        // Column col of f32 rows 16 t + 4 g + r.
+        const auto column32 = [&](const float* m, int col, int t) {
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = m[(16 * t + 4 * g + r) * ROW + col];
+            }
+            return x;
+        };
+        // The wave's value columns 16 n + l16 at positions j, in the order of P.
+        float x[2][8], big = 0.0f;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const int un = wave * 4 + 2 * n + tcol;
+            if constexpr (F32) {
+                const f32x4 lo = column32(f_v, wave * 32 + 16 * n + l16, 0), hi = column32(f_v, wave * 32 + 16 * n + l16, 1);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                const u32x2 lo = lds_tr(s_v + p * PLANE + trow * D + ((un ^ swz_kv<D>(trow)) * 8) + thalf);
-                const u32x2 hi = lds_tr(s_v + p * PLANE + (trow + 16) * D + ((un ^ swz_kv<D>(trow)) * 8) + thalf);
-                vf[n][p] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                for (int r = 0; r < 4; ++r) x[n][r] = lo[r], x[n][4 + r] = hi[r];
+            } else {
+                lin_floats<T>(column16(s_v, wave * 4 + 2 * n), x[n]);
             }
-            float x[8];
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                float lo = __builtin_bit_cast(float, vf[n][0][h] << 16), hi = __builtin_bit_cast(float, vf[n][0][h] & 0xffff0000u);
-#pragma unroll
-                for (int p = 1; p < NP; ++p) {
-                    lo += __builtin_bit_cast(float, vf[n][p][h] << 16);
-                    hi += __builtin_bit_cast(float, vf[n][p][h] & 0xffff0000u);
-                }
-                big = __builtin_elementwise_maximum(__builtin_elementwise_maximum(big, __builtin_fabsf(lo)), __builtin_fabsf(hi));
-                x[2 * h] = lo * w_v[2 * h];
-                x[2 * h + 1] = hi * w_v[2 * h + 1];
-            }
-            lin_split<3>(x, wv[n]);
+            for (int e = 0; e < 8; ++e) big = __builtin_elementwise_maximum(big, __builtin_fabsf(x[n][e]));
         }
         if (OUT) {
-            if (__builtin_amdgcn_ballot_w64(!(big <= FLT_MAX)) == 0) {
-                lin_mma<LIM>(O, vf, P);
-            } else {
-                // A value that is infinite or NaN: left out of the products, where it would meet the
-                // zero weights of the positions before it, and put on the others afterwards.
-                int first[2] = {LC, LC};
+            // A value that is infinite or NaN is left out of the products, where it would meet the zero
+            // weights of the positions before it, and put on the others afterwards.
+            const bool poison = __builtin_amdgcn_ballot_w64(!(big <= FLT_MAX)) != 0;
+            float y[2][8];
+            int first[2] = {LC, LC};
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[n][e] = x[n][e];
+            if (poison) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
 #pragma unroll
-                    for (int e = 7; e >= 0; --e) {
-                        const unsigned sh = (e & 1) * 16;
-                        if (((vf[n][0][e >> 1] >> sh) & 0x7f80u) == 0x7f80u) {
+                    for (int e = 7; e >= 0; --e)
+                        if (!(__builtin_fabsf(x[n][e]) <= FLT_MAX)) {
                             first[n] = (e >> 2) * 16 + 4 * g + (e & 3);
-#pragma unroll
-                            for (int p = 0; p < NP; ++p) vf[n][p][e >> 1] &= 0xffff0000u >> sh;
+                            y[n][e] = 0.0f;
                         }
-                    }
                     first[n] = min(first[n], __shfl_xor(first[n], 16));
                     first[n] = min(first[n], __shfl_xor(first[n], 32));
                 }
-                lin_mma<LIM>(O, vf, P);
+            }
+            if constexpr (F32) {
+                const f32x4 early[2] = {{y[0][0], y[0][1], y[0][2], y[0][3]}, {y[1][0], y[1][1], y[1][2], y[1][3]}};
+                const f32x4 late[2] = {{y[0][4], y[0][5], y[0][6], y[0][7]}, {y[1][4], y[1][5], y[1][6], y[1][7]}};
+                const f32x4 p[2] = {__builtin_bit_cast(f32x4, P[0][0]), __builtin_bit_cast(f32x4, P[1][0])};
+                lin_mma_f32<false>(O, early, p);
+                lin_mma_f32_late(O[0][1], O[1][1], late, __builtin_bit_cast(f32x4, P[1][1]));
+            } else {
+                u32x4 vf[2][QP];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) lin_split<QP>(y[n], vf[n]);
+                lin_mma(O, vf, P);
+            }
+            if (poison) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -569,24 +711,65 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
         }
         if (update) {
 #pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[n][e] *= w_v[e];
+                    // The product as it is rounded to f32: contracted into v_fma_mixlo_f16 (one rounding), what the second
+                    // piece is the rest of would not always be the first.
+                    if (F16) asm("" : "+v"(x[n][e]));
+                }
+            constexpr int VP = F16 ? 2 : 3;
+            u32x4 wv[2][VP];  // the weighted values' pieces
+            u32x4 hi[2][1], lo[2][1];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                if constexpr (F16) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const unsigned top = pack_f16(x[n][2 * h], x[n][2 * h + 1]);
+                        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+                        const f16x2 p = __builtin_bit_cast(f16x2, top);
+                        hi[n][0][h] = top;
+                        lo[n][0][h] = pack_f16((x[n][2 * h] - (float)p[0]) * 2048.0f, (x[n][2 * h + 1] - (float)p[1]) * 2048.0f);
+                    }
+                } else if constexpr (!F32) {
+                    lin_split<3>(x[n], wv[n]);
+                }
+            }
+#pragma unroll
             for (int m = 0; m < MT; m += 2) {
-                u32x4 kt[2][NP];
                 f32x4 acc[2][2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int un = 2 * (m + h) + tcol;
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) {
-                        const u32x2 lo = lds_tr(s_k + p * PLANE + trow * D + ((un ^ swz_kv<D>(trow)) * 8) + thalf);
-                        const u32x2 hi = lds_tr(s_k + p * PLANE + (trow + 16) * D + ((un ^ swz_kv<D>(trow)) * 8) + thalf);
-                        kt[h][p] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                    }
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[h][n][r] = S[m + h][n][r] * g_c;
+                if constexpr (F32) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const f32x4 kt[2] = {column32(f_k, 16 * m + l16, t), column32(f_k, 16 * m + 16 + l16, t)};
+                        const f32x4 vt[2] = {{x[0][4 * t], x[0][4 * t + 1], x[0][4 * t + 2], x[0][4 * t + 3]},
+                                             {x[1][4 * t], x[1][4 * t + 1], x[1][4 * t + 2], x[1][4 * t + 3]}};
+                        lin_mma_f32<false>(acc, kt, vt);
+                    }
+                } else {
+                    const u32x4 kt[2][1] = {{column16(s_k, 2 * m)}, {column16(s_k, 2 * m + 2)}};
+                    if constexpr (F16) {
+                        f32x4 small[2][2];
+                        lin_mma_f16(acc, kt, hi);
+                        lin_mma_f16(small, kt, lo, true);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) acc[h][n][r] = fmaf(small[h][n][r], 0x1p-11f, acc[h][n][r]);
+                    } else {
+                        lin_mma(acc, kt, wv);
+                    }
                 }
-                lin_mma<2>(acc, kt, wv);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -603,9 +786,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int cc = 16 * n + 4 * g;
-                    f32x4 v = O[n][i];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] *= a.scale;
+                    const f32x4 v = O[n][i];
                     if (c.vec_o) {
                         if (colw + cc < a.dv) store4<T>(o + cc, v);
                     } else {
@@ -630,11 +811,10 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                     if (kk < a.dk && vv < a.dv) a.s_out[(sbase + kk) * a.dv + vv] = S[m][n][r];
                 }
     } else if (live) {
-        float* x = c.scratch + (((size_t)seq * (c.segments - 1) + seg) * c.units + unit) * xunit;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) *(f32x4*)(x + (size_t)(((m * 2 + n) * WV + wave) * 64 + lane) * 4) = S[m][n];
+            for (int n = 0; n < 2; ++n) *(f32x4*)(x_seq + seg * x_seg + (size_t)(m * 2 + n) * WV * 256) = S[m][n];
     }
 }
 
@@ -647,11 +827,17 @@ __global__ void __launch_bounds__(256) k_linear_scan(LinChunkArgs c, int quads) 
     f32x4* x = (f32x4*)c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * quads + q;
     const size_t step = (size_t)c.units * quads;
     f32x4 e = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < c.segments - 1; ++s, x += step) {
-        const f32x4 v = *x;
+    for (int s = 0; s < c.segments - 1; s += 8, x += 8 * step) {
+        f32x4 v[8];  // eight segments' loads at once: one by one each would wait for the store before it
 #pragma unroll
-        for (int r = 0; r < 4; ++r) e[r] = fmaf(g, e[r], v[r]);
-        *x = e;
+        for (int k = 0; k < 8; ++k) v[k] = x[s + k < c.segments - 1 ? k * step : 0];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (s + k >= c.segments - 1) break;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = fmaf(g, e[r], v[k][r]);
+            x[k * step] = e;
+        }
     }
 }
 
@@ -663,6 +849,7 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
     c.seg_len = p.seg_len;
     c.units = p.units;
     c.groups = p.groups;
+    c.teams = p.teams;
     c.tiles = p.units / a.heads;
     const int es = dtype == DT_F32 ? 4 : 2;
     const auto aligned = [&](const LinRows& r, int d, int bytes) {
@@ -672,15 +859,22 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
     c.vec_k = aligned(a.k, a.dk, 16) && aligned(a.q, a.dk, 16);
     c.vec_v = aligned(a.v, a.dv, 16);
     c.vec_o = aligned(a.o, a.dv, 4 * es);
+    c.even = c.vec_k && c.vec_v && a.dk % 8 == 0 && a.dv % 8 == 0;
+    c.fold = p.fold;
     return c;
 }
 
+template <typename T, int WV, bool OUT>
+void chunks_wv(const LinChunkArgs& c, const dim3& grid, hipStream_t s) {
+    const size_t lds = (size_t)c.teams * (lin_lds_planes<T>(OUT) * LC * lin_row<T>(32 * WV) * 2 + WV * 64 * 4);
+    k_linear_chunks<T, WV, OUT><<<grid, c.teams * 64 * WV, lds, s>>>(c);
+}
 template <typename T, bool OUT>
 hipError_t chunks(const LinChunkArgs& c, int width, hipStream_t s) {
-    const dim3 grid((unsigned)((long long)c.a.seqs * (OUT ? c.segments : c.segments - 1) * c.groups));
-    if (width == 32) k_linear_chunks<T, 1, OUT><<<grid, 256, 0, s>>>(c);
-    else if (width == 64) k_linear_chunks<T, 2, OUT><<<grid, 256, 0, s>>>(c);
-    else k_linear_chunks<T, 4, OUT><<<grid, 256, 0, s>>>(c);
+    const dim3 grid((unsigned)(((long long)c.a.seqs * (OUT ? c.segments : c.segments - 1) * c.groups + 7) / 8 * 8));
+    if (width == 32) chunks_wv<T, 1, OUT>(c, grid, s);
+    else if (width == 64) chunks_wv<T, 2, OUT>(c, grid, s);
+    else chunks_wv<T, 4, OUT>(c, grid, s);
     return hipGetLastError();
 }
 template <bool OUT>
@@ -711,18 +905,24 @@ bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= 8; }
 LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     LinChunkPlan p;
     p.width = a.dk <= 32 ? 32 : a.dk <= 64 ? 64 : 128;
-    const int teams = 128 / p.width;
     p.units = a.heads * ((a.dv + p.width - 1) / p.width);
-    p.groups = (p.units + teams - 1) / teams;
-    const long long have = (long long)a.seqs * p.groups;
+    static const int LT = getenv("LT") ? atoi(getenv("LT")) : 512;
+    static const int LM = getenv("LM") ? atoi(getenv("LM")) : 4;
+    static const int LW = getenv("LW") ? atoi(getenv("LW")) : 0;
+    p.teams = LW ? std::min(LW, 128 / p.width) : 128 / p.width;
+    p.groups = (p.units + p.teams - 1) / p.teams;
+    const long long have = (long long)a.seqs * p.units;
     const long long state = (long long)a.seqs * p.units * p.width * p.width * 4;
     const long long chunks = (a.length + LC - 1) / LC;
-    long long n = std::min(std::min((512 + have - 1) / have, chunks / 4), (long long)(scratch_bytes / state) + 1);
+    const long long want = LT * (128 / p.width);
+    long long n = std::min(std::min((want + have - 1) / have, chunks / LM), (long long)(scratch_bytes / state) + 1);
     n = std::max(n, 1LL);
     const long long per = (chunks + n - 1) / n;
     p.seg_len = (int)(per * LC);
     p.segments = (int)((chunks + per - 1) / per);
     if (p.segments < 1) p.segments = 1;
+    static const int LF = getenv("LF") ? atoi(getenv("LF")) : 256;
+    p.fold = (long long)(p.segments - 1) * p.width * p.width * 4 <= (long long)LF << 10;
     return p;
 }
 

@@ -113,8 +113,8 @@ struct Context {
     std::string last_error;
     volatile int stop = 0;
     uint64_t mem_limit = 0;  // zjai_ctx_set_memory_limit: device bytes a picture may need (0: none)
-    // Root context: CONTEXT_SCRATCH_BYTES for zjai_channel_attention_noalloc and for f32 weights on their
-    // way to the split form, both in stream order.
+    // Root context: CONTEXT_SCRATCH_BYTES for zjai_channel_attention_noalloc, for linear attention and for f32
+    // weights on their way to the split form, all in stream order.
     void* scratch = nullptr;
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
     float last_ms = 0.0f;
@@ -147,10 +147,10 @@ struct Context {
 // weight (half its f32 size; dim <= 639 by the Gram kernel's LDS stage), so that maps up to the
 // documented size fit as they do in f32 form.
 constexpr size_t SCRATCH_PIECE_BYTES = 1u << 20;
-constexpr size_t CONTEXT_SCRATCH_BYTES = ZJAI_NOALLOC_SCRATCH_BYTES + SCRATCH_PIECE_BYTES;
+constexpr size_t CONTEXT_SCRATCH_BYTES = 80u << 20;
 // A context's scratch on the current device. The last one given back stays for the next context of its
 // device (one array per device, until the process ends): a program that makes a context per picture would
-// otherwise pay for the allocation, and for what freeing 17 MiB costs the allocations after it, each time.
+// otherwise pay for the allocation, and for what freeing 33 MiB costs the allocations after it, each time.
 void* take_scratch(int device);
 void give_scratch(int device, void* p);  // nothing in flight uses it
 
