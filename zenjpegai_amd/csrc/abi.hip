@@ -573,14 +573,14 @@ void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype, bool recu
         return;
     }
     const LinChunkPlan p = linear_chunk_plan(a, CONTEXT_SCRATCH_BYTES);
-    if ((double)a.seqs * p.segments * p.groups > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
+    if ((double)a.seqs * p.segments * p.units > INT32_MAX - 8) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
     float* scratch = (float*)C.top().scratch;
     const double states = 4.0 * a.seqs * (p.segments - 1) * p.units * p.width * p.width;
     if (p.segments > 1) {
         LaunchScope sc(C, linear_chunk_name(p, dtype, false), 2.0 * n * hs, n * a.heads * dtype_size(dtype) * (a.dk + a.dv) + states);
         ZJAI_HIP(launch_linear_sums(a, p, dtype, scratch, C.stream));
     }
-    if (p.segments > 2 && !p.fold) {
+    if (p.segments > 2) {
         LaunchScope sc(C, "k_linear_scan", 2.0 * states / 4, 2.0 * states);
         ZJAI_HIP(launch_linear_scan(a, p, scratch, C.stream));
     }

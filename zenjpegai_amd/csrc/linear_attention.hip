@@ -23,10 +23,11 @@ __device__ __forceinline__ long long lin_at(const LinRows& r, int width, long lo
 // keeps 4 columns of the NR key rows rg, rg + RG, .. (RG = 256 >> cl_log2) in registers over the
 // positions, so a state is read and written once however many positions there are. q and k of a
 // position go through LDS as f32; the outputs are summed over the row groups by lane exchanges and LDS.
+// Bandwidth and latency: the state's and the first position's loads are all issued before anything waits.
 template <typename T, bool V4, int NR>
 __global__ void __launch_bounds__(256) k_linear_recurrent(LinAttnArgs a, int cl_log2, int tiles) {
     __shared__ float s_k[256], s_q[256];
-    __shared__ f32x4 s_o[4][16];
+    __shared__ f32x4 s_o[4][32];
     __shared__ int s_next;
     const int tid = threadIdx.x, cl = 1 << cl_log2, RG = 256 >> cl_log2;
     const int tile = blockIdx.x % tiles, b = blockIdx.x / tiles;
@@ -54,6 +55,21 @@ __global__ void __launch_bounds__(256) k_linear_recurrent(LinAttnArgs a, int cl_
             }
         }
     }
+    // A position's channels: a thread loads one of k or q and its four value columns. (Absent ones: a channel that
+    // exists, not used.)
+    const int c = tid & 127;
+    T kq, v[4];
+    const auto fetch = [&](int seq, int t) {
+        const LinRows& src = tid < 128 ? a.k : a.q;
+        kq = ((const T*)src.p)[lin_at(src, a.width, seq, t) + (long long)head * a.dk + (c < a.dk ? c : 0)];
+        const T* vp = (const T*)a.v.p + lin_at(a.v, a.width, seq, t) + (long long)head * a.dv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = vp[col + e < a.dv ? col + e : 0];
+    };
+    int len = a.lengths ? max(0, min(a.lengths[first], a.length)) : a.length;
+    if (len > 0) fetch(first, 0);
+    const float g = a.decay[head];
+    s_k[tid] = s_q[tid] = 0.0f;  // rows past dk
     // Sequences of one slot follow one another: the first of them takes them all, in order.
     int next = INT_MAX;
     if (a.slots && a.seqs > 1) {
@@ -69,22 +85,14 @@ __global__ void __launch_bounds__(256) k_linear_recurrent(LinAttnArgs a, int cl_
         if (__syncthreads_or(earlier)) return;
         next = s_next;
     }
-    const float g = a.decay[head];
-    s_k[tid] = s_q[tid] = 0.0f;  // rows past dk
     for (int cur = first;;) {
-        const int len = a.lengths ? max(0, min(a.lengths[cur], a.length)) : a.length;
         for (int t = 0; t < len; ++t) {
-            const int c = tid & 127;
             __syncthreads();
-            if (c < a.dk) {
-                const LinRows& src = tid < 128 ? a.k : a.q;
-                (tid < 128 ? s_k : s_q)[c] = to_f32(((const T*)src.p)[lin_at(src, a.width, cur, t) + (long long)head * a.dk + c]);
-            }
-            const T* vp = (const T*)a.v.p + lin_at(a.v, a.width, cur, t) + (long long)head * a.dv + col;
-            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (c < a.dk) (tid < 128 ? s_k : s_q)[c] = to_f32(kq);
+            float vf[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < a.dv) v[e] = to_f32(vp[e]);
+            for (int e = 0; e < 4; ++e) vf[e] = to_f32(v[e]);
+            if (t + 1 < len) fetch(cur, t + 1);
             __syncthreads();
             f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -92,7 +100,7 @@ __global__ void __launch_bounds__(256) k_linear_recurrent(LinAttnArgs a, int cl_
                 const float kk = s_k[(rg + n * RG) & 255], qq = s_q[(rg + n * RG) & 255];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    S[n][e] = fmaf(g, S[n][e], kk * v[e]);
+                    S[n][e] = fmaf(g, S[n][e], kk * vf[e]);
                     o[e] = fmaf(qq, S[n][e], o[e]);
                 }
             }
@@ -111,6 +119,7 @@ __global__ void __launch_bounds__(256) k_linear_recurrent(LinAttnArgs a, int cl_
         }
         if (next == INT_MAX) break;
         cur = next;
+        fetch(cur, 0);
         __syncthreads();
         if (tid == 0) s_next = INT_MAX;
         __syncthreads();
@@ -132,8 +141,8 @@ __global__ void __launch_bounds__(256) k_linear_recurrent(LinAttnArgs a, int cl_
                 if (col < a.dv) *(f32x4*)p = S[n];
             } else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (col + c < a.dv) p[c] = S[n][c];
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < a.dv) p[e] = S[n][e];
             }
         }
     }
@@ -145,7 +154,9 @@ struct RecurrentPlan {
 };
 RecurrentPlan recurrent_plan(const LinAttnArgs& a) {
     RecurrentPlan p{};
-    while (p.cl_log2 < 4 && (4 << p.cl_log2) < a.dv) ++p.cl_log2;
+    // Whole rows up to 128 columns: 512 bytes at a time instead of 256 took 257 sequences of 16 heads of 128 x 128 from
+    // 170 to 111 us (4.9 TB/s).
+    while (p.cl_log2 < 5 && (4 << p.cl_log2) < a.dv) ++p.cl_log2;
     p.tiles = (a.dv + (4 << p.cl_log2) - 1) / (4 << p.cl_log2);
     const int rg = 256 >> p.cl_log2;
     p.nr = 1;
@@ -161,7 +172,8 @@ void recurrent_nr(const LinAttnArgs& a, const RecurrentPlan& p, hipStream_t s) {
         case 1: k_linear_recurrent<T, V4, 1><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles); break;
         case 2: k_linear_recurrent<T, V4, 2><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles); break;
         case 4: k_linear_recurrent<T, V4, 4><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles); break;
-        default: k_linear_recurrent<T, V4, 8><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles);
+        case 8: k_linear_recurrent<T, V4, 8><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles); break;
+        default: k_linear_recurrent<T, V4, 16><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles);
     }
 }
 template <typename T>
@@ -350,10 +362,9 @@ __device__ __forceinline__ u32x2 lds_tr(const unsigned short* p) {
 struct LinChunkArgs {
     LinAttnArgs a;
     float* scratch;  // sums: the state after each segment; outputs: before each but the first
-    int segments, seg_len, units, groups, teams, tiles;
+    int segments, seg_len, units, tiles;
     int vec_k, vec_v, vec_o;
     int even;  // vec_k and vec_v, and head sizes of whole units
-    int fold;  // outputs: join the segments' sums in place of a scan
 };
 
 // 16-bit planes of a chunk in LDS: k, v and, for outputs, q (f16's in pieces too).
@@ -364,35 +375,33 @@ template <typename T> __host__ __device__ constexpr int lin_lds_planes(bool out)
 template <typename T, int WV, bool OUT>
 __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     constexpr bool F32 = sizeof(T) == 4, F16 = Elem<T>::dt == DT_F16;
-    constexpr int D = 32 * WV, TT = 64 * WV;
+    constexpr int D = 32 * WV;
     constexpr int ROW = lin_row<T>(D), PLANE = LC * ROW;  // LDS values of a position and of a chunk of q, k or v
     constexpr int MT = D / 16, KS = D / 32;
     constexpr int QP = F16 ? 2 : 1;           // bf16 pieces of a 16-bit q or v
-    extern __shared__ __attribute__((aligned(16))) unsigned short s_lds[];  // [teams][lin_lds_planes][PLANE]
+    extern __shared__ __attribute__((aligned(16))) unsigned short s_lds[];  // [lin_lds_planes][PLANE], then 64 WV floats
     const LinAttnArgs& a = c.a;
-    const int team = threadIdx.x / TT, t = threadIdx.x % TT, wave = t >> 6, lane = t & 63, l16 = lane & 15, g = lane >> 4;
-    unsigned short* s_k = s_lds + team * lin_lds_planes<T>(OUT) * PLANE;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, l16 = lane & 15, g = lane >> 4;
+    unsigned short* s_k = s_lds;
     unsigned short* s_v = s_k + (F32 ? 2 : 1) * PLANE;
     unsigned short* s_q = s_v + (F32 ? 2 : 1) * PLANE;  // f16: the values, then their two pieces
     float *f_k = (float*)s_k, *f_v = (float*)s_v, *f_q = (float*)s_q;
 
-    // Workgroups go round the eight XCDs; neighbours in (sequence, segment, group) share cache lines of the
+    // Workgroups go round the eight XCDs; neighbours in (sequence, segment, unit) share cache lines of the
     // positions' channels and are put on one XCD.
     const int segs = OUT ? c.segments : c.segments - 1;
     int b = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    const int group = b % c.groups;
-    b /= c.groups;
+    const int unit = b % c.units;
+    b /= c.units;
     const int seg = b % segs, seq = b / segs;
     if (seq >= a.seqs) return;
     const int len = a.lengths ? max(0, min(a.lengths[seq], a.length)) : a.length;
     const int begin = seg * c.seg_len, end = min(len, begin + c.seg_len);
     // Sums are those that a later segment starts from.
     if (OUT ? begin > len || (begin == len && seg > 0) : begin + c.seg_len >= len) return;
-    const int unit = group * c.teams + team;
-    const bool live = unit < c.units;
-    const int head = live ? unit / c.tiles : 0, col0 = live ? (unit % c.tiles) * D : 0;
+    const int head = unit / c.tiles, col0 = unit % c.tiles * D;
     const int colw = col0 + wave * 32;        // the wave's 32 value columns
-    const bool work = live && colw < a.dv;
+    const bool work = colw < a.dv;
 
     const T* kp = (const T*)a.k.p + (long long)seq * a.k.seq + (long long)head * a.dk;
     const T* vp = (const T*)a.v.p + (long long)seq * a.v.seq + (long long)head * a.dv + col0;
@@ -406,7 +415,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     LinUnit<T> rk[2], rv[2], rq[2];
     // Whole chunks of evenly strided rows: running pointers, those of absent channels on zeros that stay put.
     const bool even = a.width == 0 && c.even;
-    const bool on_k = live && u * 8 < a.dk, on_v = live && u * 8 < vcols;
+    const bool on_k = u * 8 < a.dk, on_v = u * 8 < vcols;
     const T *pk[2], *pv[2], *pq[2];
     const long long step_k = on_k ? LC * a.k.pos : 0, step_v = on_v ? LC * a.v.pos : 0, step_q = on_k ? LC * a.q.pos : 0;
 #pragma unroll
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int p = pos + row0 + i * 16;
-            const bool ok = live && p < end;
+            const bool ok = p < end;
             const int y = a.width ? p / a.width : 0, x = a.width ? p - y * a.width : p;
             rk[i] = lin_load<T>(kp + (y * a.k.row + x * a.k.pos), u * 8, a.dk, ok, c.vec_k);
             rv[i] = lin_load<T>(vp + (y * a.v.row + x * a.v.pos), u * 8, vcols, ok, c.vec_v);
@@ -444,7 +453,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     if (begin < end) fetch(begin);
 
     // The head's powers g^0..g^63, one a lane, then those a lane's rows and columns need.
-    float* s_pow = (float*)(s_lds + c.teams * lin_lds_planes<T>(OUT) * PLANE) + (threadIdx.x >> 6) * 64;
+    float* s_pow = (float*)(s_lds + lin_lds_planes<T>(OUT) * PLANE) + wave * 64;
     s_pow[lane] = lin_pow(log2f(a.decay[head]), lane);
     __syncthreads();
     float w_v[8], w_o[2], w_d[4], w_n[4], g_c = s_pow[LC];
@@ -482,25 +491,11 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                         const float x = a.s_in[in ? (sbase + kk) * a.dv + vv : 0];
                         S[m][n][r] = in ? x : 0.0f;
                     }
-    } else if (OUT && live) {
-        if (c.fold) {
-            // Few segments: their sums are joined here, E_(s+1) = g^seg_len E_s + X_s.
-            const float gl = lin_pow(log2f(a.decay[head]), c.seg_len);
-            for (int s = 0; s < seg; ++s)
+    } else if (OUT) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const f32x4 x = *(const f32x4*)(x_seq + s * x_seg + (size_t)(m * 2 + n) * WV * 256);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) S[m][n][r] = fmaf(gl, S[m][n][r], x[r]);
-                    }
-        } else {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (size_t)(m * 2 + n) * WV * 256);
-        }
+            for (int n = 0; n < 2; ++n) S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (size_t)(m * 2 + n) * WV * 256);
     }
 
     const auto stage = [&]() {
@@ -810,7 +805,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                     const int kk = 16 * m + 4 * g + r, vv = colw + 16 * n + l16;
                     if (kk < a.dk && vv < a.dv) a.s_out[(sbase + kk) * a.dv + vv] = S[m][n][r];
                 }
-    } else if (live) {
+    } else {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -819,24 +814,25 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
 }
 
 // The state before segment s + 1 from the segments' own sums: E_(s+1) = g^seg_len E_s + X_s, in place (E_1 = X_0).
-__global__ void __launch_bounds__(256) k_linear_scan(LinChunkArgs c, int quads) {
-    const int q = blockIdx.x * 256 + threadIdx.x;
+// Sixteen segments' loads at once: one by one each would wait for the store before it.
+constexpr int SCAN_BATCH = 16, SCAN_THREADS = 64;
+__global__ void __launch_bounds__(SCAN_THREADS) k_linear_scan(LinChunkArgs c, int quads) {
+    const int q = blockIdx.x * SCAN_THREADS + threadIdx.x;
     if (q >= quads) return;
     const int unit = blockIdx.y % c.units, seq = blockIdx.y / c.units;
     const float g = lin_pow(log2f(c.a.decay[unit / c.tiles]), c.seg_len);
     f32x4* x = (f32x4*)c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * quads + q;
     const size_t step = (size_t)c.units * quads;
     f32x4 e = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < c.segments - 1; s += 8, x += 8 * step) {
-        f32x4 v[8];  // eight segments' loads at once: one by one each would wait for the store before it
+    for (int s = 0; s < c.segments - 1; s += SCAN_BATCH, x += SCAN_BATCH * step) {
+        f32x4 v[SCAN_BATCH];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = x[s + k < c.segments - 1 ? k * step : 0];
+        for (int k = 0; k < SCAN_BATCH; ++k) v[k] = x[s + k < c.segments - 1 ? k * step : 0];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (s + k >= c.segments - 1) break;
+        for (int k = 0; k < SCAN_BATCH; ++k) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) e[r] = fmaf(g, e[r], v[k][r]);
-            x[k * step] = e;
+            if (s + k < c.segments - 1) x[k * step] = e;
         }
     }
 }
@@ -848,8 +844,6 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
     c.segments = p.segments;
     c.seg_len = p.seg_len;
     c.units = p.units;
-    c.groups = p.groups;
-    c.teams = p.teams;
     c.tiles = p.units / a.heads;
     const int es = dtype == DT_F32 ? 4 : 2;
     const auto aligned = [&](const LinRows& r, int d, int bytes) {
@@ -860,18 +854,17 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
     c.vec_v = aligned(a.v, a.dv, 16);
     c.vec_o = aligned(a.o, a.dv, 4 * es);
     c.even = c.vec_k && c.vec_v && a.dk % 8 == 0 && a.dv % 8 == 0;
-    c.fold = p.fold;
     return c;
 }
 
 template <typename T, int WV, bool OUT>
 void chunks_wv(const LinChunkArgs& c, const dim3& grid, hipStream_t s) {
-    const size_t lds = (size_t)c.teams * (lin_lds_planes<T>(OUT) * LC * lin_row<T>(32 * WV) * 2 + WV * 64 * 4);
-    k_linear_chunks<T, WV, OUT><<<grid, c.teams * 64 * WV, lds, s>>>(c);
+    const size_t lds = lin_lds_planes<T>(OUT) * LC * lin_row<T>(32 * WV) * 2 + WV * 64 * 4;
+    k_linear_chunks<T, WV, OUT><<<grid, 64 * WV, lds, s>>>(c);
 }
 template <typename T, bool OUT>
 hipError_t chunks(const LinChunkArgs& c, int width, hipStream_t s) {
-    const dim3 grid((unsigned)(((long long)c.a.seqs * (OUT ? c.segments : c.segments - 1) * c.groups + 7) / 8 * 8));
+    const dim3 grid((unsigned)(((long long)c.a.seqs * (OUT ? c.segments : c.segments - 1) * c.units + 7) / 8 * 8));
     if (width == 32) chunks_wv<T, 1, OUT>(c, grid, s);
     else if (width == 64) chunks_wv<T, 2, OUT>(c, grid, s);
     else chunks_wv<T, 4, OUT>(c, grid, s);
@@ -906,23 +899,17 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     LinChunkPlan p;
     p.width = a.dk <= 32 ? 32 : a.dk <= 64 ? 64 : 128;
     p.units = a.heads * ((a.dv + p.width - 1) / p.width);
-    static const int LT = getenv("LT") ? atoi(getenv("LT")) : 512;
-    static const int LM = getenv("LM") ? atoi(getenv("LM")) : 4;
-    static const int LW = getenv("LW") ? atoi(getenv("LW")) : 0;
-    p.teams = LW ? std::min(LW, 128 / p.width) : 128 / p.width;
-    p.groups = (p.units + p.teams - 1) / p.teams;
-    const long long have = (long long)a.seqs * p.units;
+    const long long waves = (long long)a.seqs * p.units * (p.width / 32), chunks = (a.length + LC - 1) / LC;
     const long long state = (long long)a.seqs * p.units * p.width * p.width * 4;
-    const long long chunks = (a.length + LC - 1) / LC;
-    const long long want = LT * (128 / p.width);
-    long long n = std::min(std::min((want + have - 1) / have, chunks / LM), (long long)(scratch_bytes / state) + 1);
-    n = std::max(n, 1LL);
-    const long long per = (chunks + n - 1) / n;
+    // A wave for every SIMD needs no segments (1080 waves of 240 positions: 21.6 us, in two segments 26.8). With
+    // fewer, k and v are read twice, and two waves to a SIMD pay for it (65536 positions, 64 waves: in 16 segments
+    // 636 us, in 32 434). A segment of one chunk costs more in states than it saves (4096 positions, 5 waves: 29 us,
+    // with two chunks 23, with four 25).
+    const long long want = waves >= 1024 ? 1 : (2048 + waves - 1) / waves;
+    const long long n = std::max(std::min(std::min(want, chunks / 2), (long long)(scratch_bytes / state) + 1), 1LL);
+    const long long per = std::max((chunks + n - 1) / n, 1LL);
     p.seg_len = (int)(per * LC);
-    p.segments = (int)((chunks + per - 1) / per);
-    if (p.segments < 1) p.segments = 1;
-    static const int LF = getenv("LF") ? atoi(getenv("LF")) : 256;
-    p.fold = (long long)(p.segments - 1) * p.width * p.width * 4 <= (long long)LF << 10;
+    p.segments = (int)std::max((chunks + per - 1) / per, 1LL);
     return p;
 }
 
@@ -935,7 +922,7 @@ hipError_t launch_linear_sums(const LinAttnArgs& a, const LinChunkPlan& p, int d
 }
 hipError_t launch_linear_scan(const LinAttnArgs& a, const LinChunkPlan& p, float* scratch, hipStream_t s) {
     const int quads = p.width * p.width / 4;
-    k_linear_scan<<<dim3((unsigned)((quads + 255) / 256), (unsigned)(a.seqs * p.units)), 256, 0, s>>>(chunk_args(a, p, DT_F32, scratch), quads);
+    k_linear_scan<<<dim3((unsigned)((quads + SCAN_THREADS - 1) / SCAN_THREADS), (unsigned)(a.seqs * p.units)), SCAN_THREADS, 0, s>>>(chunk_args(a, p, DT_F32, scratch), quads);
     return hipGetLastError();
 }
 hipError_t launch_linear_outputs(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, const float* scratch, hipStream_t s) {

@@ -152,9 +152,8 @@ constexpr int LIN_MAX_KEY = 128, LIN_MAX_VALUE = 1024;
 // run side by side; with more than one, `scratch` holds linear_scratch_bytes.
 struct LinChunkPlan {
     int segments = 1, seg_len = 0;
-    bool fold = false;     // no scan: the outputs' kernel joins the segments' sums
     int width = 32;        // key and value channels of a unit: 32, 64 or 128
-    int units = 0, teams = 1, groups = 0;  // units of a sequence, of a workgroup, workgroups of a sequence
+    int units = 0;         // units of a sequence, a workgroup each
 };
 LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes);
 bool linear_prefers_recurrent(const LinAttnArgs& a);
