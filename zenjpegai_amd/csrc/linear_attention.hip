@@ -548,10 +548,96 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
         if (pos + LC < end) fetch(pos + LC);
         if (!work) continue;
 
-        f32x4 O[2][2];   // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
-        u32x4 P[2][2];   // P[i]: weighted query products of positions 16 i + l16 with j = {4 g + r, 16 + 4 g + r}, two
-                         // pieces; f32: P[i][t] with j = 16 t + 4 g + r
+        const bool last = pos + LC >= end;
+        const bool update = !OUT || !last || (end == len && a.s_out);
+        if (update && nv < LC) {  // the last chunk of a state that is kept: weights from its own end
+            g_c = s_pow[nv];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                w_v[r] = s_pow[max(0, nv - 1 - (4 * g + r))];
+                w_v[4 + r] = s_pow[max(0, nv - 1 - (16 + 4 * g + r))];
+            }
+        }
+        // Transposing reads of 16-bit rows 4 g + r (and 16 + 4 g + r): the lane's part of the address.
+        const int tbase = (4 * g + (l16 >> 2)) * ROW + (l16 & 3) * 4;
+        const auto column16 = [&](const unsigned short* m, int un) {
+            const unsigned short* p = m + tbase + un * 8;
+            const u32x2 lo = lds_tr(p), hi = lds_tr(p + 16 * ROW);
+            return u32x4{lo[0], lo[1], hi[0], hi[1]};
+        };
+        // Column col of f32 rows 16 t + 4 g + r.
+        const auto column32 = [&](const float* m, int col, int t) {
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = m[(16 * t + 4 * g + r) * ROW + col];
+            return x;
+        };
+
+        // The wave's value columns 16 n + l16 at positions j, in the order of P, and their weighted pieces.
+        float x[2][8];
+        u32x4 wv[2][3], hi[2][1], lo[2][1];
+        const auto weigh = [&]() {
+            float w[2][8];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[n][e] = x[n][e] * w_v[e];
+                    // The product as it is rounded to f32: contracted into v_fma_mixlo_f16 (one rounding), what the second
+                    // piece is the rest of would not always be the first.
+                    if (F16) asm("" : "+v"(w[n][e]));
+                }
+                if constexpr (F32) {
+                    wv[n][0] = __builtin_bit_cast(u32x4, f32x4{w[n][0], w[n][1], w[n][2], w[n][3]});
+                    wv[n][1] = __builtin_bit_cast(u32x4, f32x4{w[n][4], w[n][5], w[n][6], w[n][7]});
+                } else if constexpr (F16) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const unsigned top = pack_f16(w[n][2 * h], w[n][2 * h + 1]);
+                        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+                        const f16x2 p = __builtin_bit_cast(f16x2, top);
+                        hi[n][0][h] = top;
+                        lo[n][0][h] = pack_f16((w[n][2 * h] - (float)p[0]) * 2048.0f, (w[n][2 * h + 1] - (float)p[1]) * 2048.0f);
+                    }
+                } else {
+                    lin_split<3>(w[n], wv[n]);
+                }
+            }
+        };
+        float big = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            if constexpr (F32) {
+                const f32x4 t0 = column32(f_v, wave * 32 + 16 * n + l16, 0), t1 = column32(f_v, wave * 32 + 16 * n + l16, 1);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[n][r] = t0[r], x[n][4 + r] = t1[r];
+            } else {
+                lin_floats<T>(column16(s_v, wave * 4 + 2 * n), x[n]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) big = __builtin_elementwise_maximum(big, __builtin_fabsf(x[n][e]));
+        }
+        weigh();
+
         if (OUT) {
+            // A value that is infinite or NaN is left out of the products, where it would meet the zero
+            // weights of the positions before it, and put on the others afterwards.
+            const bool poison = __builtin_amdgcn_ballot_w64(!(big <= FLT_MAX)) != 0;
+            int first[2] = {LC, LC};
+            if (poison) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                    for (int e = 7; e >= 0; --e)
+                        if (!(__builtin_fabsf(x[n][e]) <= FLT_MAX)) {
+                            first[n] = (e >> 2) * 16 + 4 * g + (e & 3);
+                            x[n][e] = 0.0f;
+                        }
+                    first[n] = min(first[n], __shfl_xor(first[n], 16));
+                    first[n] = min(first[n], __shfl_xor(first[n], 32));
+                }
+            }
+            f32x4 O[2][2];   // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
             f32x4 pt[2][2];  // pt[j][i]: rows are positions j of the keys, columns positions i of the queries
             if constexpr (F32) {
 #pragma unroll
@@ -576,16 +662,15 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                         const int row = 16 * i + l16;
                         const unsigned short* qr = s_q + row * ROW + (4 * s + g) * 8;
                         const unsigned short* k0 = s_k + row * ROW + 32 * s + 4 * g;
-                        const unsigned short* k1 = k0 + 16;
                         qf[i][0] = *(const u32x4*)qr;
 #pragma unroll
                         for (int n = 0; n < QP; ++n) qp[i][n] = F16 ? *(const u32x4*)(qr + (n + 1) * PLANE) : qf[i][0];
-                        const u32x2 lo = *(const u32x2*)k0, hi = *(const u32x2*)k1;
-                        kf[i][0] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-                        float x[8];
+                        const u32x2 k_lo = *(const u32x2*)k0, k_hi = *(const u32x2*)(k0 + 16);
+                        kf[i][0] = u32x4{k_lo[0], k_lo[1], k_hi[0], k_hi[1]};
+                        float z[8];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) x[r] = S[2 * s][i][r], x[4 + r] = S[2 * s + 1][i][r];
-                        lin_split<2>(x, sf[i]);
+                        for (int r = 0; r < 4; ++r) z[r] = S[2 * s][i][r], z[4 + r] = S[2 * s + 1][i][r];
+                        lin_split<2>(z, sf[i]);
                     }
                     if constexpr (F16) lin_mma_f16(pt, kf, qf, s == 0);
                     else lin_mma(pt, kf, qf, s == 0);
@@ -598,98 +683,28 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) O[n][i][r] *= w_o[i];
-            float x0[8], x1[8];
+            // Weighted query products of positions 16 i + l16 with j = {4 g + r, 16 + 4 g + r}.
+            float p0[8], p1[8];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const bool seen = 4 * g + r <= l16;  // a select: products with later positions may be infinite
-                x0[r] = seen ? pt[0][0][r] * w_d[r] : 0.0f;
-                x0[4 + r] = 0.0f;
-                x1[r] = pt[0][1][r] * w_n[r];
-                x1[4 + r] = seen ? pt[1][1][r] * w_d[r] : 0.0f;
+                p0[r] = seen ? pt[0][0][r] * w_d[r] : 0.0f;
+                p0[4 + r] = 0.0f;
+                p1[r] = pt[0][1][r] * w_n[r];
+                p1[4 + r] = seen ? pt[1][1][r] * w_d[r] : 0.0f;
             }
             if constexpr (F32) {
-                P[0][0] = __builtin_bit_cast(u32x4, f32x4{x0[0], x0[1], x0[2], x0[3]});
-                P[1][0] = __builtin_bit_cast(u32x4, f32x4{x1[0], x1[1], x1[2], x1[3]});
-                P[1][1] = __builtin_bit_cast(u32x4, f32x4{x1[4], x1[5], x1[6], x1[7]});
-            } else {
-                lin_split<2>(x0, P[0]);
-                lin_split<2>(x1, P[1]);
-            }
-        }
-
-        const bool last = pos + LC >= end;
-        const bool update = !OUT || !last || (end == len && a.s_out);
-        if (update && nv < LC) {  // the last chunk of a state that is kept: weights from its own end
-            g_c = s_pow[nv];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                w_v[r] = s_pow[max(0, nv - 1 - (4 * g + r))];
-                w_v[4 + r] = s_pow[max(0, nv - 1 - (16 + 4 * g + r))];
-            }
-        }
-        // Transposing reads of 16-bit rows 4 g + r (and 16 + 4 g + r): the lane's part of the address.
-        const int tbase = (4 * g + (l16 >> 2)) * ROW + (l16 & 3) * 4;
-        const auto column16 = [&](const unsigned short* m, int un) {
-            const unsigned short* p = m + tbase + un * 8;
-            const u32x2 lo = lds_tr(p), hi = lds_tr(p + 16 * ROW);
-            return u32x4{lo[0], lo[1], hi[0], hi[1]};
-        };
-        // Column col of f32 rows 16 t + 4 g + r.
-        const auto column32 = [&](const float* m, int col, int t) {
-            f32x4 x;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[r] = m[(16 * t + 4 * g + r) * ROW + col];
-            }
-            return x;
-        };
-        // The wave's value columns 16 n + l16 at positions j, in the order of P.
-        float x[2][8], big = 0.0f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            if constexpr (F32) {
-                const f32x4 lo = column32(f_v, wave * 32 + 16 * n + l16, 0), hi = column32(f_v, wave * 32 + 16 * n + l16, 1);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[n][r] = lo[r], x[n][4 + r] = hi[r];
-            } else {
-                lin_floats<T>(column16(s_v, wave * 4 + 2 * n), x[n]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) big = __builtin_elementwise_maximum(big, __builtin_fabsf(x[n][e]));
-        }
-        if (OUT) {
-            // A value that is infinite or NaN is left out of the products, where it would meet the zero
-            // weights of the positions before it, and put on the others afterwards.
-            const bool poison = __builtin_amdgcn_ballot_w64(!(big <= FLT_MAX)) != 0;
-            float y[2][8];
-            int first[2] = {LC, LC};
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[n][e] = x[n][e];
-            if (poison) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                    for (int e = 7; e >= 0; --e)
-                        if (!(__builtin_fabsf(x[n][e]) <= FLT_MAX)) {
-                            first[n] = (e >> 2) * 16 + 4 * g + (e & 3);
-                            y[n][e] = 0.0f;
-                        }
-                    first[n] = min(first[n], __shfl_xor(first[n], 16));
-                    first[n] = min(first[n], __shfl_xor(first[n], 32));
-                }
-            }
-            if constexpr (F32) {
-                const f32x4 early[2] = {{y[0][0], y[0][1], y[0][2], y[0][3]}, {y[1][0], y[1][1], y[1][2], y[1][3]}};
-                const f32x4 late[2] = {{y[0][4], y[0][5], y[0][6], y[0][7]}, {y[1][4], y[1][5], y[1][6], y[1][7]}};
-                const f32x4 p[2] = {__builtin_bit_cast(f32x4, P[0][0]), __builtin_bit_cast(f32x4, P[1][0])};
+                const f32x4 early[2] = {{x[0][0], x[0][1], x[0][2], x[0][3]}, {x[1][0], x[1][1], x[1][2], x[1][3]}};
+                const f32x4 late[2] = {{x[0][4], x[0][5], x[0][6], x[0][7]}, {x[1][4], x[1][5], x[1][6], x[1][7]}};
+                const f32x4 p[2] = {{p0[0], p0[1], p0[2], p0[3]}, {p1[0], p1[1], p1[2], p1[3]}};
                 lin_mma_f32<false>(O, early, p);
-                lin_mma_f32_late(O[0][1], O[1][1], late, __builtin_bit_cast(f32x4, P[1][1]));
+                lin_mma_f32_late(O[0][1], O[1][1], late, f32x4{p1[4], p1[5], p1[6], p1[7]});
             } else {
-                u32x4 vf[2][QP];
+                u32x4 vf[2][QP], P[2][2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) lin_split<QP>(y[n], vf[n]);
+                for (int n = 0; n < 2; ++n) lin_split<QP>(x[n], vf[n]);
+                lin_split<2>(p0, P[0]);
+                lin_split<2>(p1, P[1]);
                 lin_mma(O, vf, P);
             }
             if (poison) {
@@ -703,81 +718,12 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                             if (16 * i + l16 >= from) O[n][i][r] = __builtin_nanf("");
                     }
             }
-        }
-        if (update) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[n][e] *= w_v[e];
-                    // The product as it is rounded to f32: contracted into v_fma_mixlo_f16 (one rounding), what the second
-                    // piece is the rest of would not always be the first.
-                    if (F16) asm("" : "+v"(x[n][e]));
-                }
-            constexpr int VP = F16 ? 2 : 3;
-            u32x4 wv[2][VP];  // the weighted values' pieces
-            u32x4 hi[2][1], lo[2][1];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                if constexpr (F16) {
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const unsigned top = pack_f16(x[n][2 * h], x[n][2 * h + 1]);
-                        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-                        const f16x2 p = __builtin_bit_cast(f16x2, top);
-                        hi[n][0][h] = top;
-                        lo[n][0][h] = pack_f16((x[n][2 * h] - (float)p[0]) * 2048.0f, (x[n][2 * h + 1] - (float)p[1]) * 2048.0f);
-                    }
-                } else if constexpr (!F32) {
-                    lin_split<3>(x[n], wv[n]);
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < MT; m += 2) {
-                f32x4 acc[2][2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[h][n][r] = S[m + h][n][r] * g_c;
-                if constexpr (F32) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const f32x4 kt[2] = {column32(f_k, 16 * m + l16, t), column32(f_k, 16 * m + 16 + l16, t)};
-                        const f32x4 vt[2] = {{x[0][4 * t], x[0][4 * t + 1], x[0][4 * t + 2], x[0][4 * t + 3]},
-                                             {x[1][4 * t], x[1][4 * t + 1], x[1][4 * t + 2], x[1][4 * t + 3]}};
-                        lin_mma_f32<false>(acc, kt, vt);
-                    }
-                } else {
-                    const u32x4 kt[2][1] = {{column16(s_k, 2 * m)}, {column16(s_k, 2 * m + 2)}};
-                    if constexpr (F16) {
-                        f32x4 small[2][2];
-                        lin_mma_f16(acc, kt, hi);
-                        lin_mma_f16(small, kt, lo, true);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) acc[h][n][r] = fmaf(small[h][n][r], 0x1p-11f, acc[h][n][r]);
-                    } else {
-                        lin_mma(acc, kt, wv);
-                    }
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) S[m + h][n] = acc[h][n];
-            }
-        }
-        if (OUT) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int p = pos + 16 * i + l16;
                 if (p >= end) continue;
-                const int y = a.width ? p / a.width : 0, x = a.width ? p - y * a.width : p;
-                T* o = op + (y * a.o.row + x * a.o.pos);
+                const int row = a.width ? p / a.width : 0, at = a.width ? p - row * a.width : p;
+                T* o = op + (row * a.o.row + at * a.o.pos);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int cc = 16 * n + 4 * g;
@@ -791,6 +737,44 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                     }
                 }
             }
+        }
+        if (!update) continue;
+#pragma unroll
+        for (int m = 0; m < MT; m += 2) {
+            f32x4 acc[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[h][n][r] = S[m + h][n][r] * g_c;
+            if constexpr (F32) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const f32x4 kt[2] = {column32(f_k, 16 * m + l16, t), column32(f_k, 16 * m + 16 + l16, t)};
+                    const f32x4 vt[2] = {__builtin_bit_cast(f32x4, wv[0][t]), __builtin_bit_cast(f32x4, wv[1][t])};
+                    lin_mma_f32<false>(acc, kt, vt);
+                }
+            } else {
+                const u32x4 kt[2][1] = {{column16(s_k, 2 * m)}, {column16(s_k, 2 * m + 2)}};
+                if constexpr (F16) {
+                    f32x4 small[2][2];
+                    lin_mma_f16(acc, kt, hi);
+                    lin_mma_f16(small, kt, lo, true);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[h][n][r] = fmaf(small[h][n][r], 0x1p-11f, acc[h][n][r]);
+                } else {
+                    lin_mma(acc, kt, wv);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) S[m + h][n] = acc[h][n];
         }
     }
 
