@@ -573,7 +573,7 @@ void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype, bool recu
         return;
     }
     const LinChunkPlan p = linear_chunk_plan(a, CONTEXT_SCRATCH_BYTES);
-    if ((double)a.seqs * p.segments * p.units > INT32_MAX - 8) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
+    if (((double)a.seqs * p.segments + 8) * p.units > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
     float* scratch = (float*)C.top().scratch;
     const double states = 4.0 * a.seqs * (p.segments - 1) * p.units * p.width * p.width;
     if (p.segments > 1) {

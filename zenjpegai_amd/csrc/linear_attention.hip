@@ -238,73 +238,148 @@ __device__ __forceinline__ void lin_split(const float (&x)[8], u32x4 (&p)[N]) {
     }
 }
 
-// c[i][j] += a[i] b[j] over the products of pieces p + q <= 1 (up to 2 with three), the small ones first (two
-// tiles of either operand; zero: the sums start here, a constant where this is inlined). Inline
-// assembly with the accumulators in place: the compiler renames the builtin's chains back to back. The
-// block carries its own wait states, as split.h's.
-#define LM(MF, i, j, p, q) MF "%[c" #i #j "], %[a" #i #p "], %[b" #j #q "], %[c" #i #j "]\n\t"
-#define LZ(MF, i, j, p, q) MF "%[c" #i #j "], %[a" #i #p "], %[b" #j #q "], 0\n\t"
-#define LM4(MF, p, q) LM(MF, 0, 0, p, q) LM(MF, 0, 1, p, q) LM(MF, 1, 0, p, q) LM(MF, 1, 1, p, q)
-#define LZ4(MF, p, q) LZ(MF, 0, 0, p, q) LZ(MF, 0, 1, p, q) LZ(MF, 1, 0, p, q) LZ(MF, 1, 1, p, q)
-#define LC4 [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1])
-#define LO4 [c00] "=&v"(c[0][0]), [c01] "=&v"(c[0][1]), [c10] "=&v"(c[1][0]), [c11] "=&v"(c[1][1])
-#define LA(p) [a0##p] "v"(a[0][p]), [a1##p] "v"(a[1][p])
-#define LB(p) [b0##p] "v"(b[0][p]), [b1##p] "v"(b[1][p])
-#define LIN_ASM(MF, WAIT, P, Q, REST, ...)                                              \
-    if (zero) asm("s_nop 1\n\t" LZ4(MF, P, Q) REST WAIT : LO4 : __VA_ARGS__);            \
-    else asm("s_nop 1\n\t" LM4(MF, P, Q) REST WAIT : LC4 : __VA_ARGS__);
-template <int NA, int NB>
-__device__ __forceinline__ void lin_mma(f32x4 (&c)[2][2], const u32x4 (&a)[2][NA], const u32x4 (&b)[2][NB], bool zero = false) {
-    if constexpr (NA == 1 && NB == 1) {
-        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 0, 0, , LA(0), LB(0))
-    } else if constexpr (NA == 1 && NB == 2) {
-        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 0, 1, LM4(ZJAI_MF, 0, 0), LA(0), LB(0), LB(1))
-    } else if constexpr (NA == 2 && NB == 1) {
-        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 1, 0, LM4(ZJAI_MF, 0, 0), LA(0), LA(1), LB(0))
-    } else if constexpr (NA == 1 && NB == 3) {
-        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 0, 2, LM4(ZJAI_MF, 0, 1) LM4(ZJAI_MF, 0, 0), LA(0), LB(0), LB(1), LB(2))
-    } else {
-        static_assert(NA == 2 && NB == 2, "piece products");
-        LIN_ASM(ZJAI_MF, ZJAI_WAIT, 1, 0, LM4(ZJAI_MF, 0, 1) LM4(ZJAI_MF, 0, 0), LA(0), LA(1), LB(0), LB(1))
-    }
-}
+// Sums of matrix products, the tiles of an instruction group given as pairs (c, a, b), over the products of pieces
+// p + q <= 1 (up to 2 with three), the small ones first (zero: the sums start here, a constant where this is
+// inlined). Inline assembly with the accumulators in place: the compiler renames the builtin's chains
+// back to back. A block carries its own wait states, as split.h's.
+#define LM(MF, c, a, b) MF "%[c" #c "], %[a" #a "], %[b" #b "], %[c" #c "]\n\t"
+#define LZ(MF, c, a, b) MF "%[c" #c "], %[a" #a "], %[b" #b "], 0\n\t"
+#define LIN_LIST(...) __VA_ARGS__
+#define LIN_ASM(PRODUCTS_ZERO, PRODUCTS, OUT_ZERO, OUT, ...)                          \
+    if (zero) asm("s_nop 1\n\t" PRODUCTS_ZERO : LIN_LIST OUT_ZERO : __VA_ARGS__);     \
+    else asm("s_nop 1\n\t" PRODUCTS : LIN_LIST OUT : __VA_ARGS__);
 #define LIN_F16 "v_mfma_f32_16x16x32_f16 "
-__device__ __forceinline__ void lin_mma_f16(f32x4 (&c)[2][2], const u32x4 (&a)[2][1], const u32x4 (&b)[2][1], bool zero = false) {
-    LIN_ASM(LIN_F16, ZJAI_WAIT, 0, 0, , LA(0), LB(0))
-}
-// The f32 form: sixteen (a tile's four K slots, one register each) or, with TRI, the twelve but c[1][0]'s.
 #define LIN_F32 "v_mfma_f32_16x16x4_f32 "
 #define LIN_F32_WAIT "s_nop 9"
-#define LM3(MF, p, q) LM(MF, 0, 0, p, q) LM(MF, 0, 1, p, q) LM(MF, 1, 1, p, q)
-template <bool TRI>
-__device__ __forceinline__ void lin_mma_f32(f32x4 (&c)[2][2], const f32x4 (&a)[2], const f32x4 (&b)[2], bool zero = false) {
-    if constexpr (TRI) {
-        if (zero) c[0][0] = c[0][1] = c[1][0] = c[1][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        asm("s_nop 1\n\t" LM3(LIN_F32, 0, 0) LM3(LIN_F32, 1, 1) LM3(LIN_F32, 2, 2) LM3(LIN_F32, 3, 3) LIN_F32_WAIT
-            : [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c11] "+v"(c[1][1])
-            : LA(0), LA(1), LA(2), LA(3), LB(0), LB(1), LB(2), LB(3));
+
+// pt[j][i] += k[j] q[i] on the stored values: the three tiles that have a position of the past in them.
+#define L3(X, MF) X(MF, 00, 0, 0) X(MF, 01, 0, 1) X(MF, 11, 1, 1)
+#define LO3 ([c00] "=&v"(c[0][0]), [c01] "=&v"(c[0][1]), [c11] "=&v"(c[1][1]))
+#define LC3 ([c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c11] "+v"(c[1][1]))
+template <bool F16>
+__device__ __forceinline__ void lin_scores(f32x4 (&c)[2][2], const u32x4 (&a)[2], const u32x4 (&b)[2], bool zero) {
+    if constexpr (F16) {
+        LIN_ASM(L3(LZ, LIN_F16) ZJAI_WAIT, L3(LM, LIN_F16) ZJAI_WAIT, LO3, LC3, [a0] "v"(a[0]), [a1] "v"(a[1]), [b0] "v"(b[0]), [b1] "v"(b[1]))
     } else {
-        LIN_ASM(LIN_F32, LIN_F32_WAIT, 0, 0, LM4(LIN_F32, 1, 1) LM4(LIN_F32, 2, 2) LM4(LIN_F32, 3, 3), LA(0), LA(1), LA(2), LA(3), LB(0),
-                LB(1), LB(2), LB(3))
+        LIN_ASM(L3(LZ, ZJAI_MF) ZJAI_WAIT, L3(LM, ZJAI_MF) ZJAI_WAIT, LO3, LC3, [a0] "v"(a[0]), [a1] "v"(a[1]), [b0] "v"(b[0]), [b1] "v"(b[1]))
     }
 }
-// c[n] += a[n] b: the values of the later sixteen positions, which only the later sixteen queries see.
-__device__ __forceinline__ void lin_mma_f32_late(f32x4& c0, f32x4& c1, const f32x4 (&a)[2], const f32x4& b) {
-    asm("s_nop 1\n\t" LIN_F32 "%0, %2, %10, %0\n\t" LIN_F32 "%1, %6, %10, %1\n\t" LIN_F32 "%0, %3, %11, %0\n\t" LIN_F32
-        "%1, %7, %11, %1\n\t" LIN_F32 "%0, %4, %12, %0\n\t" LIN_F32 "%1, %8, %12, %1\n\t" LIN_F32 "%0, %5, %13, %0\n\t" LIN_F32
-        "%1, %9, %13, %1\n\t" LIN_F32_WAIT
-        : "+v"(c0), "+v"(c1)
-        : "v"(a[0][0]), "v"(a[0][1]), "v"(a[0][2]), "v"(a[0][3]), "v"(a[1][0]), "v"(a[1][1]), "v"(a[1][2]), "v"(a[1][3]), "v"(b[0]),
-          "v"(b[1]), "v"(b[2]), "v"(b[3]));
+#define L3R(X, r) X(LIN_F32, 00, 0##r, 0##r) X(LIN_F32, 01, 0##r, 1##r) X(LIN_F32, 11, 1##r, 1##r)
+#define LA4(n) [a##n##0] "v"(a[n][0]), [a##n##1] "v"(a[n][1]), [a##n##2] "v"(a[n][2]), [a##n##3] "v"(a[n][3])
+#define LB4(n) [b##n##0] "v"(b[n][0]), [b##n##1] "v"(b[n][1]), [b##n##2] "v"(b[n][2]), [b##n##3] "v"(b[n][3])
+__device__ __forceinline__ void lin_scores_f32(f32x4 (&c)[2][2], const f32x4 (&a)[2], const f32x4 (&b)[2], bool zero) {
+    LIN_ASM(L3R(LZ, 0) L3R(LM, 1) L3R(LM, 2) L3R(LM, 3) LIN_F32_WAIT, L3R(LM, 0) L3R(LM, 1) L3R(LM, 2) L3R(LM, 3) LIN_F32_WAIT, LO3, LC3,
+            LA4(0), LA4(1), LB4(0), LB4(1))
 }
-#undef LM3
+
+// o[n][i] += a[n] b[i]: tiles of the state or of the values (one or two to a wave) with the queries or their products.
+#define LO1(X, MF, p, q) X(MF, 00, 0##p, 0##q) X(MF, 01, 0##p, 1##q)
+#define LO2(X, MF, p, q) LO1(X, MF, p, q) X(MF, 10, 1##p, 0##q) X(MF, 11, 1##p, 1##q)
+#define OZ1 ([c00] "=&v"(c[0][0]), [c01] "=&v"(c[0][1]))
+#define OZ2 ([c00] "=&v"(c[0][0]), [c01] "=&v"(c[0][1]), [c10] "=&v"(c[1][0]), [c11] "=&v"(c[1][1]))
+#define OC1 ([c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]))
+#define OC2 ([c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1]))
+#define A1(p) [a0##p] "v"(a[0][p])
+#define A2(p) A1(p), [a1##p] "v"(a[1][p])
+#define B1(q) [b0##q] "v"(b[0][q])
+#define B2(q) B1(q), [b1##q] "v"(b[1][q])
+#define LIN_OUT(L, OZ, OC, A)                                                                                                   \
+    if constexpr (NA == 1) {                                                                                                    \
+        static_assert(NB == 2, "piece products");                                                                               \
+        LIN_ASM(L(LZ, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, OZ, OC, A(0), \
+                B2(0), B2(1))                                                                                                   \
+    } else if constexpr (NB == 1) {                                                                                             \
+        LIN_ASM(L(LZ, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, L(LM, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, OZ, OC, A(0), \
+                A(1), B2(0))                                                                                                    \
+    } else {                                                                                                                    \
+        LIN_ASM(L(LZ, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT,                                       \
+                L(LM, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, OZ, OC, A(0), A(1), B2(0), B2(1))      \
+    }
+template <int NV, int NA, int NB>
+__device__ __forceinline__ void lin_outputs(f32x4 (&c)[NV][2], const u32x4 (&a)[NV][NA], const u32x4 (&b)[2][NB], bool zero = false) {
+    if constexpr (NV == 1) {
+        LIN_OUT(LO1, OZ1, OC1, A1)
+    } else {
+        LIN_OUT(LO2, OZ2, OC2, A2)
+    }
+}
+#define R4(L, X) L(X, LIN_F32, 0, 0) L(LM, LIN_F32, 1, 1) L(LM, LIN_F32, 2, 2) L(LM, LIN_F32, 3, 3) LIN_F32_WAIT
+template <int NV>
+__device__ __forceinline__ void lin_outputs_f32(f32x4 (&c)[NV][2], const f32x4 (&a)[NV], const f32x4 (&b)[2], bool zero = false) {
+    if constexpr (NV == 1) {
+        LIN_ASM(R4(LO1, LZ), R4(LO1, LM), OZ1, OC1, A1(0), A1(1), A1(2), A1(3), LB4(0), LB4(1))
+    } else {
+        LIN_ASM(R4(LO2, LZ), R4(LO2, LM), OZ2, OC2, A2(0), A2(1), A2(2), A2(3), LB4(0), LB4(1))
+    }
+}
+// c += a b: the later sixteen values, which only the later sixteen queries see.
+#define LL(X, MF, p, q) X(MF, 0, p, q)
+__device__ __forceinline__ void lin_late_f32(f32x4& c, const f32x4& a, const f32x4& b) {
+    asm("s_nop 1\n\t" R4(LL, LM)
+        : [c0] "+v"(c)
+        : [a0] "v"(a[0]), [a1] "v"(a[1]), [a2] "v"(a[2]), [a3] "v"(a[3]), [b0] "v"(b[0]), [b1] "v"(b[1]), [b2] "v"(b[2]), [b3] "v"(b[3]));
+}
+
+// c[m][n] += a[m] b[n]: two key tiles of the state.
+#define LS1(X, MF, p, q) X(MF, 00, 0##p, 0##q) X(MF, 10, 1##p, 0##q)
+#define LS2(X, MF, p, q) LS1(X, MF, p, q) X(MF, 01, 0##p, 1##q) X(MF, 11, 1##p, 1##q)
+#define SZ1 ([c00] "=&v"(c[0][0]), [c10] "=&v"(c[1][0]))
+#define SZ2 ([c00] "=&v"(c[0][0]), [c10] "=&v"(c[1][0]), [c01] "=&v"(c[0][1]), [c11] "=&v"(c[1][1]))
+#define SC1 ([c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]))
+#define SC2 ([c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [c01] "+v"(c[0][1]), [c11] "+v"(c[1][1]))
+#define LIN_STATE(L, SZ, SC, B)                                                                                                   \
+    if constexpr (F16) {                                                                                                          \
+        static_assert(NB == 1, "piece products");                                                                                 \
+        LIN_ASM(L(LZ, LIN_F16, 0, 0) ZJAI_WAIT, L(LM, LIN_F16, 0, 0) ZJAI_WAIT, SZ, SC, A2(0), B(0))                              \
+    } else {                                                                                                                      \
+        static_assert(NB == 3, "piece products");                                                                                 \
+        LIN_ASM(L(LZ, ZJAI_MF, 0, 2) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT,                                         \
+                L(LM, ZJAI_MF, 0, 2) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, SZ, SC, A2(0), B(0), B(1), B(2))        \
+    }
+template <bool F16, int NV, int NB>
+__device__ __forceinline__ void lin_state(f32x4 (&c)[2][NV], const u32x4 (&a)[2][1], const u32x4 (&b)[NV][NB], bool zero = false) {
+    if constexpr (NV == 1) {
+        LIN_STATE(LS1, SZ1, SC1, B1)
+    } else {
+        LIN_STATE(LS2, SZ2, SC2, B2)
+    }
+}
+template <int NV>
+__device__ __forceinline__ void lin_state_f32(f32x4 (&c)[2][NV], const f32x4 (&a)[2], const f32x4 (&b)[NV], bool zero) {
+    if constexpr (NV == 1) {
+        LIN_ASM(R4(LS1, LZ), R4(LS1, LM), SZ1, SC1, LA4(0), LA4(1), LB4(0))
+    } else {
+        LIN_ASM(R4(LS2, LZ), R4(LS2, LM), SZ2, SC2, LA4(0), LA4(1), LB4(0), LB4(1))
+    }
+}
+#undef LIN_STATE
+#undef SC2
+#undef SC1
+#undef SZ2
+#undef SZ1
+#undef LS2
+#undef LS1
+#undef LL
+#undef R4
+#undef LIN_OUT
+#undef B2
+#undef B1
+#undef A2
+#undef A1
+#undef OC2
+#undef OC1
+#undef OZ2
+#undef OZ1
+#undef LO2
+#undef LO1
+#undef LB4
+#undef LA4
+#undef L3R
+#undef LC3
+#undef LO3
+#undef L3
 #undef LIN_ASM
-#undef LB
-#undef LA
-#undef LO4
-#undef LC4
-#undef LZ4
-#undef LM4
+#undef LIN_LIST
 #undef LZ
 #undef LM
 
@@ -372,10 +447,16 @@ template <typename T> __host__ __device__ constexpr int lin_lds_planes(bool out)
     return sizeof(T) == 4 ? (out ? 6 : 4) : Elem<T>::dt == DT_F16 ? (out ? 5 : 2) : (out ? 3 : 2);
 }
 
-template <typename T, int WV, bool OUT>
-__global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
+// D: channels of a unit; a wave has one 16-column tile of its values or, for the outputs of the widest, two: each of
+// its waves weighs all query products, and with eight waves to a unit (instead of four) that and a barrier
+// between so many cost more than the registers of one tile less give (65536 positions, 16 heads, bf16: 365 us, with two tiles
+// 288). The sums have no such products, and more waves load more (150 us with two tiles, 113 with one).
+constexpr int lin_tiles(int d, bool out) { return out && d == 128 ? 2 : 1; }
+constexpr int lin_waves(int d, bool out) { return d / 16 / lin_tiles(d, out); }
+template <typename T, int D, bool OUT>
+__global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 2 : 3) k_linear_chunks(LinChunkArgs c) {
     constexpr bool F32 = sizeof(T) == 4, F16 = Elem<T>::dt == DT_F16;
-    constexpr int D = 32 * WV;
+    constexpr int NV = lin_tiles(D, OUT);
     constexpr int ROW = lin_row<T>(D), PLANE = LC * ROW;  // LDS values of a position and of a chunk of q, k or v
     constexpr int MT = D / 16, KS = D / 32;
     constexpr int QP = F16 ? 2 : 1;           // bf16 pieces of a 16-bit q or v
@@ -387,20 +468,19 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     unsigned short* s_q = s_v + (F32 ? 2 : 1) * PLANE;  // f16: the values, then their two pieces
     float *f_k = (float*)s_k, *f_v = (float*)s_v, *f_q = (float*)s_q;
 
-    // Workgroups go round the eight XCDs; neighbours in (sequence, segment, unit) share cache lines of the
-    // positions' channels and are put on one XCD.
-    const int segs = OUT ? c.segments : c.segments - 1;
-    int b = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    const int unit = b % c.units;
-    b /= c.units;
-    const int seg = b % segs, seq = b / segs;
+    // Workgroups go round the eight XCDs. The units of a segment share cache lines of the positions' channels and are
+    // put on one XCD, the segments dealt out one by one (a contiguous share of the sequences to an XCD
+    // leaves some with the long ones); with fewer segments than XCDs, units are dealt out instead.
+    const int segs = OUT ? c.segments : c.segments - 1, spread = a.seqs * segs >= 8 ? 8 : 1;
+    const int b = blockIdx.x / spread, part = b / c.units * spread + blockIdx.x % spread;
+    const int unit = b % c.units, seg = part % segs, seq = part / segs;
     if (seq >= a.seqs) return;
     const int len = a.lengths ? max(0, min(a.lengths[seq], a.length)) : a.length;
     const int begin = seg * c.seg_len, end = min(len, begin + c.seg_len);
     // Sums are those that a later segment starts from.
     if (OUT ? begin > len || (begin == len && seg > 0) : begin + c.seg_len >= len) return;
     const int head = unit / c.tiles, col0 = unit % c.tiles * D;
-    const int colw = col0 + wave * 32;        // the wave's 32 value columns
+    const int colw = col0 + wave * 16 * NV;   // the wave's value columns
     const bool work = colw < a.dv;
 
     const T* kp = (const T*)a.k.p + (long long)seq * a.k.seq + (long long)head * a.dk;
@@ -409,39 +489,38 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     T* op = OUT ? (T*)a.o.p + (long long)seq * a.o.seq + (long long)head * a.dv + colw : nullptr;
     const int vcols = a.dv - col0;
 
-    // A thread stages two units of eight channels of each matrix: rows row0 and row0 + 16, unit u.
+    // A thread stages NV units of eight channels of each matrix: positions row0 (and row0 + 16), unit u.
     constexpr int UPR = D / 8;
     const int row0 = t / UPR, u = t % UPR;
-    LinUnit<T> rk[2], rv[2], rq[2];
+    LinUnit<T> rk[NV], rv[NV], rq[NV];
     // Whole chunks of evenly strided rows: running pointers, those of absent channels on zeros that stay put.
     const bool even = a.width == 0 && c.even;
     const bool on_k = u * 8 < a.dk, on_v = u * 8 < vcols;
-    const T *pk[2], *pv[2], *pq[2];
-    const long long step_k = on_k ? LC * a.k.pos : 0, step_v = on_v ? LC * a.v.pos : 0, step_q = on_k ? LC * a.q.pos : 0;
+    const T *pk[NV], *pv[NV], *pq[NV];
+    constexpr int STEP = OUT ? LC : -LC;
+    const long long step_k = on_k ? STEP * a.k.pos : 0, step_v = on_v ? STEP * a.v.pos : 0, step_q = on_k ? STEP * a.q.pos : 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const long long p = begin + row0 + i * 16;
+    for (int i = 0; i < NV; ++i) {
+        const long long p = (OUT ? begin : end - LC) + row0 + i * 16;
         pk[i] = on_k ? kp + p * a.k.pos + u * 8 : (const T*)g_lin_zero;
         pv[i] = on_v ? vp + p * a.v.pos + u * 8 : (const T*)g_lin_zero;
-        if (OUT) pq[i] = on_k ? qp + p * a.q.pos + u * 8 : (const T*)g_lin_zero;
+        pq[i] = OUT && on_k ? qp + p * a.q.pos + u * 8 : (const T*)g_lin_zero;
     }
     const auto fetch = [&](int pos) {
         if (even && pos + LC <= end) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < NV; ++i) {
                 rk[i] = *(const LinUnit<T>*)pk[i];
                 rv[i] = *(const LinUnit<T>*)pv[i];
+                if (OUT) rq[i] = *(const LinUnit<T>*)pq[i];
                 pk[i] += step_k;
                 pv[i] += step_v;
-                if (OUT) {
-                    rq[i] = *(const LinUnit<T>*)pq[i];
-                    pq[i] += step_q;
-                }
+                pq[i] += step_q;
             }
             return;
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NV; ++i) {
             const int p = pos + row0 + i * 16;
             const bool ok = p < end;
             const int y = a.width ? p / a.width : 0, x = a.width ? p - y * a.width : p;
@@ -450,7 +529,9 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
             if (OUT) rq[i] = lin_load<T>(qp + (y * a.q.row + x * a.q.pos), u * 8, a.dk, ok, c.vec_k);
         }
     };
-    if (begin < end) fetch(begin);
+    // Outputs go forward. Sums go backward, from the segment's last chunk to its first: the part of k and v that the
+    // outputs begin with is then what the last-level cache has seen last.
+    if (begin < end) fetch(OUT ? begin : end - LC);
 
     // The head's powers g^0..g^63, one a lane, then those a lane's rows and columns need.
     float* s_pow = (float*)(s_lds + lin_lds_planes<T>(OUT) * PLANE) + wave * 64;
@@ -468,62 +549,55 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
     w_o[0] = s_pow[l16 + 1] * a.scale;
     w_o[1] = s_pow[l16 + 17] * a.scale;
 
-    // The state before the segment: S[mt][n][r] is key channel 16 mt + 4 g + r of value column 16 n + l16.
-    f32x4 S[MT][2];
+    // The state before the segment: S[m][n][r] is key channel 16 m + 4 g + r of value column 16 n + l16.
+    f32x4 S[MT][NV];
+    const long long sbase = ((long long)seq * a.heads + head) * a.dk;
+    const size_t xunit = (size_t)D * D;
+    float* const x_seq = c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * xunit + (size_t)(wave * NV * 64 + lane) * 4;
+    const size_t x_seg = c.units * xunit;
+    const float g_seg = OUT ? 1.0f : lin_pow(log2f(a.decay[head]), c.seg_len);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const long long sbase = ((long long)seq * a.heads + head) * a.dk;
-    const size_t xunit = (size_t)D * D;
-    float* const x_seq = c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * xunit + (size_t)(wave * 64 + lane) * 4;
-    const size_t x_seg = c.units * xunit;
-    if (seg == 0) {
-        if (a.s_in && work)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NV; ++n) {
+            S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (seg == 0) {
+                if (a.s_in && work)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int kk = 16 * m + 4 * g + r, vv = colw + 16 * n + l16;
                         const bool in = kk < a.dk && vv < a.dv;
                         const float x = a.s_in[in ? (sbase + kk) * a.dv + vv : 0];
-                        S[m][n][r] = in ? x : 0.0f;
+                        S[m][n][r] = in ? OUT ? x : x * g_seg : 0.0f;
                     }
-    } else if (OUT) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < 2; ++n) S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (size_t)(m * 2 + n) * WV * 256);
-    }
+            } else if (OUT) {
+                S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (m * (D / 16) + n) * 256);
+            }
+        }
 
     const auto stage = [&]() {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NV; ++i) {
             const int row = row0 + i * 16;
             if constexpr (F32) {
-                const int at = row * ROW, u0 = u * 8, u1 = u * 8 + 4;
-                *(u32x4*)(f_k + at + u0) = rk[i].v[0];
-                *(u32x4*)(f_k + at + u1) = rk[i].v[1];
-                *(u32x4*)(f_v + at + u0) = rv[i].v[0];
-                *(u32x4*)(f_v + at + u1) = rv[i].v[1];
+                const int at = row * ROW + u * 8;
+                *(u32x4*)(f_k + at) = rk[i].v[0];
+                *(u32x4*)(f_k + at + 4) = rk[i].v[1];
+                *(u32x4*)(f_v + at) = rv[i].v[0];
+                *(u32x4*)(f_v + at + 4) = rv[i].v[1];
                 if (OUT) {
-                    *(u32x4*)(f_q + at + u0) = rq[i].v[0];
-                    *(u32x4*)(f_q + at + u1) = rq[i].v[1];
+                    *(u32x4*)(f_q + at) = rq[i].v[0];
+                    *(u32x4*)(f_q + at + 4) = rq[i].v[1];
                 }
             } else {
-                const int kv = row * ROW + u * 8;
-                *(u32x4*)(s_k + kv) = rk[i].v[0];
-                *(u32x4*)(s_v + kv) = rv[i].v[0];
+                *(u32x4*)(s_k + row * ROW + u * 8) = rk[i].v[0];
+                *(u32x4*)(s_v + row * ROW + u * 8) = rv[i].v[0];
                 if (OUT) {
                     // Channels 4 x of a 32-channel block go to unit x % 4, half x / 4.
-                    const int unit0 = (u & ~3) + 2 * (u & 1), half = ((u >> 1) & 1) * 4;
-                    unsigned short* q0 = s_q + row * ROW + unit0 * 8 + half;
-                    unsigned short* q1 = q0 + 8;
+                    unsigned short* q0 = s_q + row * ROW + ((u & ~3) + 2 * (u & 1)) * 8 + ((u >> 1) & 1) * 4;
                     const u32x4 v = rq[i].v[0];
                     *(u32x2*)q0 = u32x2{v[0], v[1]};
-                    *(u32x2*)q1 = u32x2{v[2], v[3]};
+                    *(u32x2*)(q0 + 8) = u32x2{v[2], v[3]};
                     if constexpr (F16) {
                         float x[8];
                         u32x4 p[2];
@@ -532,7 +606,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
                             *(u32x2*)(q0 + (n + 1) * PLANE) = u32x2{p[n][0], p[n][1]};
-                            *(u32x2*)(q1 + (n + 1) * PLANE) = u32x2{p[n][2], p[n][3]};
+                            *(u32x2*)(q0 + 8 + (n + 1) * PLANE) = u32x2{p[n][2], p[n][3]};
                         }
                     }
                 }
@@ -540,12 +614,13 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
         }
     };
 
-    for (int pos = begin; pos < end; pos += LC) {
+    float ahead = 1.0f;  // sums: g^(positions of the segment after this chunk)
+    for (int pos = OUT ? begin : end - LC; OUT ? pos < end : pos >= begin; pos += STEP) {
         __syncthreads();
         stage();
         __syncthreads();
         const int nv = min(LC, end - pos);
-        if (pos + LC < end) fetch(pos + LC);
+        if (OUT ? pos + LC < end : pos > begin) fetch(pos + STEP);
         if (!work) continue;
 
         const bool last = pos + LC >= end;
@@ -573,60 +648,50 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
             return x;
         };
 
-        // The wave's value columns 16 n + l16 at positions j, in the order of P, and their weighted pieces.
-        float x[2][8];
-        u32x4 wv[2][3], hi[2][1], lo[2][1];
-        const auto weigh = [&]() {
-            float w[2][8];
+        // The wave's value columns 16 n + l16 at positions j = {4 g + r, 16 + 4 g + r}, and their weighted pieces.
+        float x[NV][8], w[NV][8], big = 0.0f;
+        u32x4 wv[NV][3], hi[NV][1], lo[NV][1];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[n][e] = x[n][e] * w_v[e];
-                    // The product as it is rounded to f32: contracted into v_fma_mixlo_f16 (one rounding), what the second
-                    // piece is the rest of would not always be the first.
-                    if (F16) asm("" : "+v"(w[n][e]));
-                }
-                if constexpr (F32) {
-                    wv[n][0] = __builtin_bit_cast(u32x4, f32x4{w[n][0], w[n][1], w[n][2], w[n][3]});
-                    wv[n][1] = __builtin_bit_cast(u32x4, f32x4{w[n][4], w[n][5], w[n][6], w[n][7]});
-                } else if constexpr (F16) {
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const unsigned top = pack_f16(w[n][2 * h], w[n][2 * h + 1]);
-                        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-                        const f16x2 p = __builtin_bit_cast(f16x2, top);
-                        hi[n][0][h] = top;
-                        lo[n][0][h] = pack_f16((w[n][2 * h] - (float)p[0]) * 2048.0f, (w[n][2 * h + 1] - (float)p[1]) * 2048.0f);
-                    }
-                } else {
-                    lin_split<3>(w[n], wv[n]);
-                }
-            }
-        };
-        float big = 0.0f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < NV; ++n) {
+            const int col = wave * NV + n;
             if constexpr (F32) {
-                const f32x4 t0 = column32(f_v, wave * 32 + 16 * n + l16, 0), t1 = column32(f_v, wave * 32 + 16 * n + l16, 1);
+                const f32x4 t0 = column32(f_v, col * 16 + l16, 0), t1 = column32(f_v, col * 16 + l16, 1);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[n][r] = t0[r], x[n][4 + r] = t1[r];
             } else {
-                lin_floats<T>(column16(s_v, wave * 4 + 2 * n), x[n]);
+                lin_floats<T>(column16(s_v, col * 2), x[n]);
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) big = __builtin_elementwise_maximum(big, __builtin_fabsf(x[n][e]));
+            for (int e = 0; e < 8; ++e) {
+                big = __builtin_elementwise_maximum(big, __builtin_fabsf(x[n][e]));
+                w[n][e] = x[n][e] * w_v[e];
+                // The product as it is rounded to f32: contracted into v_fma_mixlo_f16 (one rounding), what the second
+                // piece is the rest of would not always be the first.
+                if (F16) asm("" : "+v"(w[n][e]));
+            }
+            if constexpr (F16) {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const unsigned top = pack_f16(w[n][2 * h], w[n][2 * h + 1]);
+                    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+                    const f16x2 p = __builtin_bit_cast(f16x2, top);
+                    hi[n][0][h] = top;
+                    lo[n][0][h] = pack_f16((w[n][2 * h] - (float)p[0]) * 2048.0f, (w[n][2 * h + 1] - (float)p[1]) * 2048.0f);
+                }
+            } else if constexpr (!F32) {
+                lin_split<3>(w[n], wv[n]);
+            }
         }
-        weigh();
 
         if (OUT) {
             // A value that is infinite or NaN is left out of the products, where it would meet the zero
             // weights of the positions before it, and put on the others afterwards.
             const bool poison = __builtin_amdgcn_ballot_w64(!(big <= FLT_MAX)) != 0;
-            int first[2] = {LC, LC};
+            int first[NV];
             if (poison) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
+                for (int n = 0; n < NV; ++n) {
+                    first[n] = LC;
 #pragma unroll
                     for (int e = 7; e >= 0; --e)
                         if (!(__builtin_fabsf(x[n][e]) <= FLT_MAX)) {
@@ -637,53 +702,53 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                     first[n] = min(first[n], __shfl_xor(first[n], 32));
                 }
             }
-            f32x4 O[2][2];   // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
+            f32x4 O[NV][2];  // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
             f32x4 pt[2][2];  // pt[j][i]: rows are positions j of the keys, columns positions i of the queries
             if constexpr (F32) {
 #pragma unroll
                 for (int s = 0; s < MT; ++s) {
-                    f32x4 kf[2], qf[2], sf[2];
+                    f32x4 kf[2], qf[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int at = (16 * i + l16) * ROW + (4 * s + g) * 4;
                         kf[i] = *(const f32x4*)(f_k + at);
                         qf[i] = *(const f32x4*)(f_q + at);
-                        sf[i] = S[s][i];
                     }
-                    lin_mma_f32<true>(pt, kf, qf, s == 0);
-                    lin_mma_f32<false>(O, sf, qf, s == 0);
+                    lin_scores_f32(pt, kf, qf, s == 0);
+                    lin_outputs_f32<NV>(O, S[s], qf, s == 0);
                 }
             } else {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    u32x4 qf[2][1], qp[2][QP], kf[2][1], sf[2][2];
+                    u32x4 qf[2], qp[2][QP], kf[2], sf[NV][2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int row = 16 * i + l16;
-                        const unsigned short* qr = s_q + row * ROW + (4 * s + g) * 8;
-                        const unsigned short* k0 = s_k + row * ROW + 32 * s + 4 * g;
-                        qf[i][0] = *(const u32x4*)qr;
+                        const unsigned short* qr = s_q + (16 * i + l16) * ROW + (4 * s + g) * 8;
+                        const unsigned short* kr = s_k + (16 * i + l16) * ROW + 32 * s + 4 * g;
+                        qf[i] = *(const u32x4*)qr;
 #pragma unroll
-                        for (int n = 0; n < QP; ++n) qp[i][n] = F16 ? *(const u32x4*)(qr + (n + 1) * PLANE) : qf[i][0];
-                        const u32x2 k_lo = *(const u32x2*)k0, k_hi = *(const u32x2*)(k0 + 16);
-                        kf[i][0] = u32x4{k_lo[0], k_lo[1], k_hi[0], k_hi[1]};
+                        for (int n = 0; n < QP; ++n) qp[i][n] = F16 ? *(const u32x4*)(qr + (n + 1) * PLANE) : qf[i];
+                        const u32x2 k_lo = *(const u32x2*)kr, k_hi = *(const u32x2*)(kr + 16);
+                        kf[i] = u32x4{k_lo[0], k_lo[1], k_hi[0], k_hi[1]};
+                    }
+#pragma unroll
+                    for (int n = 0; n < NV; ++n) {
                         float z[8];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) z[r] = S[2 * s][i][r], z[4 + r] = S[2 * s + 1][i][r];
-                        lin_split<2>(z, sf[i]);
+                        for (int r = 0; r < 4; ++r) z[r] = S[2 * s][n][r], z[4 + r] = S[2 * s + 1][n][r];
+                        lin_split<2>(z, sf[n]);
                     }
-                    if constexpr (F16) lin_mma_f16(pt, kf, qf, s == 0);
-                    else lin_mma(pt, kf, qf, s == 0);
-                    lin_mma(O, sf, qp, s == 0);
+                    lin_scores<F16>(pt, kf, qf, s == 0);
+                    lin_outputs<NV>(O, sf, qp, s == 0);
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NV; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) O[n][i][r] *= w_o[i];
-            // Weighted query products of positions 16 i + l16 with j = {4 g + r, 16 + 4 g + r}.
+            // Weighted query products of positions 16 i + l16 with the positions j.
             float p0[8], p1[8];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -694,22 +759,25 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
                 p1[4 + r] = seen ? pt[1][1][r] * w_d[r] : 0.0f;
             }
             if constexpr (F32) {
-                const f32x4 early[2] = {{x[0][0], x[0][1], x[0][2], x[0][3]}, {x[1][0], x[1][1], x[1][2], x[1][3]}};
-                const f32x4 late[2] = {{x[0][4], x[0][5], x[0][6], x[0][7]}, {x[1][4], x[1][5], x[1][6], x[1][7]}};
                 const f32x4 p[2] = {{p0[0], p0[1], p0[2], p0[3]}, {p1[0], p1[1], p1[2], p1[3]}};
-                lin_mma_f32<false>(O, early, p);
-                lin_mma_f32_late(O[0][1], O[1][1], late, f32x4{p1[4], p1[5], p1[6], p1[7]});
-            } else {
-                u32x4 vf[2][QP], P[2][2];
+                f32x4 early[NV];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) lin_split<QP>(x[n], vf[n]);
+                for (int n = 0; n < NV; ++n) early[n] = f32x4{x[n][0], x[n][1], x[n][2], x[n][3]};
+                lin_outputs_f32<NV>(O, early, p);
+#pragma unroll
+                for (int n = 0; n < NV; ++n)
+                    lin_late_f32(O[n][1], f32x4{x[n][4], x[n][5], x[n][6], x[n][7]}, f32x4{p1[4], p1[5], p1[6], p1[7]});
+            } else {
+                u32x4 vf[NV][QP], P[2][2];
+#pragma unroll
+                for (int n = 0; n < NV; ++n) lin_split<QP>(x[n], vf[n]);
                 lin_split<2>(p0, P[0]);
                 lin_split<2>(p1, P[1]);
-                lin_mma(O, vf, P);
+                lin_outputs<NV>(O, vf, P);
             }
             if (poison) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < NV; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int from = __shfl(first[n], 4 * g + r);
@@ -722,18 +790,17 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
             for (int i = 0; i < 2; ++i) {
                 const int p = pos + 16 * i + l16;
                 if (p >= end) continue;
-                const int row = a.width ? p / a.width : 0, at = a.width ? p - row * a.width : p;
-                T* o = op + (row * a.o.row + at * a.o.pos);
+                const int y = a.width ? p / a.width : 0, at = a.width ? p - y * a.width : p;
+                T* o = op + (y * a.o.row + at * a.o.pos);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
+                for (int n = 0; n < NV; ++n) {
                     const int cc = 16 * n + 4 * g;
-                    const f32x4 v = O[n][i];
                     if (c.vec_o) {
-                        if (colw + cc < a.dv) store4<T>(o + cc, v);
+                        if (colw + cc < a.dv) store4<T>(o + cc, O[n][i]);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (colw + cc + r < a.dv) o[cc + r] = from_f32<T>(v[r]);
+                            if (colw + cc + r < a.dv) o[cc + r] = from_f32<T>(O[n][i][r]);
                     }
                 }
             }
@@ -741,59 +808,68 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(LinChunkArgs c) {
         if (!update) continue;
 #pragma unroll
         for (int m = 0; m < MT; m += 2) {
-            f32x4 acc[2][2];
+            f32x4 acc[2][NV];
+            if (OUT)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < NV; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[h][n][r] = S[m + h][n][r] * g_c;
+                        for (int r = 0; r < 4; ++r) acc[h][n][r] = S[m + h][n][r] * g_c;
             if constexpr (F32) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const f32x4 kt[2] = {column32(f_k, 16 * m + l16, t), column32(f_k, 16 * m + 16 + l16, t)};
-                    const f32x4 vt[2] = {__builtin_bit_cast(f32x4, wv[0][t]), __builtin_bit_cast(f32x4, wv[1][t])};
-                    lin_mma_f32<false>(acc, kt, vt);
+                for (int i = 0; i < 2; ++i) {
+                    const f32x4 kt[2] = {column32(f_k, 16 * m + l16, i), column32(f_k, 16 * m + 16 + l16, i)};
+                    f32x4 vt[NV];
+#pragma unroll
+                    for (int n = 0; n < NV; ++n) vt[n] = f32x4{w[n][4 * i], w[n][4 * i + 1], w[n][4 * i + 2], w[n][4 * i + 3]};
+                    lin_state_f32<NV>(acc, kt, vt, !OUT && i == 0);
                 }
             } else {
                 const u32x4 kt[2][1] = {{column16(s_k, 2 * m)}, {column16(s_k, 2 * m + 2)}};
                 if constexpr (F16) {
-                    f32x4 small[2][2];
-                    lin_mma_f16(acc, kt, hi);
-                    lin_mma_f16(small, kt, lo, true);
+                    f32x4 small[2][NV];
+                    lin_state<true, NV>(acc, kt, hi, !OUT);
+                    lin_state<true, NV>(small, kt, lo, true);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
+                        for (int n = 0; n < NV; ++n)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) acc[h][n][r] = fmaf(small[h][n][r], 0x1p-11f, acc[h][n][r]);
                 } else {
-                    lin_mma(acc, kt, wv);
+                    lin_state<false, NV>(acc, kt, wv, !OUT);
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) S[m + h][n] = acc[h][n];
+                for (int n = 0; n < NV; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[m + h][n][r] = OUT ? acc[h][n][r] : fmaf(ahead, acc[h][n][r], S[m + h][n][r]);
         }
+        if (!OUT) ahead *= g_c;
     }
 
     if (OUT) {
         if (!a.s_out || end != len || !work) return;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int n = 0; n < NV; ++n) {
+            const int vv = colw + 16 * n + l16;
+            if (vv >= a.dv) continue;
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int kk = 16 * m + 4 * g + r, vv = colw + 16 * n + l16;
-                    if (kk < a.dk && vv < a.dv) a.s_out[(sbase + kk) * a.dv + vv] = S[m][n][r];
+                    const int kk = 16 * m + 4 * g + r;
+                    if (kk < a.dk) a.s_out[(sbase + kk) * a.dv + vv] = S[m][n][r];
                 }
+        }
     } else {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) *(f32x4*)(x_seq + seg * x_seg + (size_t)(m * 2 + n) * WV * 256) = S[m][n];
+            for (int n = 0; n < NV; ++n) *(f32x4*)(x_seq + seg * x_seg + (m * (D / 16) + n) * 256) = S[m][n];
     }
 }
 
@@ -856,17 +932,19 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
     return c;
 }
 
-template <typename T, int WV, bool OUT>
-void chunks_wv(const LinChunkArgs& c, const dim3& grid, hipStream_t s) {
-    const size_t lds = lin_lds_planes<T>(OUT) * LC * lin_row<T>(32 * WV) * 2 + WV * 64 * 4;
-    k_linear_chunks<T, WV, OUT><<<grid, 64 * WV, lds, s>>>(c);
+template <typename T, int D, bool OUT>
+void chunks_d(const LinChunkArgs& c, const dim3& grid, hipStream_t s) {
+    constexpr int threads = 64 * lin_waves(D, OUT);
+    const size_t lds = lin_lds_planes<T>(OUT) * LC * lin_row<T>(D) * 2 + threads * 4;
+    k_linear_chunks<T, D, OUT><<<grid, threads, lds, s>>>(c);
 }
 template <typename T, bool OUT>
 hipError_t chunks(const LinChunkArgs& c, int width, hipStream_t s) {
-    const dim3 grid((unsigned)(((long long)c.a.seqs * (OUT ? c.segments : c.segments - 1) * c.units + 7) / 8 * 8));
-    if (width == 32) chunks_wv<T, 1, OUT>(c, grid, s);
-    else if (width == 64) chunks_wv<T, 2, OUT>(c, grid, s);
-    else chunks_wv<T, 4, OUT>(c, grid, s);
+    const long long parts = (long long)c.a.seqs * (OUT ? c.segments : c.segments - 1);
+    const dim3 grid((unsigned)((parts >= 8 ? (parts + 7) / 8 * 8 : parts) * c.units));
+    if (width == 32) chunks_d<T, 32, OUT>(c, grid, s);
+    else if (width == 64) chunks_d<T, 64, OUT>(c, grid, s);
+    else chunks_d<T, 128, OUT>(c, grid, s);
     return hipGetLastError();
 }
 template <bool OUT>
@@ -913,7 +991,7 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
 }
 
 std::string linear_chunk_name(const LinChunkPlan& p, int dtype, bool outputs) {
-    return std::string("k_linear_chunks<") + type_name(dtype) + ", " + std::to_string(p.width / 32) + (outputs ? ", true>" : ", false>");
+    return std::string("k_linear_chunks<") + type_name(dtype) + ", " + std::to_string(p.width) + (outputs ? ", true>" : ", false>");
 }
 
 hipError_t launch_linear_sums(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, float* scratch, hipStream_t s) {
