@@ -7,7 +7,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from devbuf import DevBuf, from_raw, to_raw
+from devbuf import DevBuf, from_raw, hip, to_raw
 from linear_attention_oracle import oracle, out_bound, state_bound
 from zenjpegai_amd import _lib, nn
 
@@ -73,7 +73,7 @@ def run_whole(eng, prec, seqs, length, heads, dk, dv, lengths=None, keep=(True, 
 @pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("heads,dk,dv", [(1, 1, 1), (4, 32, 32), (3, 24, 40), (2, 20, 30), (2, 64, 128), (1, 128, 64),
                                          (2, 128, 256), (5, 16, 8)])
-@pytest.mark.parametrize("length", [1, 31, 64, 193])
+@pytest.mark.parametrize("length", [1, 5, 6, 31, 64, 193])
 def test_whole_sequences_equal_the_recurrence(eng, prec, heads, dk, dv, length):
     run_whole(eng, prec, 2, length, heads, dk, dv, seed=length)
 
@@ -160,6 +160,137 @@ def test_an_infinity_reaches_only_its_position_and_later_ones(eng, prec, dk, dv)
         (o, oa, ob), _ = oracle(*parts(to_raw(clean[s], prec), prec, heads, dk, dv), decay, 1.0, length)
         ok = ~hit[s]
         assert (np.abs(got[s] - o) <= out_bound(prec, dk, o, oa, ob))[ok].all()
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+def test_a_memory_of_a_million_positions(eng, prec):
+    """Decays next to one, over many segments."""
+    seqs, length, heads, dk, dv = 1, 6001, 2, 16, 16
+    qkv, out, _, state = inputs(20, prec, seqs, length, heads, dk, dv)
+    decay = np.array([1 - 2.0 ** -20, 1 - 2.0 ** -24], np.float32)
+    b = [DevBuf(a) for a in (qkv, out, decay, state)]
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=1,
+                                                              length=length, decay=b[2], state_in=b[3], state_out=b[3]))
+    eng.sync()
+    check_sequence(prec, heads, dk, dv, qkv[0], decay, 1.0, length, state[0], b[1].get()[0], out[0], b[3].get()[0])
+
+
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 64), (128, 128)])
+@pytest.mark.parametrize("k_size,v_size", [(200.0, 20000.0), (20000.0, 200.0), (1e-3, 1e-4)])
+def test_f16_values_at_the_ends_of_their_range(eng, dk, dv, k_size, v_size):
+    """Products and states far beyond f16's range, outputs back in it by the scale; and small ones."""
+    prec, length, heads = "f16", 100, 2
+    qkv, out, decay, _ = inputs(21, prec, 1, length, heads, dk, dv)
+    x = from_raw(qkv, prec)
+    x[..., heads * dk:2 * heads * dk] *= k_size
+    x[..., 2 * heads * dk:] *= v_size
+    qkv = to_raw(np.clip(x, -6e4, 6e4), prec)
+    scale = 1.0 / (k_size * v_size)
+    b = [DevBuf(a) for a in (qkv, out, decay)]
+    fin = DevBuf(np.zeros((1, heads, dk, dv), np.float32))
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=1,
+                                                              length=length, decay=b[2], scale=scale, state_out=fin))
+    eng.sync()
+    check_sequence(prec, heads, dk, dv, qkv[0], decay, scale, length, None, b[1].get()[0], out[0], fin.get()[0])
+
+
+@pytest.mark.parametrize("prec", ["f32", "bf16"])
+def test_two_contexts_and_other_calls_in_flight_together(prec):
+    """Calls of two contexts that nothing orders, each between channel-attention calls that use its scratch too."""
+    engs = [nn.Engine(0, prec) for _ in range(2)]
+    seqs, length, heads, dk, dv = 1, 1500, 2, 32, 32
+    runs = []
+    for i, e in enumerate(engs):
+        qkv, out, decay, state = inputs(30 + i, prec, seqs, length, heads, dk, dv)
+        b = [DevBuf(a) for a in (qkv, out, decay, state)]
+        other = DevBuf(np.random.default_rng(i).standard_normal((20, 24, 3 * 64)).astype(np.float32))
+        y = DevBuf(np.zeros((20, 24, 64), np.float32))
+        temp = DevBuf(np.ones(4, np.float32))
+        d = nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=1, length=length,
+                                     decay=b[2], scale=0.5)
+        runs.append((e, b, d, qkv, out, decay, other, y, temp))
+    for _ in range(3):
+        for e, _, d, _, _, _, other, y, temp in runs:
+            _lib.check(_lib.lib().zjai_channel_attention_noalloc(e.handle, other.address, 192, 20, 24, 4, temp.address,
+                                                                 _lib.F32, y.address), e.handle)
+            nn.linear_attention_noalloc(e, d)
+    for e, b, _, qkv, out, decay, *_ in runs:
+        e.sync()
+        check_sequence(prec, heads, dk, dv, qkv[0], decay, 0.5, length, None, b[1].get()[0], out[0], None)
+    del runs, b
+    for e in engs:
+        e.close()
+
+
+def test_offsets_that_pass_32_bits(eng):
+    """Two sequences 2^31 + 64 elements apart, and a state slot whose offset passes 2^31 floats."""
+    prec, heads, dk, dv, length = "bf16", 1, 32, 32, 70
+    qkv, out, decay, _ = inputs(40, prec, 2, length, heads, dk, dv)
+    gap, width = (1 << 31) + 64, heads * (2 * dk + dv)
+    big = ctypes.c_void_p()
+    assert hip().hipMalloc(ctypes.byref(big), 2 * (2 * gap + length * width)) == 0
+    try:
+        d_decay = DevBuf(decay)
+        for s in range(2):
+            at = big.value + 2 * s * gap
+            assert hip().hipMemcpy(at, np.ascontiguousarray(qkv[s]).ctypes.data, qkv[s].nbytes, 1) == 0
+        out_at = big.value + 2 * length * width  # behind the first sequence's inputs, and behind the second's
+        nn.linear_attention_noalloc(eng, nn.linear_attention_desc(
+            prec, big.value, out_at, heads=heads, key_dim=dk, value_dim=dv, sequences=2, length=length, decay=d_decay,
+            q_sequence=gap, k_sequence=gap, v_sequence=gap, out_sequence=gap))
+        eng.sync()
+        for s in range(2):
+            got = np.empty((length, heads * dv), np.uint16)
+            assert hip().hipMemcpy(got.ctypes.data, out_at + 2 * s * gap, got.nbytes, 2) == 0
+            check_sequence(prec, heads, dk, dv, qkv[s], decay, 1.0, length, None, got, got, None)
+    finally:
+        hip().hipFree(big)
+    heads, dk, dv, slots = 1, 128, 1024, 16386  # 2^17 floats a state
+    qkv, out, decay, state = inputs(41, "f32", 1, 1, heads, dk, dv)
+    assert hip().hipMalloc(ctypes.byref(big), 4 * slots * dk * dv) == 0
+    try:
+        at = big.value + 4 * (slots - 1) * dk * dv
+        assert hip().hipMemcpy(at, state.ctypes.data, state.nbytes, 1) == 0
+        b = [DevBuf(a) for a in (qkv, out, decay, np.array([slots - 1], np.int32))]
+        nn.linear_attention_step(eng, nn.linear_attention_desc("f32", b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=1,
+                                                               length=1, decay=b[2], slots=b[3], num_slots=slots,
+                                                               state_in=big.value, state_out=big.value))
+        eng.sync()
+        fin = np.empty_like(state[0])
+        assert hip().hipMemcpy(fin.ctypes.data, at, fin.nbytes, 2) == 0
+        check_sequence("f32", heads, dk, dv, qkv[0], decay, 1.0, 1, state[0], b[1].get()[0], out[0], fin)
+    finally:
+        hip().hipFree(big)
+
+
+@pytest.mark.parametrize("what,after", [(_lib.FAIL_LAUNCH, 0), (_lib.FAIL_LAUNCH, 1), (_lib.FAIL_LAUNCH, 2), (_lib.FAIL_ALLOC, 0),
+                                        (_lib.FAIL_ALLOC, 1)])
+def test_an_injected_failure_is_reported_and_the_context_goes_on(what, after):
+    e = nn.Engine(0)
+    x = np.random.default_rng(0).standard_normal((96, 40, 50)).astype(np.float32)
+    t = nn.BTensor.from_planar(e, x)
+    want = nn.linear_attention(e, t, 1, 32, [0.9]).to_planar()
+    e.inject_failure(what, after)
+    with pytest.raises(_lib.HipError) as err:
+        nn.linear_attention(e, t, 1, 32, [0.9])
+    assert err.value.kind == ("Device" if what == _lib.FAIL_LAUNCH else "LimitExceeded")
+    assert np.array_equal(nn.linear_attention(e, t, 1, 32, [0.9]).to_planar(), want)
+    del t
+    e.close()
+
+
+def test_repeated_calls_give_the_same_bits(eng):
+    for prec, seqs, length, dk, dv in (("bf16", 1, 5000, 64, 64), ("f32", 3, 700, 32, 48)):
+        qkv, out, decay, state = inputs(50, prec, seqs, length, 2, dk, dv)
+        b = [DevBuf(a) for a in (qkv, out, decay, state)]
+        fin = [DevBuf(np.zeros_like(state)) for _ in range(2)]
+        got = []
+        for f in fin:
+            nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=2, key_dim=dk, value_dim=dv, sequences=seqs,
+                                                                      length=length, decay=b[2], state_in=b[3], state_out=f))
+            eng.sync()
+            got.append((b[1].get(), f.get()))
+        assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
 
 
 # ------------------------------------------------------------------------- single positions

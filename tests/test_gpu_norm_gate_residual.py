@@ -119,7 +119,7 @@ def test_every_norm_and_gate(eng, prec, post, act, pre):
 @pytest.mark.parametrize("prec", ["f32", "bf16"])
 @pytest.mark.parametrize("c,groups", [(1, 1), (3, 1), (7, 7), (8, 2), (20, 5), (64, 1), (96, 8), (100, 4), (128, 4), (129, 3),
                                       (192, 12), (250, 5), (512, 16), (1000, 8), (1024, 1), (1536, 4), (2048, 128), (4096, 1),
-                                      (5000, 5), (8192, 64), (16384, 2), (16380, 1)])
+                                      (5000, 5), (8192, 64), (16384, 2), (16380, 1), (16383, 3), (9000, 45)])
 def test_channel_and_group_counts(eng, prec, c, groups):
     run(eng, prec, 3, c, groups=groups, act="sigmoid", pre="layer")
     run(eng, prec, 1, c, groups=groups, post="rms", act="silu", weights=False)

@@ -191,13 +191,13 @@ const char* type_name(int dtype) { return dtype == DT_F32 ? "float" : dtype == D
 // 32 positions at a time, with the state S before them, i, j = 0..31 within the chunk:
 //   o_i = scale * ( g^(i+1) q_i S + sum_{j<=i} g^(i-j) (q_i . k_j) v_j )
 //   S  <- g^32 S + sum_j k_j^T (g^(31-j) v_j)
-// all four products on 16x16x32 bf16 MFMAs with f32 accumulators. A unit is one head's up to 32 WV key
-// channels by 32 WV value channels (wider values are several units), the work of WV waves, each with the
-// state of 32 value columns in registers as MFMA accumulators; a workgroup of four waves holds 4 / WV
-// units of one stretch of a sequence. Every operand comes from the accumulator layout itself or from
-// LDS rows of one position: an accumulator tile holds rows 4 g + r of a column in lane group g, so two
-// tiles under one another are the K slots {4 g + r, 16 + 4 g + r} of the next product's operand, and
-// the other operand is read in the same order (q stored so, k^T and v through the transposing LDS read).
+// all four products on MFMAs with f32 accumulators. A unit is one head's up to D = 32, 64 or 128 key channels by
+// D value channels (wider values are several units), a workgroup each; a wave keeps the state of 16 (or 32)
+// of its value columns in registers, as MFMA accumulators. Every operand comes from the accumulator layout
+// itself or from LDS rows of one position: an accumulator tile holds rows 4 g + r of a column in lane
+// group g, so two tiles under one another are the K slots {4 g + r, 16 + 4 g + r} of the next product's
+// operand, and the other operand is read in the same order (q stored so, k^T and v through the
+// transposing LDS read).
 //
 // f32 runs on the f32 MFMAs (16x16x4; the same slots, one register at a time). The 16-bit types run on
 // 16x16x32 MFMAs, q.k on the stored values themselves. What is computed in f32 enters the matrix cores in pieces:
@@ -211,6 +211,21 @@ constexpr int LC = 32;
 
 __device__ u32x4 g_lin_zero[2];  // zeros: the source of absent positions and channels
 
+// log2 g to a few units in its last place, also for g next to 1, where log2f has the places of 1 (a memory of a
+// million positions takes them): there ln g = 2 atanh s, s = (g - 1) / (g + 1), by its series to s^15 (|s| <= 1/3).
+__device__ __forceinline__ float lin_log2(float g) {
+    if (!(g >= 0.5f)) return log2f(g);
+    const float s = (g - 1.0f) * __builtin_amdgcn_rcpf(g + 1.0f), z = s * s;
+    float p = 1.0f / 15.0f;
+    p = fmaf(p, z, 1.0f / 13.0f);
+    p = fmaf(p, z, 1.0f / 11.0f);
+    p = fmaf(p, z, 1.0f / 9.0f);
+    p = fmaf(p, z, 1.0f / 7.0f);
+    p = fmaf(p, z, 1.0f / 5.0f);
+    p = fmaf(p, z, 1.0f / 3.0f);
+    p = fmaf(p, z, 1.0f);
+    return s * p * 2.88539008177792681472f;
+}
 // g^n for n >= 0, l2 = log2 g (-inf for g = 0).
 __device__ __forceinline__ float lin_pow(float l2, int n) { return n == 0 ? 1.0f : exp2f((float)n * l2); }
 
@@ -535,7 +550,7 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 
     // The head's powers g^0..g^63, one a lane, then those a lane's rows and columns need.
     float* s_pow = (float*)(s_lds + lin_lds_planes<T>(OUT) * PLANE) + wave * 64;
-    s_pow[lane] = lin_pow(log2f(a.decay[head]), lane);
+    s_pow[lane] = lin_pow(lin_log2(a.decay[head]), lane);
     __syncthreads();
     float w_v[8], w_o[2], w_d[4], w_n[4], g_c = s_pow[LC];
 #pragma unroll
@@ -555,7 +570,7 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
     const size_t xunit = (size_t)D * D;
     float* const x_seq = c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * xunit + (size_t)(wave * NV * 64 + lane) * 4;
     const size_t x_seg = c.units * xunit;
-    const float g_seg = OUT ? 1.0f : lin_pow(log2f(a.decay[head]), c.seg_len);
+    const float g_seg = OUT ? 1.0f : lin_pow(lin_log2(a.decay[head]), c.seg_len);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -882,7 +897,7 @@ __global__ void __launch_bounds__(1024) k_linear_scan(LinChunkArgs c, int quads,
     __shared__ f32x4 s_total[1024];
     const int lane = threadIdx.x % width, part = threadIdx.x / width, q = blockIdx.x * width + lane;
     const int unit = blockIdx.y % c.units, seq = blockIdx.y / c.units;
-    const float g = lin_pow(log2f(c.a.decay[unit / c.tiles]), c.seg_len);
+    const float g = lin_pow(lin_log2(c.a.decay[unit / c.tiles]), c.seg_len);
     const int s0 = part * SCAN_SEGS, n = c.segments - 1 - s0;
     f32x4* x = (f32x4*)c.scratch + (((size_t)seq * (c.segments - 1) + s0) * c.units + unit) * quads + q;
     const size_t step = (size_t)c.units * quads;
@@ -970,7 +985,10 @@ hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t 
     return recurrent<__bf16>(a, s);
 }
 
-bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= 8; }
+// A position takes the recurrent form 0.8 to 2.7 us, a chunk costs its 32 positions whether they are there or not (one
+// sequence of 4 heads of 32, f32: 4 positions 5.4 against 6.3 us, 8 8.7; 500 of 4 heads of 32 x 64, f16: 14.1
+// against 19.3, 8 22).
+bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= 5; }
 
 LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     LinChunkPlan p;
@@ -980,10 +998,11 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     const long long state = (long long)a.seqs * p.units * p.width * p.width * 4;
     // A wave for every SIMD needs no segments (1080 waves of 240 positions: 21.6 us, in two segments 26.8). With
     // fewer, k and v are read twice, and two waves to a SIMD pay for it (65536 positions, 64 waves: in 16 segments
-    // 636 us, in 32 434). A segment of one chunk costs more in states than it saves (4096 positions, 5 waves: 29 us,
-    // with two chunks 23, with four 25).
-    const long long want = waves >= 1024 ? 1 : (2048 + waves - 1) / waves;
-    const long long n = std::max(std::min(std::min(std::min(want, 1024LL), chunks / 2), (long long)(scratch_bytes / state) + 1), 1LL);
+    // 636 us, in 32 434); with lengths, half of the segments may be empty (12 ragged sequences of up to 3001: six
+    // segments 88 us, eleven 83). A segment has at least as many bytes of channels as of state: 4096 positions in
+    // five heads of 32, f32: one chunk a segment 15.4 us, two 16.8.
+    const long long want = waves >= 1024 ? 1 : ((a.lengths ? 4096 : 2048) + waves - 1) / waves;
+    const long long n = std::max(std::min(std::min(std::min(want, 1024LL), chunks * 32 / p.width), (long long)(scratch_bytes / state) + 1), 1LL);
     const long long per = std::max((chunks + n - 1) / n, 1LL);
     p.seg_len = (int)(per * LC);
     p.segments = (int)std::max((chunks + per - 1) / per, 1LL);
