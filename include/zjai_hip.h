@@ -241,8 +241,8 @@ ZJAI_API int32_t zjai_channel_attention(zjai_ctx* ctx, const zjai_tensor* qkv, i
  * [h][w][channels] (channels = 3 * dim: q, k, v), out [h][w][dim]; temperature is a device array
  * of `heads` floats. The work is enqueued on the context's stream (zjai_sync waits for it) and
  * allocates nothing: its scratch (Gram partial sums, attention matrix, folded weight) is an array
- * of ZJAI_NOALLOC_SCRATCH_BYTES (and 1 MiB beside it) that zjai_ctx_create takes for the context
- * (new, or the one that the last destroyed context of the device left), so calls on several contexts may overlap on one GPU. A map that needs more scratch (with
+ * of 33 MiB, of which it uses ZJAI_NOALLOC_SCRATCH_BYTES (and 1 MiB beside them), that zjai_ctx_create
+ * takes for the context (new, or the one that the last destroyed context of the device left), so calls on several contexts may overlap on one GPU. A map that needs more scratch (with
  * dim 128 and 4 heads: more than ~240k positions) returns ZJAI_E_LIMIT before anything is launched. */
 #define ZJAI_NOALLOC_SCRATCH_BYTES (16u << 20)
 ZJAI_API int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv, int32_t channels,
@@ -259,8 +259,9 @@ ZJAI_API int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv, 
  * context model of this form can be evaluated over a whole map of known latents at once (the
  * encoder) or position by position as they are decoded, with the same result up to rounding. It has
  * no counterpart in the reference, whose channel attention (src/nn/fast/math.rs:512) has the same
- * cost, linear in the positions, but is not causal. Products and sums are f32 whatever the
- * precision, states are f32 arrays. A non-finite q, k or v reaches the outputs of its own position
+ * cost, linear in the positions, but is not causal. Sums and states are f32
+ * whatever the precision, and so are the products, except that whole sequences of more than five f16 or bf16
+ * positions take states and weighted products into the next product with 16 bits (2^-16 of each). A non-finite q, k or v reaches the outputs of its own position
  * and later ones only (infinities may arrive there as NaN), a non-finite state_in every output of its
  * head.
  *
@@ -279,7 +280,9 @@ ZJAI_API int32_t zjai_linear_attention(zjai_ctx* ctx, const zjai_tensor* qkv, in
  * their element; 16-byte aligned buffers, strides and head sizes of whole 16 bytes run fastest. */
 typedef struct zjai_linear_attention_desc {
     int32_t precision, heads, key_dim, value_dim; /* key_dim 1..128, value_dim 1..1024 */
-    int32_t sequences, length;                    /* length: the positions a sequence has room for */
+    int32_t sequences, length;                    /* length: the positions a sequence has room for, up
+                                                     to 2^30; sequences * heads * (blocks of 128 value
+                                                     channels): up to 2^22 (else ZJAI_E_LIMIT) */
     const void *q, *k, *v;
     void* out;
     int64_t q_position, k_position, v_position, out_position; /* from one position to the next */
@@ -416,7 +419,7 @@ ZJAI_API int32_t zjai_picture_upload(zjai_ctx* ctx, zjai_picture* pic, const flo
  * live and pool are models calibrated on measured pool use that bound it from above (bytes per
  * sample of each tile batch's 16 x latent window, +8 %). The nets' own bytes
  * (zjai_net_device_bytes), the buffers of zjai_picture_download_rgb (6 bytes per displayed
- * pixel, 18 with float planes) and what a context holds by itself (17 MiB of scratch) are not
+ * pixel, 18 with float planes) and what a context holds by itself (33 MiB of scratch) are not
  * included. */
 typedef struct zjai_memory_estimate {
     uint64_t picture_bytes;

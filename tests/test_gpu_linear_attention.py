@@ -293,6 +293,62 @@ def test_repeated_calls_give_the_same_bits(eng):
         assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1])
 
 
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 40), (128, 128)])
+def test_what_lies_behind_a_sequence_is_not_read(eng, prec, dk, dv):
+    """NaN in q, k and v past the lengths."""
+    lengths, length, heads = [1, 31, 33, 0, 64], 70, 2
+    qkv, out, decay, state = inputs(60, prec, len(lengths), length, heads, dk, dv)
+    clean = qkv.copy()
+    for s, n in enumerate(lengths):
+        qkv[s, n:] = to_raw(np.full(qkv[s, n:].shape, np.nan), prec)
+    b = [DevBuf(a) for a in (qkv, out, decay, state, np.zeros_like(state), np.asarray(lengths, np.int32))]
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv,
+                                                              sequences=len(lengths), length=length, decay=b[2], state_in=b[3],
+                                                              state_out=b[4], lengths=b[5]))
+    eng.sync()
+    got, fin = b[1].get(), b[4].get()
+    for s, n in enumerate(lengths):
+        check_sequence(prec, heads, dk, dv, clean[s], decay, 1.0, n, state[s], got[s], out[s], fin[s])
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("length", [3, 100, 2500])
+def test_one_query_for_all_positions_and_keys_that_sequences_share(eng, prec, length):
+    heads, dk, dv, seqs = 2, 32, 64, 2
+    qkv, out, decay, _ = inputs(61, prec, 1, length, heads, dk, dv)
+    n = heads * dk
+    b = [DevBuf(a) for a in (qkv, np.repeat(out, seqs, 0), decay)]
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=seqs,
+                                                              length=length, decay=b[2], q_position=0, q_sequence=0,
+                                                              k_sequence=0, v_sequence=0))
+    eng.sync()
+    same = qkv[0].copy()
+    same[:, :n] = same[:1, :n]
+    got = b[1].get()
+    for s in range(seqs):
+        check_sequence(prec, heads, dk, dv, same, decay, 1.0, length, None, got[s], out[0], None)
+
+
+def test_more_than_a_launch_takes_is_refused_before_anything_is_read(eng):
+    b = {n: DevBuf(np.zeros(64, np.float32)) for n in ("qkv", "out", "decay", "s0")}
+    still = dict.fromkeys(("q_position", "k_position", "v_position", "q_sequence", "k_sequence", "v_sequence"), 0)
+
+    def code(heads, sequences, length, step=False, **kw):
+        d = nn.linear_attention_desc("f32", b["qkv"], b["out"], heads=heads, key_dim=1, value_dim=1, sequences=sequences,
+                                     length=length, decay=b["decay"], **{**still, **kw})
+        f = _lib.lib().zjai_linear_attention_step if step else _lib.lib().zjai_linear_attention_noalloc
+        return f(eng.handle, ctypes.byref(d))
+
+    assert code(1, 1, (1 << 30) + 1) == _lib.E_LIMIT
+    for length in (1, 6):
+        assert code(1, (1 << 22) + 1, length) == _lib.E_LIMIT
+        assert code(1 << 12, (1 << 10) + 1, length) == _lib.E_LIMIT
+        assert code(2**31 - 1, 2**31 - 1, length, out_sequence=2**40) == _lib.E_LIMIT
+    assert code(1, (1 << 22) + 1, 1, step=True, state_in=b["s0"], state_out=b["s0"]) == _lib.E_LIMIT
+    eng.sync()
+
+
 # ------------------------------------------------------------------------- single positions
 def run_step(eng, prec, n, heads, dk, dv, num_slots, slots, in_place, seed=11):
     qkv, out, decay, _ = inputs(seed, prec, n, 1, heads, dk, dv)

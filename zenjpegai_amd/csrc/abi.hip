@@ -561,19 +561,22 @@ void check_linear_dims(int heads, int dk, int dv) {
         throw Error(ZJAI_E_UNSUPPORTED, "linear attention: more than 128 key or 1024 value channels per head");
 }
 
+// LIN_MAX_HEADS keeps a grid below 2^32 lanes (256 for 128 value columns of the recurrent form, up to 512 of the
+// chunked one, the sequences up to a multiple of eight), LIN_MAX_LENGTH a position plus a segment in an int.
 void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype, bool recurrent = false) {
+    if (a.length > LIN_MAX_LENGTH) throw Error(ZJAI_E_LIMIT, "linear attention: more than 2^30 positions");
+    if ((double)a.seqs * a.heads * ((a.dv + 127) / 128) > LIN_MAX_HEADS)
+        throw Error(ZJAI_E_LIMIT, "linear attention: more than 2^22 heads of sequences");
     const double n = (double)a.seqs * a.length, hs = (double)a.heads * a.dk * a.dv;
     const double bytes = n * a.heads * dtype_size(dtype) * (2.0 * a.dk + 2.0 * a.dv) +
                          4.0 * a.seqs * hs * ((a.s_in != nullptr) + (a.s_out != nullptr));
     const double flops = 4.0 * n * hs;
     if (recurrent || linear_prefers_recurrent(a)) {
-        if (linear_recurrent_groups(a) > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
         LaunchScope sc(C, linear_recurrent_name(a, dtype), flops, bytes);
         ZJAI_HIP(launch_linear_recurrent(a, dtype, C.stream));
         return;
     }
     const LinChunkPlan p = linear_chunk_plan(a, CONTEXT_SCRATCH_BYTES);
-    if (((double)a.seqs * p.segments + 8) * p.units > INT32_MAX) throw Error(ZJAI_E_LIMIT, "linear attention: too many sequences");
     float* scratch = (float*)C.top().scratch;
     const double states = 4.0 * a.seqs * (p.segments - 1) * p.units * p.width * p.width;
     if (p.segments > 1) {

@@ -167,7 +167,7 @@ RecurrentPlan recurrent_plan(const LinAttnArgs& a) {
 
 template <typename T, bool V4>
 void recurrent_nr(const LinAttnArgs& a, const RecurrentPlan& p, hipStream_t s) {
-    const dim3 grid((unsigned)linear_recurrent_groups(a));
+    const dim3 grid((unsigned)(p.tiles * a.heads * a.seqs));
     switch (p.nr) {
         case 1: k_linear_recurrent<T, V4, 1><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles); break;
         case 2: k_linear_recurrent<T, V4, 2><<<grid, 256, 0, s>>>(a, p.cl_log2, p.tiles); break;
@@ -287,6 +287,16 @@ __device__ __forceinline__ void lin_scores_f32(f32x4 (&c)[2][2], const f32x4 (&a
             LA4(0), LA4(1), LB4(0), LB4(1))
 }
 
+// One of those tiles.
+template <bool F16>
+__device__ __forceinline__ void lin_score(f32x4& c, const u32x4& a, const u32x4& b, bool zero) {
+    if constexpr (F16) {
+        LIN_ASM(LZ(LIN_F16, 0, 0, 0) ZJAI_WAIT, LM(LIN_F16, 0, 0, 0) ZJAI_WAIT, ([c0] "=&v"(c)), ([c0] "+v"(c)), [a0] "v"(a), [b0] "v"(b))
+    } else {
+        LIN_ASM(LZ(ZJAI_MF, 0, 0, 0) ZJAI_WAIT, LM(ZJAI_MF, 0, 0, 0) ZJAI_WAIT, ([c0] "=&v"(c)), ([c0] "+v"(c)), [a0] "v"(a), [b0] "v"(b))
+    }
+}
+
 // o[n][i] += a[n] b[i]: tiles of the state or of the values (one or two to a wave) with the queries or their products.
 #define LO1(X, MF, p, q) X(MF, 00, 0##p, 0##q) X(MF, 01, 0##p, 1##q)
 #define LO2(X, MF, p, q) LO1(X, MF, p, q) X(MF, 10, 1##p, 0##q) X(MF, 11, 1##p, 1##q)
@@ -327,12 +337,11 @@ __device__ __forceinline__ void lin_outputs_f32(f32x4 (&c)[NV][2], const f32x4 (
         LIN_ASM(R4(LO2, LZ), R4(LO2, LM), OZ2, OC2, A2(0), A2(1), A2(2), A2(3), LB4(0), LB4(1))
     }
 }
-// c += a b: the later sixteen values, which only the later sixteen queries see.
+// c += a b: one tile.
 #define LL(X, MF, p, q) X(MF, 0, p, q)
-__device__ __forceinline__ void lin_late_f32(f32x4& c, const f32x4& a, const f32x4& b) {
-    asm("s_nop 1\n\t" R4(LL, LM)
-        : [c0] "+v"(c)
-        : [a0] "v"(a[0]), [a1] "v"(a[1]), [a2] "v"(a[2]), [a3] "v"(a[3]), [b0] "v"(b[0]), [b1] "v"(b[1]), [b2] "v"(b[2]), [b3] "v"(b[3]));
+__device__ __forceinline__ void lin_tile_f32(f32x4& c, const f32x4& a, const f32x4& b, bool zero = false) {
+    LIN_ASM(R4(LL, LZ), R4(LL, LM), ([c0] "=&v"(c)), ([c0] "+v"(c)), [a0] "v"(a[0]), [a1] "v"(a[1]), [a2] "v"(a[2]), [a3] "v"(a[3]),
+            [b0] "v"(b[0]), [b1] "v"(b[1]), [b2] "v"(b[2]), [b3] "v"(b[3]))
 }
 
 // c[m][n] += a[m] b[n]: two key tiles of the state.
@@ -496,7 +505,11 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
     if (OUT ? begin > len || (begin == len && seg > 0) : begin + c.seg_len >= len) return;
     const int head = unit / c.tiles, col0 = unit % c.tiles * D;
     const int colw = col0 + wave * 16 * NV;   // the wave's value columns
-    const bool work = colw < a.dv;
+    // Four waves share the query products: each of three makes one tile of them, weighed and in pieces, in LDS, at the
+    // price of one more barrier a chunk (12 ragged f16 sequences of 64 channels 84 -> 78 us, 65536 positions of 128
+    // bf16 channels 421 -> 410 us). The two waves of 32 channels would save half a tile's work each and make their own.
+    constexpr bool SHARE = OUT && D > 32;
+    const bool work = SHARE || colw < a.dv;
 
     const T* kp = (const T*)a.k.p + (long long)seq * a.k.seq + (long long)head * a.dk;
     const T* vp = (const T*)a.v.p + (long long)seq * a.v.seq + (long long)head * a.dv + col0;
@@ -550,6 +563,8 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 
     // The head's powers g^0..g^63, one a lane, then those a lane's rows and columns need.
     float* s_pow = (float*)(s_lds + lin_lds_planes<T>(OUT) * PLANE) + wave * 64;
+    u32x4* s_p = (u32x4*)((float*)(s_lds + lin_lds_planes<T>(OUT) * PLANE) + lin_waves(D, OUT) * 64);
+    if (SHARE && !F32 && wave == 0) s_p[lane] = s_p[64 + lane] = u32x4{0, 0, 0, 0};  // products with later positions
     s_pow[lane] = lin_pow(lin_log2(a.decay[head]), lane);
     __syncthreads();
     float w_v[8], w_o[2], w_d[4], w_n[4], g_c = s_pow[LC];
@@ -719,6 +734,41 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
             }
             f32x4 O[NV][2];  // O[n][i], transposed: rows are value columns 16 n + 4 g + r, columns positions 16 i + l16
             f32x4 pt[2][2];  // pt[j][i]: rows are positions j of the keys, columns positions i of the queries
+            const auto weighed = [&](const f32x4& t, int j, int i) {
+                f32x4 p;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)  // a select: products with later positions may be infinite
+                    p[r] = j != i ? t[r] * w_n[r] : 4 * g + r <= l16 ? t[r] * w_d[r] : 0.0f;
+                return p;
+            };
+            if constexpr (SHARE) {
+                const int j = wave == 2, i = wave >= 1;
+                if (wave < 3) {
+                    f32x4 tile;
+#pragma unroll
+                    for (int s = 0; s < (F32 ? MT : KS); ++s) {
+                        if constexpr (F32) {
+                            lin_tile_f32(tile, *(const f32x4*)(f_k + (16 * j + l16) * ROW + (4 * s + g) * 4),
+                                         *(const f32x4*)(f_q + (16 * i + l16) * ROW + (4 * s + g) * 4), s == 0);
+                        } else {
+                            const unsigned short* kr = s_k + (16 * j + l16) * ROW + 32 * s + 4 * g;
+                            const u32x2 k_lo = *(const u32x2*)kr, k_hi = *(const u32x2*)(kr + 16);
+                            lin_score<F16>(tile, u32x4{k_lo[0], k_lo[1], k_hi[0], k_hi[1]},
+                                           *(const u32x4*)(s_q + (16 * i + l16) * ROW + (4 * s + g) * 8), s == 0);
+                        }
+                    }
+                    const f32x4 p = weighed(tile, j, i);
+                    if constexpr (F32) {
+                        s_p[wave * 64 + lane] = __builtin_bit_cast(u32x4, p);
+                    } else {
+                        const float z[8] = {p[0], p[1], p[2], p[3], 0.0f, 0.0f, 0.0f, 0.0f};
+                        u32x4 q[2];
+                        lin_split<2>(z, q);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) ((u32x2*)(s_p + (2 * i + n) * 64 + lane))[j] = u32x2{q[n][0], q[n][1]};
+                    }
+                }
+            }
             if constexpr (F32) {
 #pragma unroll
                 for (int s = 0; s < MT; ++s) {
@@ -726,10 +776,10 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int at = (16 * i + l16) * ROW + (4 * s + g) * 4;
-                        kf[i] = *(const f32x4*)(f_k + at);
+                        if (!SHARE) kf[i] = *(const f32x4*)(f_k + at);
                         qf[i] = *(const f32x4*)(f_q + at);
                     }
-                    lin_scores_f32(pt, kf, qf, s == 0);
+                    if (!SHARE) lin_scores_f32(pt, kf, qf, s == 0);
                     lin_outputs_f32<NV>(O, S[s], qf, s == 0);
                 }
             } else {
@@ -740,11 +790,13 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
                     for (int i = 0; i < 2; ++i) {
                         const unsigned short* qr = s_q + (16 * i + l16) * ROW + (4 * s + g) * 8;
                         const unsigned short* kr = s_k + (16 * i + l16) * ROW + 32 * s + 4 * g;
-                        qf[i] = *(const u32x4*)qr;
+                        if (!SHARE || !F16) qf[i] = *(const u32x4*)qr;
 #pragma unroll
                         for (int n = 0; n < QP; ++n) qp[i][n] = F16 ? *(const u32x4*)(qr + (n + 1) * PLANE) : qf[i];
-                        const u32x2 k_lo = *(const u32x2*)kr, k_hi = *(const u32x2*)(kr + 16);
-                        kf[i] = u32x4{k_lo[0], k_lo[1], k_hi[0], k_hi[1]};
+                        if (!SHARE) {
+                            const u32x2 k_lo = *(const u32x2*)kr, k_hi = *(const u32x2*)(kr + 16);
+                            kf[i] = u32x4{k_lo[0], k_lo[1], k_hi[0], k_hi[1]};
+                        }
                     }
 #pragma unroll
                     for (int n = 0; n < NV; ++n) {
@@ -753,7 +805,7 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
                         for (int r = 0; r < 4; ++r) z[r] = S[2 * s][n][r], z[4 + r] = S[2 * s + 1][n][r];
                         lin_split<2>(z, sf[n]);
                     }
-                    lin_scores<F16>(pt, kf, qf, s == 0);
+                    if (!SHARE) lin_scores<F16>(pt, kf, qf, s == 0);
                     lin_outputs<NV>(O, sf, qp, s == 0);
                 }
             }
@@ -763,31 +815,39 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) O[n][i][r] *= w_o[i];
-            // Weighted query products of positions 16 i + l16 with the positions j.
-            float p0[8], p1[8];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool seen = 4 * g + r <= l16;  // a select: products with later positions may be infinite
-                p0[r] = seen ? pt[0][0][r] * w_d[r] : 0.0f;
-                p0[4 + r] = 0.0f;
-                p1[r] = pt[0][1][r] * w_n[r];
-                p1[4 + r] = seen ? pt[1][1][r] * w_d[r] : 0.0f;
-            }
+            // The weighed query products of positions 16 i + l16 with the positions j.
+            if (SHARE) __syncthreads();
             if constexpr (F32) {
-                const f32x4 p[2] = {{p0[0], p0[1], p0[2], p0[3]}, {p1[0], p1[1], p1[2], p1[3]}};
+                f32x4 p[2], p11;
+                if constexpr (SHARE) {
+                    p[0] = __builtin_bit_cast(f32x4, s_p[lane]);
+                    p[1] = __builtin_bit_cast(f32x4, s_p[64 + lane]);
+                    p11 = __builtin_bit_cast(f32x4, s_p[128 + lane]);
+                } else {
+                    p[0] = weighed(pt[0][0], 0, 0);
+                    p[1] = weighed(pt[0][1], 0, 1);
+                    p11 = weighed(pt[1][1], 1, 1);
+                }
                 f32x4 early[NV];
 #pragma unroll
                 for (int n = 0; n < NV; ++n) early[n] = f32x4{x[n][0], x[n][1], x[n][2], x[n][3]};
                 lin_outputs_f32<NV>(O, early, p);
 #pragma unroll
-                for (int n = 0; n < NV; ++n)
-                    lin_late_f32(O[n][1], f32x4{x[n][4], x[n][5], x[n][6], x[n][7]}, f32x4{p1[4], p1[5], p1[6], p1[7]});
+                for (int n = 0; n < NV; ++n) lin_tile_f32(O[n][1], f32x4{x[n][4], x[n][5], x[n][6], x[n][7]}, p11);
             } else {
                 u32x4 vf[NV][QP], P[2][2];
 #pragma unroll
                 for (int n = 0; n < NV; ++n) lin_split<QP>(x[n], vf[n]);
-                lin_split<2>(p0, P[0]);
-                lin_split<2>(p1, P[1]);
+                if constexpr (SHARE) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) P[i >> 1][i & 1] = s_p[i * 64 + lane];
+                } else {
+                    const f32x4 p00 = weighed(pt[0][0], 0, 0), p01 = weighed(pt[0][1], 0, 1), p11 = weighed(pt[1][1], 1, 1);
+                    const float z0[8] = {p00[0], p00[1], p00[2], p00[3], 0.0f, 0.0f, 0.0f, 0.0f};
+                    const float z1[8] = {p01[0], p01[1], p01[2], p01[3], p11[0], p11[1], p11[2], p11[3]};
+                    lin_split<2>(z0, P[0]);
+                    lin_split<2>(z1, P[1]);
+                }
                 lin_outputs<NV>(O, vf, P);
             }
             if (poison) {
@@ -950,7 +1010,7 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
 template <typename T, int D, bool OUT>
 void chunks_d(const LinChunkArgs& c, const dim3& grid, hipStream_t s) {
     constexpr int threads = 64 * lin_waves(D, OUT);
-    const size_t lds = lin_lds_planes<T>(OUT) * LC * lin_row<T>(D) * 2 + threads * 4;
+    const size_t lds = lin_lds_planes<T>(OUT) * LC * lin_row<T>(D) * 2 + threads * 4 + (OUT && D > 32 ? 4 * 64 * 16 : 0);
     k_linear_chunks<T, D, OUT><<<grid, threads, lds, s>>>(c);
 }
 template <typename T, bool OUT>
@@ -971,8 +1031,6 @@ hipError_t chunks_of(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, flo
 }
 
 }  // namespace
-
-long long linear_recurrent_groups(const LinAttnArgs& a) { return (long long)recurrent_plan(a).tiles * a.heads * a.seqs; }
 
 std::string linear_recurrent_name(const LinAttnArgs& a, int dtype) {
     const RecurrentPlan p = recurrent_plan(a);
@@ -1000,7 +1058,9 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     // fewer, k and v are read twice, and two waves to a SIMD pay for it (65536 positions, 64 waves: in 16 segments
     // 636 us, in 32 434); with lengths, half of the segments may be empty (12 ragged sequences of up to 3001: six
     // segments 88 us, eleven 83). A segment has at least as many bytes of channels as of state: 4096 positions in
-    // five heads of 32, f32: one chunk a segment 15.4 us, two 16.8.
+    // five heads of 32, f32: one chunk a segment 15.4 us, two 16.8. The context's 33 MiB hold what 2048 waves ask for;
+    // ragged batches of the widest heads get half of theirs (in 80 MiB, 12 sequences of up to 3001 in eight heads
+    // of 128, f16: 126 us instead of 119; 6 of up to 9000 126 instead of 144, 30 of up to 4000 296 instead of 265).
     const long long want = waves >= 1024 ? 1 : ((a.lengths ? 4096 : 2048) + waves - 1) / waves;
     const long long n = std::max(std::min(std::min(std::min(want, 1024LL), chunks * 32 / p.width), (long long)(scratch_bytes / state) + 1), 1LL);
     const long long per = std::max((chunks + n - 1) / n, 1LL);

@@ -147,7 +147,7 @@ struct LinAttnArgs {
     const float* s_in;
     float* s_out;
 };
-constexpr int LIN_MAX_KEY = 128, LIN_MAX_VALUE = 1024;
+constexpr int LIN_MAX_KEY = 128, LIN_MAX_VALUE = 1024, LIN_MAX_LENGTH = 1 << 30, LIN_MAX_HEADS = 1 << 22;  // heads: of all sequences
 // The chunked form: `segments` stretches of each sequence (a multiple of 32 positions each, the last one shorter)
 // run side by side; with more than one, `scratch` holds linear_scratch_bytes.
 struct LinChunkPlan {
@@ -162,7 +162,6 @@ hipError_t launch_linear_sums(const LinAttnArgs& a, const LinChunkPlan& p, int d
 hipError_t launch_linear_scan(const LinAttnArgs& a, const LinChunkPlan& p, float* scratch, hipStream_t s);
 hipError_t launch_linear_outputs(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, const float* scratch, hipStream_t s);
 // The recurrent form: a workgroup keeps its part of a state in registers over the positions.
-long long linear_recurrent_groups(const LinAttnArgs& a);
 std::string linear_recurrent_name(const LinAttnArgs& a, int dtype);
 hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t s);
 // Norm, gate, residual scale, residual sum and norm of each position (zjai_norm_gate_residual): views of

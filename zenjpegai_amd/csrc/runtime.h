@@ -147,7 +147,7 @@ struct Context {
 // weight (half its f32 size; dim <= 639 by the Gram kernel's LDS stage), so that maps up to the
 // documented size fit as they do in f32 form.
 constexpr size_t SCRATCH_PIECE_BYTES = 1u << 20;
-constexpr size_t CONTEXT_SCRATCH_BYTES = 80u << 20;
+constexpr size_t CONTEXT_SCRATCH_BYTES = 33u << 20;
 // A context's scratch on the current device. The last one given back stays for the next context of its
 // device (one array per device, until the process ends): a program that makes a context per picture would
 // otherwise pay for the allocation, and for what freeing 33 MiB costs the allocations after it, each time.
