@@ -644,6 +644,7 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
         }
     };
 
+    T* po = OUT && a.width == 0 ? op + (begin + l16) * a.o.pos : op;  // the output of position pos + l16
     float ahead = 1.0f;  // sums: g^(positions of the segment after this chunk)
     for (int pos = OUT ? begin : end - LC; OUT ? pos < end : pos >= begin; pos += STEP) {
         __syncthreads();
@@ -865,8 +866,11 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
             for (int i = 0; i < 2; ++i) {
                 const int p = pos + 16 * i + l16;
                 if (p >= end) continue;
-                const int y = a.width ? p / a.width : 0, at = a.width ? p - y * a.width : p;
-                T* o = op + (y * a.o.row + at * a.o.pos);
+                T* o = po + i * 16 * a.o.pos;
+                if (a.width) {
+                    const int y = p / a.width;
+                    o = op + (y * a.o.row + (p - y * a.width) * a.o.pos);
+                }
 #pragma unroll
                 for (int n = 0; n < NV; ++n) {
                     const int cc = 16 * n + 4 * g;
@@ -880,6 +884,7 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
                 }
             }
         }
+        if (OUT && a.width == 0) po += LC * a.o.pos;
         if (!update) continue;
 #pragma unroll
         for (int m = 0; m < MT; m += 2) {
@@ -958,7 +963,10 @@ __global__ void __launch_bounds__(1024) k_linear_scan(LinChunkArgs c, int quads,
     const int lane = threadIdx.x % width, part = threadIdx.x / width, q = blockIdx.x * width + lane;
     const int unit = blockIdx.y % c.units, seq = blockIdx.y / c.units;
     const float g = lin_pow(lin_log2(c.a.decay[unit / c.tiles]), c.seg_len);
-    const int s0 = part * SCAN_SEGS, n = c.segments - 1 - s0;
+    // A sequence has the sums of its segments but the last.
+    const int len = c.a.lengths ? max(0, min(c.a.lengths[seq], c.a.length)) : c.a.length, sums = max(len - 1, 0) / c.seg_len;
+    if (sums < 2) return;
+    const int s0 = part * SCAN_SEGS, n = sums - s0;
     f32x4* x = (f32x4*)c.scratch + (((size_t)seq * (c.segments - 1) + s0) * c.units + unit) * quads + q;
     const size_t step = (size_t)c.units * quads;
     f32x4 v[SCAN_SEGS];
