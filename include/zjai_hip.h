@@ -259,11 +259,11 @@ ZJAI_API int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv, 
  * context model of this form can be evaluated over a whole map of known latents at once (the
  * encoder) or position by position as they are decoded, with the same result up to rounding. It has
  * no counterpart in the reference, whose channel attention (src/nn/fast/math.rs:512) has the same
- * cost, linear in the positions, but is not causal. Sums and states are f32
- * whatever the precision, and so are the products, except that whole sequences of more than five f16 or bf16
- * positions take states and weighted products into the next product with 16 bits (2^-16 of each). A non-finite q, k or v reaches the outputs of its own position
- * and later ones only (infinities may arrive there as NaN), a non-finite state_in every output of its
- * head.
+ * cost, linear in the positions, but is not causal. Sums and states are f32 whatever the
+ * precision, and so are the products, except that whole sequences of f16 or bf16 may take states and
+ * weighted products into the next product with 16 bits (2^-16 of each). A non-finite q, k or v
+ * reaches the outputs of its own position and later ones only (infinities may arrive there as NaN), a
+ * non-finite state_in every output of its head.
  *
  * zjai_linear_attention takes a map of packed channels, [q | k | v] of heads * key_dim, heads *
  * key_dim and heads * value_dim channels, the heads one after another in each (value_dim is what the

@@ -349,6 +349,13 @@ def test_more_than_a_launch_takes_is_refused_before_anything_is_read(eng):
     eng.sync()
 
 
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("keep", [(False, False), (False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("length", [2, 3, 4, 5, 6])
+def test_short_sequences_with_and_without_states(eng, prec, keep, length):
+    run_whole(eng, prec, 3, length, 2, 24, 40, lengths=[length, 1, length - 1], keep=keep, seed=70 + length)
+
+
 # ------------------------------------------------------------------------- single positions
 def run_step(eng, prec, n, heads, dk, dv, num_slots, slots, in_place, seed=11):
     qkv, out, decay, _ = inputs(seed, prec, n, 1, heads, dk, dv)

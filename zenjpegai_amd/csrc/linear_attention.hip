@@ -471,10 +471,10 @@ template <typename T> __host__ __device__ constexpr int lin_lds_planes(bool out)
     return sizeof(T) == 4 ? (out ? 6 : 4) : Elem<T>::dt == DT_F16 ? (out ? 5 : 2) : (out ? 3 : 2);
 }
 
-// D: channels of a unit; a wave has one 16-column tile of its values or, for the outputs of the widest, two: each of
-// its waves weighs all query products, and with eight waves to a unit (instead of four) that and a barrier
-// between so many cost more than the registers of one tile less give (65536 positions, 16 heads, bf16: 365 us, with two tiles
-// 288). The sums have no such products, and more waves load more (150 us with two tiles, 113 with one).
+// D: channels of a unit; a wave has one 16-column tile of its values or, for the outputs of the widest, two: with
+// eight waves to a unit instead of four, what the waves share and the barriers between so many cost more than the
+// registers of one tile less give (65536 positions, 16 heads, bf16: 451 us, with two tiles 408; held to 128
+// registers 526). The sums have no query products, and more waves load more (two tiles 150 us, one 113).
 constexpr int lin_tiles(int d, bool out) { return out && d == 128 ? 2 : 1; }
 constexpr int lin_waves(int d, bool out) { return d / 16 / lin_tiles(d, out); }
 template <typename T, int D, bool OUT>
@@ -1051,10 +1051,11 @@ hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t 
     return recurrent<__bf16>(a, s);
 }
 
-// A position takes the recurrent form 0.8 to 2.7 us, a chunk costs its 32 positions whether they are there or not (one
-// sequence of 4 heads of 32, f32: 4 positions 5.4 against 6.3 us, 8 8.7; 500 of 4 heads of 32 x 64, f16: 14.1
-// against 19.3, 8 22).
-bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= 5; }
+// A position takes the recurrent form 0.8 to 2.7 us, a chunk costs its 32 positions whether they are there or not, but a
+// state is read and written faster by the recurrent form (both, us: one f32 sequence of 4 heads of 32, no
+// states: 3 positions 4.7 and 4.7, 4 5.5 and 4.7; with states 5 6.5 and 6.6, 6 7.2 and 6.5; 500 f16 sequences of 4
+// heads of 32 x 64 with states: 5 16.0 and 19.7, 7 20.1 and 19.7; 500 of 8 heads of 64, none: 3 16.5 and 21.8, 6 28.1 and 22.1).
+bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= (a.s_in || a.s_out ? 5 : 3); }
 
 LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     LinChunkPlan p;
@@ -1062,11 +1063,11 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     p.units = a.heads * ((a.dv + p.width - 1) / p.width);
     const long long waves = (long long)a.seqs * p.units * (p.width / 32), chunks = (a.length + LC - 1) / LC;
     const long long state = (long long)a.seqs * p.units * p.width * p.width * 4;
-    // A wave for every SIMD needs no segments (1080 waves of 240 positions: 21.6 us, in two segments 26.8). With
+    // A wave for every SIMD needs no segments (2160 waves of 240 positions: 16.6 us, in two segments 22.4). With
     // fewer, k and v are read twice, and two waves to a SIMD pay for it (65536 positions, 64 waves: in 16 segments
-    // 636 us, in 32 434); with lengths, half of the segments may be empty (12 ragged sequences of up to 3001: six
-    // segments 88 us, eleven 83). A segment has at least as many bytes of channels as of state: 4096 positions in
-    // five heads of 32, f32: one chunk a segment 15.4 us, two 16.8. The context's 33 MiB hold what 2048 waves ask for;
+    // 490 us, in 32 404); with lengths, half of the segments may be empty (12 ragged sequences of up to 3001: six
+    // segments 77 us, eleven 71). A segment has at least as many bytes of channels as of state: 4096 positions in
+    // five heads of 32, f32: one chunk a segment 16.4 us, two 17.5. The context's 33 MiB hold what 2048 waves ask for;
     // ragged batches of the widest heads get half of theirs (in 80 MiB, 12 sequences of up to 3001 in eight heads
     // of 128, f16: 126 us instead of 119; 6 of up to 9000 126 instead of 144, 30 of up to 4000 296 instead of 265).
     const long long want = waves >= 1024 ? 1 : ((a.lengths ? 4096 : 2048) + waves - 1) / waves;
