@@ -241,9 +241,11 @@ ZJAI_API int32_t zjai_channel_attention(zjai_ctx* ctx, const zjai_tensor* qkv, i
  * [h][w][channels] (channels = 3 * dim: q, k, v), out [h][w][dim]; temperature is a device array
  * of `heads` floats. The work is enqueued on the context's stream (zjai_sync waits for it) and
  * allocates nothing: its scratch (Gram partial sums, attention matrix, folded weight) is an array
- * of 33 MiB, of which it uses ZJAI_NOALLOC_SCRATCH_BYTES (and 1 MiB beside them), that zjai_ctx_create
- * takes for the context (new, or the one that the last destroyed context of the device left), so calls on several contexts may overlap on one GPU. A map that needs more scratch (with
- * dim 128 and 4 heads: more than ~240k positions) returns ZJAI_E_LIMIT before anything is launched. */
+ * of 33 MiB, of which it uses ZJAI_NOALLOC_SCRATCH_BYTES (and 1 MiB beside them), that
+ * zjai_ctx_create takes for the context (new, or the one that the last destroyed context of the
+ * device left), so calls on several contexts may overlap on one GPU. A map that needs more scratch
+ * (with dim 128 and 4 heads: more than ~240k positions) returns ZJAI_E_LIMIT before anything is
+ * launched. */
 #define ZJAI_NOALLOC_SCRATCH_BYTES (16u << 20)
 ZJAI_API int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv, int32_t channels,
                                                 int32_t h, int32_t w, int32_t heads,
@@ -299,7 +301,8 @@ typedef struct zjai_linear_attention_desc {
 } zjai_linear_attention_desc;
 
 /* Whole sequences. desc->slots must be NULL. Enqueued on the context's stream (zjai_sync waits for
- * it); works in the context's scratch, as zjai_channel_attention_noalloc, and allocates nothing. */
+ * it); works in the context's scratch, as zjai_channel_attention_noalloc, and allocates nothing: a
+ * graph it is captured into must not run at the same time as another call of the context. */
 ZJAI_API int32_t zjai_linear_attention_noalloc(zjai_ctx* ctx, const zjai_linear_attention_desc* desc);
 /* The recurrent form: one position of each sequence (length 1, lengths NULL, both states given).
  * Sequence i reads state_in[slots[i]] and writes state_out[slots[i]]; states of other slots stay as
