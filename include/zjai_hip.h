@@ -265,7 +265,8 @@ ZJAI_API int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv, 
  * precision, and so are the products, except that whole sequences of f16 or bf16 may take states and
  * weighted products into the next product with 16 bits (2^-16 of each). A non-finite q, k or v
  * reaches the outputs of its own position and later ones only (infinities may arrive there as NaN), a
- * non-finite state_in every output of its head.
+ * non-finite state_in every output of its head. (q . k of two positions, which whole sequences form
+ * before they meet v, has to stay within f32's range.)
  *
  * zjai_linear_attention takes a map of packed channels, [q | k | v] of heads * key_dim, heads *
  * key_dim and heads * value_dim channels, the heads one after another in each (value_dim is what the

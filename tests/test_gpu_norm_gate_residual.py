@@ -143,6 +143,41 @@ def test_position_counts(eng, n, c):
     run(eng, "bf16", n, c, act="silu")
 
 
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,c", [(700, 64), (33, 1000), (1, 24)])
+def test_one_gate_for_all_positions_and_interleaved_outputs(eng, prec, n, c):
+    """x and the gate are one row each (stride 0); x_out and h alternate in one buffer."""
+    rng = np.random.default_rng(c)
+    x, g = (to_raw(rng.standard_normal((1, c)), prec) for _ in range(2))
+    y = to_raw(rng.standard_normal((n, c)), prec)
+    dx, dg, dy = DevBuf(x), DevBuf(g), DevBuf(y)
+    both = DevBuf(to_raw(np.zeros((n, 2, c)), prec))
+    es = 4 if prec == "f32" else 2
+    nn.norm_gate_residual_noalloc(eng, nn.norm_gate_residual_desc(
+        prec, dx, dy, dg, both, both.address + c * es, positions=n, channels=c, gate_act="sigmoid", post_norm="rms",
+        post_eps=POST_EPS, pre_norm="layer", pre_eps=PRE_EPS, x_stride=0, gate_stride=0, x_out_stride=2 * c, h_stride=2 * c))
+    eng.sync()
+    f = [np.broadcast_to(from_raw(a, prec), (n, c)) for a in (x, y, g)]
+    (xo, ex), (h, eh) = oracle_join(*f, "sigmoid", "rms", 1, "layer", None, None, None, None, None)
+    got = both.get()
+    near(got[:, 0], prec, xo, ex)
+    near(got[:, 1], prec, h, eh)
+
+
+@pytest.mark.parametrize("prec", ["f32", "bf16"])
+@pytest.mark.parametrize("n,c", [(700, 64), (40, 2000)])
+def test_h_in_the_place_of_x(eng, prec, n, c):
+    rng = np.random.default_rng(c + 1)
+    x, y = (to_raw(rng.standard_normal((n, c)), prec) for _ in range(2))
+    dx, dy, dxo = DevBuf(x), DevBuf(y), DevBuf(y)
+    nn.norm_gate_residual_noalloc(eng, nn.norm_gate_residual_desc(prec, dx, dy, None, dxo, dx, positions=n, channels=c,
+                                                                  post_norm="layer", post_eps=POST_EPS, pre_norm="rms", pre_eps=PRE_EPS))
+    eng.sync()
+    (xo, ex), (h, eh) = oracle_join(from_raw(x, prec), from_raw(y, prec), None, "linear", "layer", 1, "rms", None, None, None, None, None)
+    near(dxo.get(), prec, xo, ex)
+    near(dx.get(), prec, h, eh)
+
+
 def test_a_position_with_an_infinity_leaves_the_others_alone(eng):
     n, c, prec = 40, 96, "f32"
     rng = np.random.default_rng(3)
