@@ -581,7 +581,10 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 
     // The state before the segment: S[m][n][r] is key channel 16 m + 4 g + r of value column 16 n + l16.
     f32x4 S[MT][NV];
+    // Where it is in the caller's arrays: the row by scalar arithmetic (one that exists), the lane's part added.
     const long long sbase = ((long long)seq * a.heads + head) * a.dk;
+    const auto s_row = [&](int row) { return (sbase + min(row, a.dk - 1)) * a.dv + col0; };
+    const unsigned s_lane = 4 * g * a.dv + colw - col0 + l16;
     const size_t xunit = (size_t)D * D;
     float* const x_seq = c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * xunit + (size_t)(wave * NV * 64 + lane) * 4;
     const size_t x_seg = c.units * xunit;
@@ -589,21 +592,36 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (seg == 0) {
-                if (a.s_in && work)
+        for (int n = 0; n < NV; ++n) S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // One branch for all tiles, so that their loads are issued together (a branch for each: 16 waits one after
+    // another for 128 channels, 6 positions with states 14.3 us).
+    if (OUT && seg > 0) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int kk = 16 * m + 4 * g + r, vv = colw + 16 * n + l16;
-                        const bool in = kk < a.dk && vv < a.dv;
-                        const float x = a.s_in[in ? (sbase + kk) * a.dv + vv : 0];
-                        S[m][n][r] = in ? OUT ? x : x * g_seg : 0.0f;
-                    }
-            } else if (OUT) {
-                S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (m * (D / 16) + n) * 256);
-            }
-        }
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NV; ++n) S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (m * (D / 16) + n) * 256);
+    } else if (seg == 0 && a.s_in && work) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool in = 16 * m + 4 * g + r < a.dk && colw + 16 * n + l16 < a.dv;
+                    S[m][n][r] = a.s_in[s_row(16 * m + r) + (in ? s_lane + 16 * n : 0)];
+                }
+        int keys = a.dk, values = a.dv;  // compared again: 64 masks kept over the loads leave no scalar registers
+        asm("" : "+s"(keys), "+s"(values));
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool in = 16 * m + 4 * g + r < keys && colw + 16 * n + l16 < values;
+                    S[m][n][r] = in ? OUT ? S[m][n][r] : S[m][n][r] * g_seg : 0.0f;
+                }
+    }
 
     const auto stage = [&]() {
 #pragma unroll
@@ -935,15 +953,12 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
         if (!a.s_out || end != len || !work) return;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int vv = colw + 16 * n + l16;
-            if (vv >= a.dv) continue;
+            if (colw + 16 * n + l16 >= a.dv) continue;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int kk = 16 * m + 4 * g + r;
-                    if (kk < a.dk) a.s_out[(sbase + kk) * a.dv + vv] = S[m][n][r];
-                }
+                for (int r = 0; r < 4; ++r)
+                    if (16 * m + 4 * g + r < a.dk) a.s_out[s_row(16 * m + r) + s_lane + 16 * n] = S[m][n][r];
         }
     } else {
 #pragma unroll
