@@ -1066,10 +1066,11 @@ hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t 
     return recurrent<__bf16>(a, s);
 }
 
-// A position takes the recurrent form 0.8 to 2.7 us, a chunk costs its 32 positions whether they are there or not, but a
+// A position takes the recurrent form 0.7 to 3 us, a chunk costs its 32 positions whether they are there or not, but a
 // state is read and written faster by the recurrent form (both, us: one f32 sequence of 4 heads of 32, no
-// states: 3 positions 4.7 and 4.7, 4 5.5 and 4.7; with states 5 6.5 and 6.6, 6 7.2 and 6.5; 500 f16 sequences of 4
-// heads of 32 x 64 with states: 5 16.0 and 19.7, 7 20.1 and 19.7; 500 of 8 heads of 64, none: 3 16.5 and 21.8, 6 28.1 and 22.1).
+// states: 3 positions 4.7 and 4.7, 4 5.5 and 4.7; with states 4 5.8 and 6.1, 6 7.1 and 6.1; 500 f16 sequences of
+// 4 heads of 32 x 64 with states: 5 16.0 and 18.4; 64 bf16 ones of 16 heads of 128: 5 37.9 and 39.3, 6 41.0 and 39.7;
+// 500 f16 ones of 8 heads of 64 without: 3 16.5 and 21.8, 6 28.1 and 22.1).
 bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= (a.s_in || a.s_out ? 5 : 3); }
 
 LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
