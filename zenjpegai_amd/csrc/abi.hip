@@ -578,7 +578,7 @@ void run_linear_attention(Context& C, const LinAttnArgs& a, int dtype, bool recu
     }
     const LinChunkPlan p = linear_chunk_plan(a, CONTEXT_SCRATCH_BYTES);
     float* scratch = (float*)C.top().scratch;
-    const double states = 4.0 * a.seqs * (p.segments - 1) * p.units * p.width * p.width;
+    const double states = 4.0 * a.seqs * p.slots * p.units * p.width * p.width;
     if (p.segments > 1) {
         LaunchScope sc(C, linear_chunk_name(p, dtype, false), 2.0 * n * hs, n * a.heads * dtype_size(dtype) * (a.dk + a.dv) + states);
         ZJAI_HIP(launch_linear_sums(a, p, dtype, scratch, C.stream));

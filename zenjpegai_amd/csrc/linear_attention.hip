@@ -462,6 +462,7 @@ struct LinChunkArgs {
     LinAttnArgs a;
     float* scratch;  // sums: the state after each segment; outputs: before each but the first
     int segments, seg_len, units, tiles;
+    int slots;  // states of a sequence in it: one for each segment but the last and, in place, the state before the first
     int vec_k, vec_v, vec_o;
     int even;  // vec_k and vec_v, and head sizes of whole units
 };
@@ -586,20 +587,25 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
     const auto s_row = [&](int row) { return (sbase + min(row, a.dk - 1)) * a.dv + col0; };
     const unsigned s_lane = 4 * g * a.dv + colw - col0 + l16;
     const size_t xunit = (size_t)D * D;
-    float* const x_seq = c.scratch + ((size_t)seq * (c.segments - 1) * c.units + unit) * xunit + (size_t)(wave * NV * 64 + lane) * 4;
+    float* const x_seq = c.scratch + ((size_t)seq * c.slots * c.units + unit) * xunit + (size_t)(wave * NV * 64 + lane) * 4;
     const size_t x_seg = c.units * xunit;
     const float g_seg = OUT ? 1.0f : lin_pow(lin_log2(a.decay[head]), c.seg_len);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NV; ++n) S[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // In place, the workgroup of a sequence's last segment writes the states that the first one's outputs start from,
+    // and nothing orders the two: the sums, a launch before, keep a copy of them. (A sequence of one segment
+    // is read and written by the same lanes.)
+    const bool copied = a.s_in && a.s_in == a.s_out && len > c.seg_len;
     // One branch for all tiles, so that their loads are issued together (a branch for each: 16 waits one after
     // another for 128 channels; six positions with states 14.4 us, now 11.6).
-    if (OUT && seg > 0) {
+    if (OUT && (seg > 0 || copied)) {
+        const int slot = seg > 0 ? seg - 1 : c.segments - 1;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int n = 0; n < NV; ++n) S[m][n] = *(const f32x4*)(x_seq + (seg - 1) * x_seg + (m * (D / 16) + n) * 256);
+            for (int n = 0; n < NV; ++n) S[m][n] = *(const f32x4*)(x_seq + slot * x_seg + (m * (D / 16) + n) * 256);
     } else if (seg == 0 && a.s_in && work) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -619,8 +625,18 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const bool in = 16 * m + 4 * g + r < keys && colw + 16 * n + l16 < values;
-                    S[m][n][r] = in ? OUT ? S[m][n][r] : S[m][n][r] * g_seg : 0.0f;
+                    S[m][n][r] = in ? S[m][n][r] : 0.0f;
                 }
+        if (!OUT) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NV; ++n) {
+                    if (copied) *(f32x4*)(x_seq + (c.segments - 1) * x_seg + (m * (D / 16) + n) * 256) = S[m][n];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[m][n][r] *= g_seg;
+                }
+        }
     }
 
     const auto stage = [&]() {
@@ -982,7 +998,7 @@ __global__ void __launch_bounds__(1024) k_linear_scan(LinChunkArgs c, int quads,
     const int len = c.a.lengths ? max(0, min(c.a.lengths[seq], c.a.length)) : c.a.length, sums = max(len - 1, 0) / c.seg_len;
     if (sums < 2) return;
     const int s0 = part * SCAN_SEGS, n = sums - s0;
-    f32x4* x = (f32x4*)c.scratch + (((size_t)seq * (c.segments - 1) + s0) * c.units + unit) * quads + q;
+    f32x4* x = (f32x4*)c.scratch + (((size_t)seq * c.slots + s0) * c.units + unit) * quads + q;
     const size_t step = (size_t)c.units * quads;
     f32x4 v[SCAN_SEGS];
 #pragma unroll
@@ -1016,6 +1032,7 @@ LinChunkArgs chunk_args(const LinAttnArgs& a, const LinChunkPlan& p, int dtype, 
     c.scratch = scratch;
     c.segments = p.segments;
     c.seg_len = p.seg_len;
+    c.slots = p.slots;
     c.units = p.units;
     c.tiles = p.units / a.heads;
     const int es = dtype == DT_F32 ? 4 : 2;
@@ -1087,10 +1104,12 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     // ragged batches of the widest heads get half of theirs (in 80 MiB, 12 sequences of up to 3001 in eight heads
     // of 128, f16: 126 us instead of 119; 6 of up to 9000 126 instead of 144, 30 of up to 4000 296 instead of 265).
     const long long want = waves >= 1024 ? 1 : ((a.lengths ? 4096 : 2048) + waves - 1) / waves;
-    const long long n = std::max(std::min(std::min(std::min(want, 1024LL), chunks * 32 / p.width), (long long)(scratch_bytes / state) + 1), 1LL);
+    const int kept = a.s_in && a.s_in == a.s_out;  // states updated in place have a copy in the scratch
+    const long long n = std::max(std::min(std::min(std::min(want, 1024LL), chunks * 32 / p.width), (long long)(scratch_bytes / state) + 1 - kept), 1LL);
     const long long per = std::max((chunks + n - 1) / n, 1LL);
     p.seg_len = (int)(per * LC);
     p.segments = (int)std::max((chunks + per - 1) / per, 1LL);
+    p.slots = p.segments - 1 + kept;
     return p;
 }
 

@@ -152,6 +152,7 @@ constexpr int LIN_MAX_KEY = 128, LIN_MAX_VALUE = 1024, LIN_MAX_LENGTH = 1 << 30,
 // run side by side; with more than one, `scratch` holds linear_scratch_bytes.
 struct LinChunkPlan {
     int segments = 1, seg_len = 0;
+    int slots = 0;         // states of a sequence in the scratch
     int width = 32;        // key and value channels of a unit: 32, 64 or 128
     int units = 0;         // units of a sequence, a workgroup each
 };
