@@ -4,7 +4,7 @@ single terms, and how fast they forget."""
 import numpy as np
 import pytest
 
-from devbuf import DevBuf
+from devbuf import DevBuf, to_raw
 from test_gpu_linear_attention import check_sequence, eng, inputs  # noqa: F401 (eng: the fixture)
 from zenjpegai_amd import nn
 
@@ -44,3 +44,56 @@ def test_states_updated_in_place_over_many_segments(eng, prec, seqs, length, hea
         b[3].put(state)
         got = call(b[3], b[3])
         assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+def packed(prec, q, k, v):
+    """[t][h][d] arrays as one sequence of packed channels in the storage type."""
+    t = q.shape[0]
+    return to_raw(np.concatenate([a.reshape(t, -1) for a in (q, k, v)], axis=1), prec)[None]
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 40), (128, 128)])
+@pytest.mark.parametrize("length,every", [(32, 32), (70, 32), (330, 16)])
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6])
+def test_a_value_followed_by_zeros_stays_in_the_state(eng, prec, dk, dv, length, every, size):  # noqa: F811
+    """Values at every 32nd or 16th position, zeros between: what is left of them has decayed by up to 2^-62 (2^-82 at a
+    decay of 0.4 and 63 positions), and nothing newer covers what is lost of it. The scale brings the
+    outputs right after a value back to about one."""
+    heads = 4
+    rng = np.random.default_rng(82)
+    q, k = (rng.standard_normal((length, heads, dk)) for _ in range(2))
+    v = np.zeros((length, heads, dv))
+    v[::every] = size * rng.uniform(1.0, 2.0, v[::every].shape)
+    decay = np.array([0.5, 0.25, 0.4, 0.97], np.float32)
+    scale = float(np.float32(0.1 / size))
+    qkv = packed(prec, q, k, v)
+    out = to_raw(np.zeros((1, length, heads * dv)), prec)
+    b = [DevBuf(a) for a in (qkv, out, decay, np.zeros((1, heads, dk, dv), np.float32))]
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=1,
+                                                              length=length, decay=b[2], scale=scale, state_out=b[3]))
+    eng.sync()
+    check_sequence(prec, heads, dk, dv, qkv[0], decay, scale, length, None, b[1].get()[0], out[0], b[3].get()[0])
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6])
+def test_positions_with_key_channels_of_their_own(eng, prec, d, size):  # noqa: F811
+    """Every key has one channel, which no other position of its run of d positions has: every state row is one decayed
+    value, beside far larger ones in the other rows. Values of one head are dense and small."""
+    heads, length = 3, d + 32
+    rng = np.random.default_rng(83)
+    q, k, v = (np.zeros((length, heads, d)) for _ in range(3))
+    k[np.arange(length), :, np.arange(length) % d] = rng.uniform(1.0, 2.0, (length, heads))
+    q[:] = rng.standard_normal(q.shape)
+    v[:] = size * rng.standard_normal(v.shape)
+    decay = np.array([0.5, 0.8, 0.97], np.float32)
+    qkv = packed(prec, q, k, v)
+    out = to_raw(np.zeros((1, length, heads * d)), prec)
+    scale = float(np.float32(0.1 / size))
+    b = [DevBuf(a) for a in (qkv, out, decay, np.zeros((1, heads, d, d), np.float32))]
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=d, value_dim=d, sequences=1,
+                                                              length=length, decay=b[2], scale=scale, state_out=b[3]))
+    eng.sync()
+    check_sequence(prec, heads, d, d, qkv[0], decay, scale, length, None, b[1].get()[0], out[0], b[3].get()[0])

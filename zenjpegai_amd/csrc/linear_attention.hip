@@ -204,9 +204,11 @@ const char* type_name(int dtype) { return dtype == DT_F32 ? "float" : dtype == D
 //  - the query products and the state, in front of an output that is rounded to 16 bits, as two bf16
 //    pieces (2^-16 of them; bf16 has f32's range, which f16 q.k or states can leave), and so do the f16
 //    values they meet (exactly: 11 bits);
-//  - the weighted values g^(31-j) v_j, which the state's f32 sums are made of, as three bf16 pieces next to
-//    bf16 keys (exactly), and next to f16 keys as two f16 ones, the second times 2^11 in a sum of its own
-//    (2^-23 of them; |g^n v| <= |v| stays in f16's range).
+//  - the weighted values g^(31-j) v_j, which the state's f32 sums are made of, as three bf16 pieces (exactly), and the
+//    f16 keys they meet as two (exactly); of the six products the smallest is left out (2^-24). Two f16
+//    pieces of a weighted value are two products instead of five (12 ragged sequences of 64 x 128 channels 72 us
+//    instead of 81, 65536 positions of 16 heads of 128 447 instead of 547), but end at 2^-36, where a decay
+//    of a half is after a chunk: a value that zeros follow is then lost from the state.
 constexpr int LC = 32;
 
 __device__ u32x4 g_lin_zero[2];  // zeros: the source of absent positions and channels
@@ -235,15 +237,17 @@ __device__ __forceinline__ float lin_pow(float l2, int n) { return n == 0 ? 1.0f
 // all, but every address is then an instruction and a register of its own.)
 template <typename T> __host__ __device__ constexpr int lin_row(int d) { return d + (sizeof(T) == 4 ? 4 : 16); }
 
-// The bf16 pieces of eight values: p0 cut off (so that a finite value's is finite), the others rounded.
-template <int N>
+// The bf16 pieces of eight values: p0 cut off (so that a finite value's is finite) or, for values of f16's range
+// (ROUND), rounded as the others.
+template <int N, bool ROUND = false>
 __device__ __forceinline__ void lin_split(const float (&x)[8], u32x4 (&p)[N]) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
         const unsigned a = __builtin_bit_cast(unsigned, x[2 * h]), b = __builtin_bit_cast(unsigned, x[2 * h + 1]);
-        p[0][h] = __builtin_amdgcn_perm(b, a, 0x07060302);
+        p[0][h] = ROUND ? pack_bf16(x[2 * h], x[2 * h + 1]) : __builtin_amdgcn_perm(b, a, 0x07060302);
         if (N == 1) continue;
-        float ra = x[2 * h] - __builtin_bit_cast(float, a & 0xffff0000u), rb = x[2 * h + 1] - __builtin_bit_cast(float, b & 0xffff0000u);
+        const unsigned ta = ROUND ? p[0][h] << 16 : a & 0xffff0000u, tb = ROUND ? p[0][h] & 0xffff0000u : b & 0xffff0000u;
+        float ra = x[2 * h] - __builtin_bit_cast(float, ta), rb = x[2 * h + 1] - __builtin_bit_cast(float, tb);
 #pragma unroll
         for (int n = 1; n < N; ++n) {
             p[n][h] = pack_bf16(ra, rb);
@@ -351,17 +355,16 @@ __device__ __forceinline__ void lin_tile_f32(f32x4& c, const f32x4& a, const f32
 #define SZ2 ([c00] "=&v"(c[0][0]), [c10] "=&v"(c[1][0]), [c01] "=&v"(c[0][1]), [c11] "=&v"(c[1][1]))
 #define SC1 ([c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]))
 #define SC2 ([c00] "+v"(c[0][0]), [c10] "+v"(c[1][0]), [c01] "+v"(c[0][1]), [c11] "+v"(c[1][1]))
-#define LIN_STATE(L, SZ, SC, B)                                                                                                   \
-    if constexpr (F16) {                                                                                                          \
-        static_assert(NB == 1, "piece products");                                                                                 \
-        LIN_ASM(L(LZ, LIN_F16, 0, 0) ZJAI_WAIT, L(LM, LIN_F16, 0, 0) ZJAI_WAIT, SZ, SC, A2(0), B(0))                              \
-    } else {                                                                                                                      \
-        static_assert(NB == 3, "piece products");                                                                                 \
-        LIN_ASM(L(LZ, ZJAI_MF, 0, 2) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT,                                         \
-                L(LM, ZJAI_MF, 0, 2) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, SZ, SC, A2(0), B(0), B(1), B(2))        \
+// `a` is the keys or the first piece of them (b's three pieces) or the second (b's two largest).
+#define LIN_STATE(L, SZ, SC, B)                                                                                                       \
+    if constexpr (NB == 3) {                                                                                                          \
+        LIN_ASM(L(LZ, ZJAI_MF, 0, 2) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT,                                             \
+                L(LM, ZJAI_MF, 0, 2) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, SZ, SC, A2(0), B(0), B(1), B(2))            \
+    } else {                                                                                                                          \
+        LIN_ASM(L(LZ, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, SZ, SC, A2(0), B(0), B(1)) \
     }
-template <bool F16, int NV, int NB>
-__device__ __forceinline__ void lin_state(f32x4 (&c)[2][NV], const u32x4 (&a)[2][1], const u32x4 (&b)[NV][NB], bool zero = false) {
+template <int NB, int NV>
+__device__ __forceinline__ void lin_state(f32x4 (&c)[2][NV], const u32x4 (&a)[2][1], const u32x4 (&b)[NV][3], bool zero) {
     if constexpr (NV == 1) {
         LIN_STATE(LS1, SZ1, SC1, B1)
     } else {
@@ -434,14 +437,6 @@ __device__ __forceinline__ LinUnit<T> lin_load(const T* p, int c0, int d, bool v
     return r;
 }
 
-// An f16 pair of f32 values' halves.
-__device__ __forceinline__ unsigned pack_f16(float a, float b) {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    f16x2 r;
-    r[0] = (_Float16)a;
-    r[1] = (_Float16)b;
-    return __builtin_bit_cast(unsigned, r);
-}
 // Eight f16 or bf16 values as f32.
 template <typename T>
 __device__ __forceinline__ void lin_floats(const u32x4& v, float (&x)[8]) {
@@ -467,9 +462,9 @@ struct LinChunkArgs {
     int even;  // vec_k and vec_v, and head sizes of whole units
 };
 
-// 16-bit planes of a chunk in LDS: k, v and, for outputs, q (f16's in pieces too).
+// 16-bit planes of a chunk in LDS: k, v and, for outputs, q; f16's k and q in two pieces, for outputs as they are too.
 template <typename T> __host__ __device__ constexpr int lin_lds_planes(bool out) {
-    return sizeof(T) == 4 ? (out ? 6 : 4) : Elem<T>::dt == DT_F16 ? (out ? 5 : 2) : (out ? 3 : 2);
+    return sizeof(T) == 4 ? (out ? 6 : 4) : Elem<T>::dt == DT_F16 ? (out ? 7 : 3) : (out ? 3 : 2);
 }
 
 // D: channels of a unit; a wave has one 16-column tile of its values or, for the outputs of the widest, two: with
@@ -484,13 +479,14 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
     constexpr int NV = lin_tiles(D, OUT);
     constexpr int ROW = lin_row<T>(D), PLANE = LC * ROW;  // LDS values of a position and of a chunk of q, k or v
     constexpr int MT = D / 16, KS = D / 32;
-    constexpr int QP = F16 ? 2 : 1;           // bf16 pieces of a 16-bit q or v
+    constexpr int QP = F16 ? 2 : 1;           // bf16 pieces of a 16-bit q, k or v
     extern __shared__ __attribute__((aligned(16))) unsigned short s_lds[];  // [lin_lds_planes][PLANE], then 64 WV floats
     const LinAttnArgs& a = c.a;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, l16 = lane & 15, g = lane >> 4;
     unsigned short* s_k = s_lds;
-    unsigned short* s_v = s_k + (F32 ? 2 : 1) * PLANE;
-    unsigned short* s_q = s_v + (F32 ? 2 : 1) * PLANE;  // f16: the values, then their two pieces
+    unsigned short* s_v = s_k + (F32 || (F16 && !OUT) ? 2 : 1) * PLANE;
+    unsigned short* s_q = s_v + (F32 ? 2 : 1) * PLANE;           // f16: the values, then their two pieces
+    unsigned short* s_kp = F16 && OUT ? s_q + 3 * PLANE : s_k;  // the keys that the state's products take
     float *f_k = (float*)s_k, *f_v = (float*)s_v, *f_q = (float*)s_q;
 
     // Workgroups go round the eight XCDs. The units of a segment share cache lines of the positions' channels and are
@@ -654,7 +650,15 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
                     *(u32x4*)(f_q + at + 4) = rq[i].v[1];
                 }
             } else {
-                *(u32x4*)(s_k + row * ROW + u * 8) = rk[i].v[0];
+                if (OUT || !F16) *(u32x4*)(s_k + row * ROW + u * 8) = rk[i].v[0];
+                if constexpr (F16) {
+                    float x[8];
+                    u32x4 p[2];
+                    lin_floats<T>(rk[i].v[0], x);
+                    lin_split<2, true>(x, p);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) *(u32x4*)(s_kp + n * PLANE + row * ROW + u * 8) = p[n];
+                }
                 *(u32x4*)(s_v + row * ROW + u * 8) = rv[i].v[0];
                 if (OUT) {
                     // Channels 4 x of a 32-channel block go to unit x % 4, half x / 4.
@@ -715,7 +719,7 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
 
         // The wave's value columns 16 n + l16 at positions j = {4 g + r, 16 + 4 g + r}, and their weighted pieces.
         float x[NV][8], w[NV][8], big = 0.0f;
-        u32x4 wv[NV][3], hi[NV][1], lo[NV][1];
+        u32x4 wv[NV][3];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int col = wave * NV + n;
@@ -730,22 +734,8 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
             for (int e = 0; e < 8; ++e) {
                 big = __builtin_elementwise_maximum(big, __builtin_fabsf(x[n][e]));
                 w[n][e] = x[n][e] * w_v[e];
-                // The product as it is rounded to f32: contracted into v_fma_mixlo_f16 (one rounding), what the second
-                // piece is the rest of would not always be the first.
-                if (F16) asm("" : "+v"(w[n][e]));
             }
-            if constexpr (F16) {
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const unsigned top = pack_f16(w[n][2 * h], w[n][2 * h + 1]);
-                    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-                    const f16x2 p = __builtin_bit_cast(f16x2, top);
-                    hi[n][0][h] = top;
-                    lo[n][0][h] = pack_f16((w[n][2 * h] - (float)p[0]) * 2048.0f, (w[n][2 * h + 1] - (float)p[1]) * 2048.0f);
-                }
-            } else if constexpr (!F32) {
-                lin_split<3>(w[n], wv[n]);
-            }
+            if constexpr (!F32) lin_split<3>(w[n], wv[n]);
         }
 
         if (OUT) {
@@ -940,20 +930,12 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
                     lin_state_f32<NV>(acc, kt, vt, !OUT && i == 0);
                 }
             } else {
-                const u32x4 kt[2][1] = {{column16(s_k, 2 * m)}, {column16(s_k, 2 * m + 2)}};
                 if constexpr (F16) {
-                    f32x4 small[2][NV];
-                    lin_state<true, NV>(acc, kt, hi, !OUT);
-                    lin_state<true, NV>(small, kt, lo, true);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int n = 0; n < NV; ++n)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) acc[h][n][r] = fmaf(small[h][n][r], 0x1p-11f, acc[h][n][r]);
-                } else {
-                    lin_state<false, NV>(acc, kt, wv, !OUT);
+                    const u32x4 kt[2][1] = {{column16(s_kp + PLANE, 2 * m)}, {column16(s_kp + PLANE, 2 * m + 2)}};
+                    lin_state<2, NV>(acc, kt, wv, !OUT);
                 }
+                const u32x4 kt[2][1] = {{column16(s_kp, 2 * m)}, {column16(s_kp, 2 * m + 2)}};
+                lin_state<3, NV>(acc, kt, wv, !OUT && !F16);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
