@@ -4,7 +4,8 @@ single terms, and how fast they forget."""
 import numpy as np
 import pytest
 
-from devbuf import DevBuf, to_raw
+from devbuf import DevBuf, from_raw, to_raw
+from linear_attention_oracle import U, oracle
 from test_gpu_linear_attention import check_sequence, eng, inputs  # noqa: F401 (eng: the fixture)
 from zenjpegai_amd import nn
 
@@ -97,3 +98,45 @@ def test_positions_with_key_channels_of_their_own(eng, prec, d, size):  # noqa: 
                                                               length=length, decay=b[2], scale=scale, state_out=b[3]))
     eng.sync()
     check_sequence(prec, heads, d, d, qkv[0], decay, scale, length, None, b[1].get()[0], out[0], b[3].get()[0])
+
+
+def rounds_from_within(got, want, tol, prec):
+    """Every stored value is the rounding of some value within tol of the wanted one."""
+    lo, hi = (from_raw(to_raw((want + s * tol).astype(np.float32), prec), prec) for s in (-1, 1))
+    bad = (got < lo) | (got > hi)
+    assert not bad.any(), (int(bad.sum()), bad.size, float((np.abs(got - want) / want)[bad].max()))
+
+
+@pytest.mark.parametrize("prec", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("path", ["state", "values"])
+def test_what_16_bits_leave_of_the_products_before_an_output(eng, prec, d, path):  # noqa: F811
+    """A state or a weighted query product enters the product with f16 queries or values, or bf16 ones, as two bf16
+    pieces, the first cut off and the second rounded: 2^-16 of it at most, and the other operand is exact. The
+    operands are powers of two with ones in every bit behind the eighth, which makes what is left out as large as it
+    gets, with one sign. (f32's sums: d + 96 roundings of the term at most, 33 products of a chunk among them.)"""
+    length, heads = 32, 2
+    rng = np.random.default_rng(84)
+    in16 = 1.0 + 2.0 ** -7 - 2.0 ** -10 if prec == "f16" else 1.0  # as far as 16 bits go
+    in32 = 1.0 + 2.0 ** -7 - 2.0 ** -20
+
+    def powers(*shape):
+        return 0.5 ** rng.integers(0, 4, shape)
+
+    q, k, state = np.zeros((length, heads, d)), np.zeros((length, heads, d)), None
+    if path == "state":
+        q[:], v, scale = in16 * powers(*q.shape), np.zeros(q.shape), 1.0 / d
+        state = (in32 * powers(heads, d, d)).astype(np.float32)
+    else:  # the query products are the keys times the scale
+        q[:, :, 0], k[:, :, 0], v = 1.0, in16 * powers(length, heads), in16 * powers(length, heads, d)
+        scale = 1.0 if prec == "f16" else in32
+    decay = np.ones(heads, np.float32)
+    qkv = packed(prec, q, k, v)
+    b = [DevBuf(a) for a in (qkv, to_raw(np.zeros((1, length, heads * d)), prec), decay)]
+    d_state = None if state is None else DevBuf(state[None])
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=d, value_dim=d, sequences=1,
+                                                              length=length, decay=b[2], scale=scale, state_in=d_state))
+    eng.sync()
+    (o, oa, _), _ = oracle(q, k, v, decay, scale, length, state)
+    got = from_raw(b[1].get(), prec).reshape(o.shape)
+    rounds_from_within(got, o, (2.0 ** -16 + (d + 96) * U) * oa, prec)

@@ -203,7 +203,8 @@ const char* type_name(int dtype) { return dtype == DT_F32 ? "float" : dtype == D
 // 16x16x32 MFMAs, q.k on the stored values themselves. What is computed in f32 enters the matrix cores in pieces:
 //  - the query products and the state, in front of an output that is rounded to 16 bits, as two bf16
 //    pieces (2^-16 of them; bf16 has f32's range, which f16 q.k or states can leave), and so do the f16
-//    values they meet (exactly: 11 bits);
+//    values they meet (exactly: 11 bits), in all four products: the smallest is up to 2^-14 of the term where the
+//    first pieces are cut off, always of its sign (three products: 65536 f16 positions 553 us instead of 573);
 //  - the weighted values g^(31-j) v_j, which the state's f32 sums are made of, as three bf16 pieces (exactly), and the
 //    f16 keys they meet as two (exactly); of the six products the smallest is left out (2^-24). Two f16
 //    pieces of a weighted value are two products instead of five (12 ragged sequences of 64 x 128 channels 72 us
@@ -257,9 +258,9 @@ __device__ __forceinline__ void lin_split(const float (&x)[8], u32x4 (&p)[N]) {
     }
 }
 
-// Sums of matrix products, the tiles of an instruction group given as pairs (c, a, b), over the products of pieces
-// p + q <= 1 (up to 2 with three), the small ones first (zero: the sums start here, a constant where this is
-// inlined). Inline assembly with the accumulators in place: the compiler renames the builtin's chains
+// Sums of matrix products, the tiles of an instruction group given as pairs (c, a, b), over the products of pieces (all
+// of them but the smallest of an f16 key's and a weighted value's), the small ones first (zero: the sums start here, a
+// constant where this is inlined). Inline assembly with the accumulators in place: the compiler renames the builtin's chains
 // back to back. A block carries its own wait states, as split.h's.
 #define LM(MF, c, a, b) MF "%[c" #c "], %[a" #a "], %[b" #b "], %[c" #c "]\n\t"
 #define LZ(MF, c, a, b) MF "%[c" #c "], %[a" #a "], %[b" #b "], 0\n\t"
@@ -321,8 +322,9 @@ __device__ __forceinline__ void lin_score(f32x4& c, const u32x4& a, const u32x4&
         LIN_ASM(L(LZ, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, L(LM, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, OZ, OC, A(0), \
                 A(1), B2(0))                                                                                                    \
     } else {                                                                                                                    \
-        LIN_ASM(L(LZ, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT,                                       \
-                L(LM, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, OZ, OC, A(0), A(1), B2(0), B2(1))      \
+        LIN_ASM(L(LZ, ZJAI_MF, 1, 1) L(LM, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT,                  \
+                L(LM, ZJAI_MF, 1, 1) L(LM, ZJAI_MF, 1, 0) L(LM, ZJAI_MF, 0, 1) L(LM, ZJAI_MF, 0, 0) ZJAI_WAIT, OZ, OC, A(0), A(1), \
+                B2(0), B2(1))                                                                                                   \
     }
 template <int NV, int NA, int NB>
 __device__ __forceinline__ void lin_outputs(f32x4 (&c)[NV][2], const u32x4 (&a)[NV][NA], const u32x4 (&b)[2][NB], bool zero = false) {
