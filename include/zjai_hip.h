@@ -115,6 +115,16 @@ ZJAI_API int32_t zjai_ctx_destroy(zjai_ctx* ctx);
 ZJAI_API int32_t zjai_last_error(const zjai_ctx* ctx, char* buf, size_t len);
 /* Blocks until the context's stream is idle. */
 ZJAI_API int32_t zjai_sync(zjai_ctx* ctx);
+/* Order between the context's stream, which nothing else orders (not the default stream either), and a
+ * stream of the caller's on the same device (a hipStream_t; NULL: the default stream): for entry points that
+ * work on the caller's device buffers, whose contents come from that stream and are read on it. Neither blocks
+ * the host nor allocates. zjai_order_after: calls on the context from here on run after what `stream` holds
+ * now. zjai_order_before: what is enqueued on `stream` from here on runs after the calls made so far. (Some
+ * 15 us of host time each: once for many small calls.) With the
+ * first before and the second after them, enqueued calls become part of a graph that `stream` is being
+ * captured into. */
+ZJAI_API int32_t zjai_order_after(zjai_ctx* ctx, void* stream);
+ZJAI_API int32_t zjai_order_before(zjai_ctx* ctx, void* stream);
 /* Cooperative cancellation, the `enough::Stop` check between layers and tiles
  * (src/decoder/api.rs:283-299): while set, running calls return ZJAI_E_CANCELLED at their next
  * check. */
@@ -302,13 +312,14 @@ typedef struct zjai_linear_attention_desc {
 } zjai_linear_attention_desc;
 
 /* Whole sequences. desc->slots must be NULL. Enqueued on the context's stream (zjai_sync waits for
- * it); works in the context's scratch, as zjai_channel_attention_noalloc, and allocates nothing: a
+ * it, zjai_order_after and zjai_order_before order it with the stream that fills and reads the buffers); works in the context's scratch, as zjai_channel_attention_noalloc, and allocates nothing: a
  * graph it is captured into must not run at the same time as another call of the context. */
 ZJAI_API int32_t zjai_linear_attention_noalloc(zjai_ctx* ctx, const zjai_linear_attention_desc* desc);
 /* The recurrent form: one position of each sequence (length 1, lengths NULL, both states given).
  * Sequence i reads state_in[slots[i]] and writes state_out[slots[i]]; states of other slots stay as
  * they were. A slot outside 0..num_slots-1 marks an idle sequence, whose output stays as it was.
- * Sequences with the same slot follow one another in their order, as consecutive positions. */
+ * Sequences with the same slot follow one another in their order, as consecutive positions. Enqueued as
+ * zjai_linear_attention_noalloc. */
 ZJAI_API int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_attention_desc* desc);
 
 /* ---------------------------------------------- the join of two blocks: norms, gate, residual */
@@ -342,7 +353,8 @@ ZJAI_API int32_t zjai_norm_gate_residual(zjai_ctx* ctx, const zjai_tensor* x, co
 
 /* On the caller's device buffers: [positions][channels] with a stride (in elements) from one position to the
  * next. x_out may be x, and h may be y, gate or x, with that buffer's stride; buffers overlap in no other
- * way. Weights are device arrays of `channels` floats. Enqueued on the context's stream. */
+ * way. Weights are device arrays of `channels` floats. Enqueued on the context's stream (see
+ * zjai_order_after). */
 typedef struct zjai_norm_gate_residual_desc {
     int32_t precision, channels; /* channels 1..16384 */
     int64_t positions;

@@ -110,6 +110,8 @@ PROTOTYPES = {
     "zjai_ctx_destroy": [_vp],
     "zjai_last_error": [_vp, ctypes.c_char_p, ctypes.c_size_t],
     "zjai_sync": [_vp],
+    "zjai_order_after": [_vp, _vp],
+    "zjai_order_before": [_vp, _vp],
     "zjai_set_stop": [_vp, _i32],
     "zjai_get_stats": [_vp, ctypes.POINTER(ZjaiStats)],
     "zjai_release_buffers": [_vp],

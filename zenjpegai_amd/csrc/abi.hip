@@ -75,6 +75,23 @@ TensorP planar_upload(Context& c, const float* data, int ch, int h, int w, int d
     return t;
 }
 
+// Makes the context's device current for a call on the caller's buffers and restores the caller's.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int d = -1;
+        ZJAI_HIP(hipGetDevice(&d));
+        if (d == device) return;
+        ZJAI_HIP(hipSetDevice(device));
+        before = d;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
 }  // namespace
 
 // zjai_channel_attention_noalloc works in its context's scratch: every launch of a call runs on the
@@ -107,6 +124,7 @@ extern "C" int32_t zjai_ctx_create(int32_t device, uint32_t flags, zjai_ctx** ou
         ZJAI_HIP(hipStreamCreateWithFlags(&ctx->c.stream, hipStreamNonBlocking));
         ZJAI_HIP(hipEventCreate(&ctx->c.ev0));
         ZJAI_HIP(hipEventCreate(&ctx->c.ev1));
+        ZJAI_HIP(hipEventCreateWithFlags(&ctx->c.order, hipEventDisableTiming));
         ctx->c.scratch = take_scratch(device);
         ctx->c.copier.create();
     });
@@ -123,6 +141,7 @@ extern "C" int32_t zjai_ctx_destroy(zjai_ctx* ctx) {
     if (ctx->c.stream) (void)hipStreamSynchronize(ctx->c.stream);
     if (ctx->c.ev0) (void)hipEventDestroy(ctx->c.ev0);
     if (ctx->c.ev1) (void)hipEventDestroy(ctx->c.ev1);
+    if (ctx->c.order) (void)hipEventDestroy(ctx->c.order);
     if (ctx->c.stream) (void)hipStreamDestroy(ctx->c.stream);
     delete ctx;
     return ZJAI_OK;
@@ -145,6 +164,26 @@ extern "C" int32_t zjai_last_error(const zjai_ctx* ctx, char* buf, size_t len) {
 extern "C" int32_t zjai_sync(zjai_ctx* ctx) {
     if (!ctx) return ZJAI_E_INVALID_ARGUMENT;
     return guard(ctx, [&] { ZJAI_HIP(hipStreamSynchronize(ctx->c.stream)); });
+}
+
+// `later` waits for what `first` holds; one of the two is the context's, `theirs` the caller's.
+static void order_streams(Context& C, hipStream_t first, hipStream_t later, hipStream_t theirs) {
+    const OnDevice on(C.device);
+    hipDevice_t device = -1;
+    ZJAI_HIP(hipStreamGetDevice(theirs, &device));
+    need(device == C.device, "order: a stream of another device");
+    ZJAI_HIP(hipEventRecord(C.order, first));
+    ZJAI_HIP(hipStreamWaitEvent(later, C.order, 0));
+}
+
+extern "C" int32_t zjai_order_after(zjai_ctx* ctx, void* stream) {
+    if (!ctx) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] { order_streams(ctx->c, (hipStream_t)stream, ctx->c.stream, (hipStream_t)stream); });
+}
+
+extern "C" int32_t zjai_order_before(zjai_ctx* ctx, void* stream) {
+    if (!ctx) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] { order_streams(ctx->c, ctx->c.stream, (hipStream_t)stream, (hipStream_t)stream); });
 }
 
 extern "C" int32_t zjai_set_stop(zjai_ctx* ctx, int32_t stop) {
@@ -535,23 +574,6 @@ extern "C" int32_t zjai_channel_attention_noalloc(zjai_ctx* ctx, const void* qkv
 
 // ------------------------------------------------------- causal context: decayed linear attention
 namespace {
-
-// Makes the context's device current for a call on the caller's buffers and restores the caller's.
-struct OnDevice {
-    int before = -1;
-    explicit OnDevice(int device) {
-        int d = -1;
-        ZJAI_HIP(hipGetDevice(&d));
-        if (d == device) return;
-        ZJAI_HIP(hipSetDevice(device));
-        before = d;
-    }
-    ~OnDevice() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-    OnDevice(const OnDevice&) = delete;
-    OnDevice& operator=(const OnDevice&) = delete;
-};
 
 void need_aligned(const void* p, int bytes, const char* msg) { need(((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0, msg); }
 

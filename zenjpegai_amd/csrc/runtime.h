@@ -117,6 +117,7 @@ struct Context {
     // weights on their way to the split form, all in stream order.
     void* scratch = nullptr;
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
+    hipEvent_t order = nullptr;  // zjai_order_after / _before: recorded on one stream, waited for by the other
     float last_ms = 0.0f;
     long long launches = 0;
     // Per-launch profiling (zjai_profile_begin / zjai_profile_end).

@@ -100,6 +100,16 @@ class Engine:
     def sync(self):
         check(lib().zjai_sync(self._h), self._h)
 
+    def order_after(self, stream=None):
+        """Calls from here on run after what ``stream`` (a handle, a torch stream, or None: the default
+        stream) holds now (``zjai_order_after``)."""
+        check(lib().zjai_order_after(self._h, getattr(stream, "cuda_stream", stream)), self._h)
+
+    def order_before(self, stream=None):
+        """What is enqueued on ``stream`` from here on runs after the calls made so far
+        (``zjai_order_before``)."""
+        check(lib().zjai_order_before(self._h, getattr(stream, "cuda_stream", stream)), self._h)
+
     def host_array(self, shape, dtype=np.float32) -> np.ndarray:
         """A zeroed numpy array in page-locked host memory (``zjai_host_alloc``), for transfer
         buffers reused across pictures; freed with the array (``zjai_host_free``, which needs no
@@ -390,12 +400,14 @@ def linear_attention_desc(precision: str, qkv, out, *, heads: int, key_dim: int,
 
 
 def linear_attention_noalloc(eng: Engine, desc: _lib.ZjaiLinearAttentionDesc) -> None:
-    """``zjai_linear_attention_noalloc``: enqueued on the engine's stream."""
+    """``zjai_linear_attention_noalloc``: enqueued on the engine's stream, which no other stream is ordered with:
+    the buffers are filled before the call and read after ``Engine.sync()``, or on a stream that
+    ``Engine.order_after`` and ``Engine.order_before`` put before and after the call."""
     check(lib().zjai_linear_attention_noalloc(eng.handle, desc), eng.handle)
 
 
 def linear_attention_step(eng: Engine, desc: _lib.ZjaiLinearAttentionDesc) -> None:
-    """``zjai_linear_attention_step``: enqueued on the engine's stream."""
+    """``zjai_linear_attention_step``: enqueued as ``linear_attention_noalloc``."""
     check(lib().zjai_linear_attention_step(eng.handle, desc), eng.handle)
 
 
@@ -436,5 +448,5 @@ def norm_gate_residual_desc(precision: str, x, y, gate, x_out, h, *, positions: 
 
 
 def norm_gate_residual_noalloc(eng: Engine, desc: _lib.ZjaiNormGateResidualDesc) -> None:
-    """``zjai_norm_gate_residual_noalloc``: enqueued on the engine's stream."""
+    """``zjai_norm_gate_residual_noalloc``: enqueued as ``linear_attention_noalloc``."""
     check(lib().zjai_norm_gate_residual_noalloc(eng.handle, desc), eng.handle)
