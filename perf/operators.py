@@ -162,10 +162,13 @@ def prepare(case, seed):
     state = {"case": case, **_inputs(case, seed)}
     if own:
         state["engine"], state["plan"] = _engine(), _plan(case, state)
+        torch.cuda.current_stream(DEVICE).synchronize()  # the engine's stream is ordered with no other one
     return state
 
 
 def run(state):
+    """One pass. The engine's calls go on its own stream: their outputs are there, and the state's buffers free,
+    when the engine or the device has been waited for (or a stream that the engine has ordered behind them)."""
     kind = state["case"]["kind"]
     if own:
         from zenjpegai_amd import nn
