@@ -7,7 +7,7 @@ import pytest
 from devbuf import DevBuf, from_raw, to_raw
 from linear_attention_oracle import U, oracle
 from test_gpu_linear_attention import check_sequence, eng, inputs  # noqa: F401 (eng: the fixture)
-from zenjpegai_amd import nn
+from zenjpegai_amd import _lib, nn
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +140,78 @@ def test_what_16_bits_leave_of_the_products_before_an_output(eng, prec, d, path)
     (o, oa, _), _ = oracle(q, k, v, decay, scale, length, state)
     got = from_raw(b[1].get(), prec).reshape(o.shape)
     rounds_from_within(got, o, (2.0 ** -16 + (d + 96) * U) * oa, prec)
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("seqs,length,d", [(1, 6001, 16), (1, 6001, 128), (600, 1000, 16)])
+@pytest.mark.parametrize("what", ["first position", "state", "all positions"])
+def test_decays_next_to_one_are_told_from_one(eng, prec, seqs, length, d, what):  # noqa: F811
+    """What a memory of a thousand, of a million and of 16 million positions keeps of a one at the first position, of a
+    state of ones, and of a one at every position, split into up to 188 segments or (600 sequences) in one.
+    A chunk's power g^32 comes from 2^x, off by a step (2 U of a value above a half), at an exponent 32 log2 g
+    off by 8 U of itself, and joins the state with one rounding, where ones come in at every position with up
+    to 32 more: m chunks are off by m (3 + 8 * 32 |ln g|) U, or m 32 U more; 64 U for the first one's products."""
+    decay = np.array([1 - 2.0 ** -10, 1 - 2.0 ** -20, 1 - 2.0 ** -24], np.float32)
+    heads, g = 3, decay.astype(np.float64)
+    q, k, v = (np.zeros((length, heads, d)) for _ in range(3))
+    if what != "state":
+        k[0], v[0] = 1.0, 1.0
+    if what == "all positions":
+        k[:], v[:] = 1.0, 1.0
+    state = np.ones((seqs, heads, d, d), np.float32) if what == "state" else None
+    b = [DevBuf(a) for a in (packed(prec, q, k, v), to_raw(np.zeros((seqs, length, heads * d)), prec), decay)]
+    fin = DevBuf(np.zeros((seqs, heads, d, d), np.float32))
+    d_state = None if state is None else DevBuf(state)
+    nn.linear_attention_noalloc(eng, nn.linear_attention_desc(
+        prec, b[0], b[1], heads=heads, key_dim=d, value_dim=d, sequences=seqs, length=length, decay=b[2], state_in=d_state,
+        state_out=fin, q_sequence=0, k_sequence=0, v_sequence=0))
+    eng.sync()
+    n = {"first position": length - 1, "state": length}.get(what)
+    keep = -np.expm1(length * np.log(g)) / (1 - g) if n is None else np.exp(n * np.log(g))
+    m = -(-length // 32)
+    rel = U * (m * (3 + 8 * 32 * np.abs(np.log(g)) + (32 if n is None else 0)) + 64)
+    assert (np.abs(keep - (length if n is None else 1.0)) > 2 * rel * keep)[:2 if n is None or length < 6001 else 3].all()
+    err = np.abs(fin.get() - keep[:, None, None]) / keep[:, None, None]
+    assert (err <= rel[:, None, None]).all(), (err.max((0, 2, 3)) / U, rel / U)
+
+
+@pytest.mark.parametrize("prec", ["f32", "bf16"])
+def test_calls_that_share_a_scratch_keep_their_results(prec):
+    """Linear attention in segments and channel attention work in the scratch of their context, one after the other; two
+    contexts' calls overlap. Every output is that of the same call by itself."""
+    engs = [nn.Engine(0, prec) for _ in range(2)]
+    length, heads, d = 1500, 2, 32
+    runs = []
+    for i, e in enumerate(engs):
+        qkv, out, decay, _ = inputs(30 + i, prec, 1, length, heads, d, d)
+        b = [DevBuf(a) for a in (qkv, out, decay)]
+        other = DevBuf(np.random.default_rng(i).standard_normal((20, 24, 3 * 64)).astype(np.float32))
+        y, temp = DevBuf(np.zeros((20, 24, 64), np.float32)), DevBuf(np.ones(4, np.float32))
+        desc = nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=d, value_dim=d, sequences=1, length=length, decay=b[2])
+        runs.append((e, desc, b, other, y, temp))
+
+    def channel(e, other, y, temp):
+        _lib.check(_lib.lib().zjai_channel_attention_noalloc(e.handle, other.address, 192, 20, 24, 4, temp.address, _lib.F32,
+                                                             y.address), e.handle)
+
+    want = []
+    for e, desc, b, other, y, temp in runs:
+        channel(e, other, y, temp)
+        e.sync()
+        nn.linear_attention_noalloc(e, desc)
+        e.sync()
+        want.append((y.get(), b[1].get()))
+        y.put(np.zeros(y.shape, y.dtype))
+        b[1].put(np.zeros(b[1].shape, b[1].dtype))
+    assert not np.array_equal(want[0][0], want[1][0])
+    for _ in range(5):
+        for e, desc, b, other, y, temp in runs:
+            nn.linear_attention_noalloc(e, desc)
+            channel(e, other, y, temp)
+            nn.linear_attention_noalloc(e, desc)
+    for (e, _, b, _, y, _), w in zip(runs, want):
+        e.sync()
+        assert np.array_equal(y.get(), w[0]) and np.array_equal(b[1].get(), w[1])
+    del runs, b, other, y, temp, desc
+    for e in engs:
+        e.close()
