@@ -215,3 +215,20 @@ def test_calls_that_share_a_scratch_keep_their_results(prec):
     del runs, b, other, y, temp, desc
     for e in engs:
         e.close()
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,dk,dv", [(2, 64, 66), (1, 33, 1023), (3, 128, 70), (2, 100, 34), (1, 128, 129)])
+@pytest.mark.parametrize("offset", [0, 4])
+def test_steps_on_states_that_are_not_whole_16_bytes(eng, prec, heads, dk, dv, offset):  # noqa: F811
+    """Rows whose length or place is not a multiple of four floats, with up to 16 of them to a lane."""
+    n = 3
+    qkv, out, decay, state = inputs(90, prec, n, 1, heads, dk, dv)
+    b = [DevBuf(a) for a in (qkv, out, decay)]
+    d_in, d_out = DevBuf(state, offset), DevBuf(np.zeros_like(state), offset)
+    nn.linear_attention_step(eng, nn.linear_attention_desc(prec, b[0], b[1], heads=heads, key_dim=dk, value_dim=dv, sequences=n,
+                                                           length=1, decay=b[2], state_in=d_in, state_out=d_out))
+    eng.sync()
+    got, fin = b[1].get(), d_out.get()
+    for s in range(n):
+        check_sequence(prec, heads, dk, dv, qkv[s], decay, 1.0, 1, state[s], got[s], out[s], fin[s])
