@@ -70,14 +70,16 @@ struct TeamSum {
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], off);
         if (p.mode == SUM_LANES) return;
+        int t = tid, l = lane;
+        if (NV > 4) asm volatile("" : "+v"(t), "+v"(l));  // places computed here, not kept over the positions
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if ((tid & (p.lanes - 1)) == 0) s_red[i * threads + tid] = v[i];
+            if ((t & (p.lanes - 1)) == 0) s_red[i * threads + t] = v[i];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int first = (lane + tp * i) / p.group_vecs * p.group_vecs;
+            const int first = (l + tp * i) / p.group_vecs * p.group_vecs;
             float s = 0.0f;
             if (first < tp * NV)
                 for (int k = first; k < min(first + p.group_vecs, tp * NV); k += p.lanes)
@@ -97,8 +99,17 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
     const int tid = threadIdx.x, lane = tid & (p.tp - 1), team = tid / p.tp, teams = p.threads / p.tp;
     const TeamSum<NV> sum{tid, lane, p.tp, p.threads, team * p.tp, s_red};
     const int C = a.channels;
-    // Eight channels' weights stay in registers; sixteen channels' are read again for each position.
-    constexpr bool KEEP = NV * VE <= 8;
+    // Eight channels' weights stay in registers; sixteen channels', and those of single ones, are read again where a
+    // position needs them. (With 1024 lanes a lane has 128 registers. What does not fit goes to private memory, for
+    // which the runtime takes 686 MiB of the card at the first such launch: 9001 channels, f32.)
+    constexpr bool KEEP = NV * VE <= 8 && VE > 1;
+    // There, what a position's addresses are made of is not kept over the positions either (nor over its parts).
+    int here = lane;
+    const auto afresh = [&]() {
+        if constexpr (KEEP) return;
+        asm volatile("" : "+v"(here));
+    };
+    const auto vec = [&](int i) { return (here + p.tp * i) * VE; };
     bool on[NV];
     float pw[NV][VE], pb[NV][VE], sc[NV][VE], nw[NV][VE], nb[NV][VE];
     // w's VE values of vector i; lanes past the channels read the first ones, which nothing uses.
@@ -108,7 +119,8 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
             for (int e = 0; e < VE; ++e) to[e] = absent;
             return;
         }
-        w += on[i] ? (lane + p.tp * i) * VE : 0;
+        if (!KEEP) asm volatile("" : "+s"(w));
+        w += on[i] ? vec(i) : 0;
         if constexpr (VE % 4 == 0) {
             if (p.wide_weights) {
 #pragma unroll
@@ -138,26 +150,44 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
     const float inv_group = 1.0f / (float)(C / a.groups), inv_all = 1.0f / (float)C;
 
     V x[NV], y[NV], g[NV];
-    const auto fetch = [&](long long at) {
-        const bool ok = at < a.positions;
-        const T* px = (const T*)a.x.p + (ok ? join_at(a.x, a.width, at) : 0);
-        const T* py = (const T*)a.y.p + (ok ? join_at(a.y, a.width, at) : 0);
-        const T* pg = GATE ? (const T*)a.g.p + (ok ? join_at(a.g, a.width, at) : 0) : nullptr;
+    const auto place = [&](const JoinRows& r, long long at) {
+        return (const T*)r.p + (at < a.positions ? join_at(r, a.width, at) : 0);
+    };
+    // (`c`: always a channel that exists.)
+    const auto fetch_gate = [&](long long at) {
+        const T* pg = place(a.g, at);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = on[i] ? (lane + p.tp * i) * VE : 0;  // always a channel that exists
+            const int c = on[i] ? vec(i) : 0;
+            g[i] = *(const V*)(pg + c);
+        }
+    };
+    constexpr bool GATE_AHEAD = GATE && NV < 16;  // sixteen addresses more than there are registers for
+    const auto fetch = [&](long long at) {
+        const T *px = place(a.x, at), *py = place(a.y, at), *pg = GATE_AHEAD ? place(a.g, at) : nullptr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = on[i] ? vec(i) : 0;
             x[i] = *(const V*)(px + c);
             y[i] = *(const V*)(py + c);
-            if (GATE) g[i] = *(const V*)(pg + c);
+            if (GATE_AHEAD) g[i] = *(const V*)(pg + c);
         }
     };
     const long long step = (long long)gridDim.x * teams;
     long long base = (long long)blockIdx.x * teams;
     if (base < a.positions) fetch(base + team);
     if (KEEP) load_weights();
+    const auto weight = [&](const float (&kept)[NV][VE], const float* w, int i, float absent, float (&to)[VE]) {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) to[e] = kept[i][e];
+        } else {
+            weights(w, i, absent, to);
+        }
+    };
     for (; base < a.positions; base += step) {
         const long long at = base + team;
-        if (!KEEP) load_weights();
+        afresh();
         float u[NV][VE], v[NV][VE];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -193,18 +223,31 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const float inv = 1.0f / sqrtf(s[i] * inv_group + a.post_eps);
+                float w[VE], b[VE];
+                weight(pw, a.post_w, i, 1.0f, w);
+                weight(pb, a.post_b, i, 0.0f, b);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) u[i][e] = u[i][e] * inv * pw[i][e] + pb[i][e];
+                for (int e = 0; e < VE; ++e) u[i][e] = u[i][e] * inv * w[e] + b[e];
             }
         }
+        if (GATE && !GATE_AHEAD) {
+            afresh();
+            fetch_gate(at);
+        }
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float w[VE];
+            weight(sc, a.scale, i, 1.0f, w);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 if (GATE) u[i][e] *= gate_value(to_f32(g[i].e[e]), a.gate);
-                v[i][e] += u[i][e] * sc[i][e];
+                v[i][e] += u[i][e] * w[e];
+                if (!KEEP) asm volatile("" : "+v"(v[i][e]));  // before the next loads, not where it is stored
             }
+        }
+        afresh();
         fetch(at + step);
+        afresh();
         if (at < a.positions) {
             T* po = (T*)a.xo.p + join_at(a.xo, a.width, at);
 #pragma unroll
@@ -212,7 +255,7 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
                 V o;
 #pragma unroll
                 for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(v[i][e]);
-                if (on[i]) *(V*)(po + (lane + p.tp * i) * VE) = o;
+                if (on[i]) *(V*)(po + vec(i)) = o;
             }
         }
         if (!PRE) continue;
@@ -238,14 +281,18 @@ __global__ void __launch_bounds__(1024) k_join(JoinArgs a, JoinPlan p) {
             s[i] = on[i] ? s[i] : 0.0f;
         }
         const float inv = 1.0f / sqrtf(sum.all(s) * inv_all + a.pre_eps);
+        afresh();
         if (at < a.positions) {
             T* ph = (T*)a.h.p + join_at(a.h, a.width, at);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 V o;
+                float w[VE], b[VE];
+                weight(nw, a.pre_w, i, 1.0f, w);
+                weight(nb, a.pre_b, i, 0.0f, b);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(v[i][e] * inv * nw[i][e] + nb[i][e]);
-                if (on[i]) *(V*)(ph + (lane + p.tp * i) * VE) = o;
+                for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(v[i][e] * inv * w[e] + b[e]);
+                if (on[i]) *(V*)(ph + vec(i)) = o;
             }
         }
     }
