@@ -3,6 +3,7 @@ bits: every norm, gate and storage type, group counts, channel counts from one t
 in place, infinities, the calls that are refused, and a run of the causal-context operators as a block."""
 
 import ctypes
+import time
 
 import numpy as np
 import pytest
@@ -315,3 +316,29 @@ def test_a_causal_context_block(prec):
         assert rel <= 5 * 4 * HALF_STEP[prec], rel
     del t, conv, qkv, y, xo, hh
     e.close()
+
+
+@pytest.mark.parametrize("prec", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("c,groups", [(9, 3), (100, 4), (250, 5), (999, 333), (1001, 7), (1400, 7), (1536, 6), (2600, 200), (4096, 2),
+                                      (8190, 10), (8190, 2730), (9002, 2), (12000, 3), (16383, 5461), (16380, 1365)])
+@pytest.mark.parametrize("post", ["layer", "rms"])
+def test_groups_that_are_no_power_of_two(eng, prec, c, groups, post):
+    """Few long groups, many short ones, and several positions to a workgroup and one after another."""
+    run(eng, prec, 37 if c < 2000 else 3, c, groups=groups, post=post, act="silu", pre="rms", seed=5)
+
+
+def test_odd_groups_take_no_longer_than_the_size_accounts_for(eng):
+    """Two groups of 4501 channels, 600 positions: some 60 us of work (with every lane adding its whole group up 60 ms)."""
+    n, c = 600, 9002
+    rng = np.random.default_rng(6)
+    b = [DevBuf(to_raw(rng.standard_normal((n, c)), "bf16")) for _ in range(4)]
+    d = nn.norm_gate_residual_desc("bf16", b[0], b[1], None, b[2], b[3], positions=n, channels=c, post_norm="layer", post_groups=2,
+                                   pre_norm="rms")
+    for _ in range(3):  # the first call loads the kernel
+        eng.sync()
+        t = time.perf_counter()
+        for _ in range(5):
+            nn.norm_gate_residual_noalloc(eng, d)
+        eng.sync()
+        t = time.perf_counter() - t
+    assert t < 0.05, t
