@@ -511,8 +511,8 @@ __global__ void __launch_bounds__(64 * lin_waves(D, OUT), !OUT ? 4 : D == 128 ? 
     const int head = unit / c.tiles, col0 = unit % c.tiles * D;
     const int colw = col0 + wave * 16 * NV;   // the wave's value columns
     // Four waves share the query products: each of three makes one tile of them, weighed and in pieces, in LDS, at the
-    // price of one more barrier a chunk (12 ragged f16 sequences of 64 channels 84 -> 78 us, 65536 positions of 128
-    // bf16 channels 421 -> 410 us). The two waves of 32 channels would save half a tile's work each and make their own.
+    // price of one more barrier a chunk (12 ragged f16 sequences of 64 channels 87 -> 83 us, 65536 positions of 128
+    // bf16 channels 422 -> 411 us). The two waves of 32 channels would save half a tile's work each and make their own.
     constexpr bool SHARE = OUT && D > 32;
     const bool work = SHARE || colw < a.dv;
 
@@ -1075,9 +1075,9 @@ hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t 
 
 // A position takes the recurrent form 0.7 to 3 us, a chunk costs its 32 positions whether they are there or not, but a
 // state is read and written faster by the recurrent form (both, us: one f32 sequence of 4 heads of 32, no
-// states: 3 positions 4.7 and 4.7, 4 5.5 and 4.7; with states 4 5.8 and 6.1, 6 7.1 and 6.1; 500 f16 sequences of
-// 4 heads of 32 x 64 with states: 5 16.0 and 18.4; 64 bf16 ones of 16 heads of 128: 5 37.9 and 39.3, 6 41.0 and 39.7;
-// 500 f16 ones of 8 heads of 64 without: 3 16.5 and 21.8, 6 28.1 and 22.1).
+// states: 3 positions 4.8 and 4.8, 4 5.6 and 4.9; with states 4 5.7 and 6.2, 6 7.2 and 6.2; 500 f16 sequences of
+// 4 heads of 32 x 64 with states: 5 16.2 and 19.2, 6 18.2 and 19.3; 64 bf16 ones of 16 heads of 128: 5 38.0 and 39.6,
+// 6 41.2 and 39.4; 500 f16 ones of 8 heads of 64 without: 3 16.1 and 22.2, 6 27.6 and 22.4).
 bool linear_prefers_recurrent(const LinAttnArgs& a) { return a.length <= (a.s_in || a.s_out ? 5 : 3); }
 
 LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
@@ -1089,10 +1089,10 @@ LinChunkPlan linear_chunk_plan(const LinAttnArgs& a, size_t scratch_bytes) {
     // A wave for every SIMD needs no segments (2160 waves of 240 positions: 16.6 us, in two segments 22.4). With
     // fewer, k and v are read twice, and two waves to a SIMD pay for it (65536 positions, 64 waves: in 16 segments
     // 490 us, in 32 404); with lengths, half of the segments may be empty (12 ragged sequences of up to 3001: six
-    // segments 77 us, eleven 71). A segment has at least as many bytes of channels as of state: 4096 positions in
+    // segments 90 us, eleven 83). A segment has at least as many bytes of channels as of state: 4096 positions in
     // five heads of 32, f32: one chunk a segment 16.4 us, two 17.5. The context's 33 MiB hold what 2048 waves ask for;
     // ragged batches of the widest heads get half of theirs (in 80 MiB, 12 sequences of up to 3001 in eight heads
-    // of 128, f16: 126 us instead of 119; 6 of up to 9000 126 instead of 144, 30 of up to 4000 296 instead of 265).
+    // of 128, f16: 139 us instead of 136; 6 of up to 9000 150 instead of 183, 30 of up to 4000 360 instead of 343).
     const long long want = waves >= 1024 ? 1 : ((a.lengths ? 4096 : 2048) + waves - 1) / waves;
     const int kept = a.s_in && a.s_in == a.s_out;  // states updated in place have a copy in the scratch
     const long long n = std::max(std::min(std::min(std::min(want, 1024LL), chunks * 32 / p.width), (long long)(scratch_bytes / state) + 1 - kept), 1LL);
