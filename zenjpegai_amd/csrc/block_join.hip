@@ -4,7 +4,7 @@
 //
 // HBM bound: five arrays pass once (x, y, gate in, x_out, h out). A position belongs to a team of TP lanes
 // (a power of two), a lane to the vectors lane + TP i of its channels, so the five weight vectors
-// are loaded once and stay in registers over the positions a team walks through; a position's whole
+// are loaded once and stay in registers over the positions a team walks through (up to 8192 channels); a position's whole
 // arithmetic runs on registers. The next position's loads are issued before this one's sums.
 
 #include <algorithm>

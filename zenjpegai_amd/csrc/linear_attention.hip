@@ -212,7 +212,8 @@ const char* type_name(int dtype) { return dtype == DT_F32 ? "float" : dtype == D
 //    values they meet (exactly: 11 bits), in all four products: the smallest is up to 2^-14 of the term where the
 //    first pieces are cut off, always of its sign (three products: 65536 f16 positions 553 us instead of 573);
 //  - the weighted values g^(31-j) v_j, which the state's f32 sums are made of, as three bf16 pieces (exactly), and the
-//    f16 keys they meet as two (exactly); of the six products the smallest is left out (2^-24). Two f16
+//    f16 keys they meet as two (exactly); of the six products the smallest is left out (2^-24). (Weighted values
+//    below 2^-110 lose low bits.) Two f16
 //    pieces of a weighted value are two products instead of five (12 ragged sequences of 64 x 128 channels 72 us
 //    instead of 81, 65536 positions of 16 heads of 128 447 instead of 547), but end at 2^-36, where a decay
 //    of a half is after a chunk: a value that zeros follow is then lost from the state.
