@@ -322,6 +322,171 @@ ZJAI_API int32_t zjai_linear_attention_noalloc(zjai_ctx* ctx, const zjai_linear_
  * zjai_linear_attention_noalloc. */
 ZJAI_API int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_attention_desc* desc);
 
+/* --------------------------------------------------------- causal context: rotary positions */
+
+/* Rotary positions: channel pairs of each head turn by an angle that grows with the position, so that the
+ * products of queries and keys depend on their distance. Of the first rotary_dim channels of a head, pair i
+ * (i < rotary_dim / 2) at rotary position p becomes
+ *     (a, b) -> magnitude * (a cos(p f_i) - b sin(p f_i), a sin(p f_i) + b cos(p f_i))
+ * with the frequency f_i in radians a position; the other channels stay as they are. Stands in front of
+ * zjai_linear_attention, for its queries and keys. Angles are formed in 64 bits (a position's rounding stays
+ * 2^-53 of its angle however far it is), sines and products in f32, and each result is rounded once. No
+ * counterpart in the reference. */
+#define ZJAI_ROTARY_INTERLEAVED 0 /* pair i: channels 2i, 2i + 1 */
+#define ZJAI_ROTARY_HALVES 1      /* pair i: channels i, i + rotary_dim / 2 */
+
+/* Positions of a map's pixels (tensor form). */
+#define ZJAI_ROTARY_BY_RASTER 0  /* their index in raster order */
+#define ZJAI_ROTARY_BY_COLUMN 1  /* their column: every row is a sequence of its own */
+#define ZJAI_ROTARY_BY_BOTH 2    /* the first half of the pairs turns by the row, the second by the column */
+
+/* Turns the first heads * head_dim channels of x in place (of packed [q | k | v]: with twice the heads of the
+ * attention both queries and keys). frequencies: rotary_dim / 2 doubles on the host. inverse = 1 turns the other way round. */
+ZJAI_API int32_t zjai_rotary(zjai_ctx* ctx, zjai_tensor* x, int32_t heads, int32_t head_dim, int32_t rotary_dim,
+                             int32_t layout, int32_t by, int32_t inverse, const double* frequencies, float magnitude);
+
+/* On the caller's device buffers. Element strides; the heads of a position are dense. `out` may be x, with
+ * x's strides; it overlaps x in no other way. Pointers are aligned to their element; 16-byte aligned buffers
+ * and strides, head_dim, rotary_dim (HALVES: its half) of whole 16 bytes run fastest. */
+typedef struct zjai_rotary_desc {
+    int32_t precision, heads;
+    int32_t head_dim, rotary_dim; /* head_dim 1..1024; rotary_dim even, 2..head_dim */
+    int32_t layout, inverse;
+    int32_t width;                /* 0: every pair turns by the rotary position p. Else p is a place of a map of
+                                     `width` columns in raster order, the first half of the pairs turns by its
+                                     row and the second by its column (rotary_dim a multiple of 4) */
+    int32_t sequences, length;    /* length: up to 2^30 */
+    float magnitude;              /* of the turned channels (1: lengths stay) */
+    const void* x;
+    void* out;
+    int64_t x_position, out_position; /* from one position to the next */
+    int64_t x_sequence, out_sequence; /* from one sequence to the next */
+    const double* frequencies;    /* device, [rotary_dim / 2] */
+    const int32_t* positions;     /* device, [sequences][length], or NULL (0, 1, ..) */
+    const int32_t* starts;        /* device, [sequences], or NULL (zeros): added to a sequence's positions (the
+                                     sum is taken modulo 2^32, as an int32) */
+    const int32_t* lengths;       /* device, [sequences], or NULL (all of `length`): positions a sequence has,
+                                     taken into 0..length; outputs past them stay as they were */
+} zjai_rotary_desc;
+/* Enqueued on the context's stream, as zjai_linear_attention_noalloc; allocates nothing and uses no scratch. */
+ZJAI_API int32_t zjai_rotary_noalloc(zjai_ctx* ctx, const zjai_rotary_desc* desc);
+
+/* Frequencies for a length that the model was not trained on (host only; needs no context). Without scaling
+ * f_i = base^(-2i / rotary_dim). With factor s:
+ *  LINEAR: f_i / s (positions squeezed);
+ *  NTK: the base becomes base * s^(rotary_dim / (rotary_dim - 2)) (the slowest pair's frequency is divided
+ *       by s, the fastest one's stays; rotary_dim >= 4);
+ *  YARN: pair i turns r_i = trained_length f_i / (2 pi) times over the trained length; with
+ *       g_i = (r_i - 1) / 31, taken into 0..1, f_i becomes g_i f_i + (1 - g_i) f_i / s, and the magnitude
+ *       is 0.1 ln s + 1.
+ * base > 0, factor >= 1; trained_length > 0 is used by YARN alone. frequencies: rotary_dim / 2 doubles;
+ * *magnitude: 1 except with YARN. For a map by row and column a caller puts the frequencies of rotary_dim / 2
+ * twice, one behind the other. */
+#define ZJAI_ROTARY_SCALE_NONE 0
+#define ZJAI_ROTARY_SCALE_LINEAR 1
+#define ZJAI_ROTARY_SCALE_NTK 2
+#define ZJAI_ROTARY_SCALE_YARN 3
+ZJAI_API int32_t zjai_rotary_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor,
+                                         double trained_length, double* frequencies, float* magnitude);
+
+/* ------------------------------------------------- causal context: short causal convolution */
+
+/* A convolution of each channel with itself over the last positions of its sequence:
+ *     out_t[c] = act(bias[c] + sum_(j < taps) weight[c][j] x_(t - taps + 1 + j)[c])
+ * with zeros, or the inputs that state_in keeps, before the first position. It stands in front of
+ * zjai_selective_scan. Products and sums are f32, in the order of j from the bias on, and an output is rounded once. No counterpart
+ * in the reference, whose depthwise convolutions reach positions ahead.
+ *
+ * Tensor form: the positions of a map are one sequence in raster order (rows = 0), or every row is one (rows =
+ * 1). weight ([channels][taps]) and bias (or NULL) on the host; act: ZJAI_GATE_LINEAR (none), _SIGMOID, _SILU. */
+ZJAI_API int32_t zjai_causal_conv(zjai_ctx* ctx, const zjai_tensor* x, int32_t taps, const float* weight,
+                                  const float* bias, int32_t act, int32_t rows, zjai_tensor** out);
+
+/* On the caller's device buffers. Element strides; the channels of a position are dense. `out` shares no
+ * element with x, nor do the states with either. Pointers are aligned to their element; 16-byte aligned
+ * buffers, strides and channels of whole 16 bytes run fastest. */
+typedef struct zjai_causal_conv_desc {
+    int32_t precision, channels;  /* channels 1..2^20 */
+    int32_t taps, act;            /* taps 1..8 */
+    int32_t sequences, length;    /* length: up to 2^30 */
+    const void* x;
+    void* out;
+    int64_t x_position, out_position; /* from one position to the next */
+    int64_t x_sequence, out_sequence; /* from one sequence to the next */
+    const float* weight;          /* device, [channels][taps] */
+    const float* bias;            /* device, [channels], or NULL (zeros) */
+    const int32_t* lengths;       /* device, [sequences], or NULL (all of `length`): positions a sequence has,
+                                     taken into 0..length; outputs past them stay as they were */
+    const int32_t* slots;         /* step: device, [sequences], or NULL (sequence i has state i) */
+    int32_t num_slots;            /* step: states in state_in / state_out (0: as many as sequences) */
+    int32_t reserved;             /* 0 */
+    const void* state_in;         /* device, [sequences][taps - 1][channels] of the precision's type: the inputs
+                                     before the first position, oldest first; or NULL (zeros) */
+    void* state_out;              /* the inputs before the next position, or NULL; may be state_in, and overlaps
+                                     it in no other way */
+} zjai_causal_conv_desc;
+/* Whole sequences. desc->slots must be NULL. Enqueued on the context's stream, as
+ * zjai_linear_attention_noalloc; allocates nothing and uses no scratch. */
+ZJAI_API int32_t zjai_causal_conv_noalloc(zjai_ctx* ctx, const zjai_causal_conv_desc* desc);
+/* One position of each sequence (length 1, lengths NULL; both states given unless taps is 1). Sequence i reads
+ * state_in[slots[i]] and writes state_out[slots[i]]; states of other slots stay as they were. A slot
+ * outside 0..num_slots-1 marks an idle sequence, whose output stays as it was. Sequences with the same slot
+ * follow one another in their order, as consecutive positions. */
+ZJAI_API int32_t zjai_causal_conv_step(zjai_ctx* ctx, const zjai_causal_conv_desc* desc);
+
+/* ------------------------------------------- causal context: selective state-space scan */
+
+/* Every channel keeps state_dim states, whose decay and input depend on the position:
+ *     s_t = delta_t[c] + delta_bias[c];  with softplus: s_t = ln(1 + exp(s_t))
+ *     h_t[n] = exp(s_t a[c][n]) h_(t-1)[n] + s_t b_t[g][n] x_t[c]
+ *     out_t[c] = (sum_n c_t[g][n] h_t[n] + d[c] x_t[c]) * z_t[c] / (1 + exp(-z_t[c]))
+ * g = c / (channels / groups): the groups share b and c among their channels. States start at zero or at
+ * state_in. Like zjai_linear_attention it runs over a whole map of known latents at once or position by position
+ * (zjai_selective_scan_step), with the same result up to rounding. Sums, products and states are f32 whatever
+ * the precision, and an output is rounded once; the decay of a position is rounded to f32 like any factor, so
+ * that a memory of 2^k positions is kept to 2^(k - 23) of itself at worst. A non-finite x, delta or z of a
+ * channel reaches the outputs of this channel at its own position (z) and at later ones only, b or c those of its
+ * group's channels (infinities may arrive there as NaN), a state_in those of its channel. No counterpart in the
+ * reference.
+ *
+ * Tensor form: x, delta and z (or NULL: no gate) of one shape; bc: 2 * groups * state_dim channels, b ([groups]
+ * [state_dim]) and c behind one another; a ([channels][state_dim]), d and delta_bias ([channels], or NULL: zeros)
+ * on the host. rows as in zjai_causal_conv. */
+ZJAI_API int32_t zjai_selective_scan(zjai_ctx* ctx, const zjai_tensor* x, const zjai_tensor* delta,
+                                     const zjai_tensor* bc, const zjai_tensor* z, int32_t groups,
+                                     int32_t state_dim, const float* a, const float* d, const float* delta_bias,
+                                     int32_t softplus, int32_t rows, zjai_tensor** out);
+
+/* On the caller's device buffers. Element strides; the channels (x, delta, z, out) or [groups][state_dim] (b,
+ * c) of a position are dense. `out` shares no element with an input. Pointers are aligned to their element;
+ * groups of a multiple of 64 channels run fastest (those of fewer take a wave all the same). */
+typedef struct zjai_selective_scan_desc {
+    int32_t precision, channels;   /* channels 1..2^20 */
+    int32_t groups, state_dim;     /* groups divides channels; state_dim 1..256 */
+    int32_t sequences, length;     /* length: up to 2^30; sequences * groups * (waves of a group's channels): up to
+                                      2^22 (else ZJAI_E_LIMIT) */
+    int32_t softplus;              /* 1: the steps are taken through softplus */
+    int32_t num_slots;             /* step: states in state_in / state_out (0: as many as sequences) */
+    const void *x, *delta, *b, *c;
+    const void* z;                 /* or NULL: no gate */
+    void* out;
+    int64_t x_position, delta_position, b_position, c_position, z_position, out_position; /* to the next position */
+    int64_t x_sequence, delta_sequence, b_sequence, c_sequence, z_sequence, out_sequence; /* to the next sequence */
+    const float* a;                /* device, [channels][state_dim], at most 0 for states that do not grow */
+    const float* d;                /* device, [channels], or NULL (zeros) */
+    const float* delta_bias;       /* device, [channels], or NULL (zeros) */
+    const int32_t* lengths;        /* as in zjai_causal_conv_desc */
+    const int32_t* slots;          /* as in zjai_causal_conv_desc */
+    const float* state_in;         /* device, [sequences][channels][state_dim], or NULL (zeros) */
+    float* state_out;              /* the states after the last position, or NULL; may be state_in, and overlaps
+                                      it in no other way */
+} zjai_selective_scan_desc;
+/* Whole sequences. desc->slots must be NULL. Enqueued on the context's stream and working in its scratch, as
+ * zjai_linear_attention_noalloc, with the same rule for captured graphs. */
+ZJAI_API int32_t zjai_selective_scan_noalloc(zjai_ctx* ctx, const zjai_selective_scan_desc* desc);
+/* One position of each sequence (length 1, lengths NULL, both states given); slots as in zjai_causal_conv_step. */
+ZJAI_API int32_t zjai_selective_scan_step(zjai_ctx* ctx, const zjai_selective_scan_desc* desc);
+
 /* ---------------------------------------------- the join of two blocks: norms, gate, residual */
 
 #define ZJAI_NORM_NONE 0

@@ -43,6 +43,9 @@ FAIL_NONE, FAIL_ALLOC, FAIL_LAUNCH = 0, 1, 2  # zjai_inject_failure kinds
 RESIZE_BICUBIC, RESIZE_BILINEAR = 0, 1
 NORMS = {"none": 0, "layer": 1, "rms": 2}  # ZJAI_NORM_*
 GATES = {"linear": 0, "sigmoid": 1, "silu": 2}  # ZJAI_GATE_*
+ROTARY_LAYOUTS = {"interleaved": 0, "halves": 1}  # ZJAI_ROTARY_*
+ROTARY_BY = {"raster": 0, "column": 1, "both": 2}  # ZJAI_ROTARY_BY_*
+ROTARY_SCALES = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}  # ZJAI_ROTARY_SCALE_*
 PLANE_LATENT, PLANE_PSI, PLANE_HYPER_LATENT, PLANE_IMAGE = 0, 1, 2, 3
 
 
@@ -80,6 +83,31 @@ class ZjaiLinearAttentionDesc(ctypes.Structure):
                     "q_sequence", "k_sequence", "v_sequence", "out_sequence")]
                 + [("decay", ctypes.c_void_p), ("scale", ctypes.c_float), ("num_slots", ctypes.c_int32)]
                 + [(n, ctypes.c_void_p) for n in ("lengths", "slots", "state_in", "state_out")])
+
+
+class ZjaiRotaryDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in (
+                    "precision", "heads", "head_dim", "rotary_dim", "layout", "inverse", "width", "sequences", "length")]
+                + [("magnitude", ctypes.c_float), ("x", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in ("x_position", "out_position", "x_sequence", "out_sequence")]
+                + [(n, ctypes.c_void_p) for n in ("frequencies", "positions", "starts", "lengths")])
+
+
+class ZjaiCausalConvDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("precision", "channels", "taps", "act", "sequences", "length")]
+                + [("x", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in ("x_position", "out_position", "x_sequence", "out_sequence")]
+                + [(n, ctypes.c_void_p) for n in ("weight", "bias", "lengths", "slots")]
+                + [("num_slots", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                + [("state_in", ctypes.c_void_p), ("state_out", ctypes.c_void_p)])
+
+
+class ZjaiSelectiveScanDesc(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in (
+                    "precision", "channels", "groups", "state_dim", "sequences", "length", "softplus", "num_slots")]
+                + [(n, ctypes.c_void_p) for n in ("x", "delta", "b", "c", "z", "out")]
+                + [(n + end, ctypes.c_int64) for end in ("_position", "_sequence") for n in ("x", "delta", "b", "c", "z", "out")]
+                + [(n, ctypes.c_void_p) for n in ("a", "d", "delta_bias", "lengths", "slots", "state_in", "state_out")])
 
 
 class ZjaiNormGateResidualDesc(ctypes.Structure):
@@ -147,6 +175,16 @@ PROTOTYPES = {
     "zjai_linear_attention": [_vp, _vp, _i32, _i32, _f32p, ctypes.c_float, _i32, _pp],
     "zjai_linear_attention_noalloc": [_vp, ctypes.POINTER(ZjaiLinearAttentionDesc)],
     "zjai_linear_attention_step": [_vp, ctypes.POINTER(ZjaiLinearAttentionDesc)],
+    "zjai_rotary": [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(ctypes.c_double), ctypes.c_float],
+    "zjai_rotary_noalloc": [_vp, ctypes.POINTER(ZjaiRotaryDesc)],
+    "zjai_rotary_frequencies": [_i32, ctypes.c_double, _i32, ctypes.c_double, ctypes.c_double,
+                                ctypes.POINTER(ctypes.c_double), _f32p],
+    "zjai_causal_conv": [_vp, _vp, _i32, _f32p, _f32p, _i32, _i32, _pp],
+    "zjai_causal_conv_noalloc": [_vp, ctypes.POINTER(ZjaiCausalConvDesc)],
+    "zjai_causal_conv_step": [_vp, ctypes.POINTER(ZjaiCausalConvDesc)],
+    "zjai_selective_scan": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32p, _f32p, _f32p, _i32, _i32, _pp],
+    "zjai_selective_scan_noalloc": [_vp, ctypes.POINTER(ZjaiSelectiveScanDesc)],
+    "zjai_selective_scan_step": [_vp, ctypes.POINTER(ZjaiSelectiveScanDesc)],
     "zjai_norm_gate_residual": [_vp, _vp, _vp, _vp, _i32, _i32, _i32, ctypes.c_float, _f32p, _f32p, _f32p,
                                 _i32, ctypes.c_float, _f32p, _f32p, _pp, _pp],
     "zjai_norm_gate_residual_noalloc": [_vp, ctypes.POINTER(ZjaiNormGateResidualDesc)],

@@ -742,6 +742,440 @@ extern "C" int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_a
     });
 }
 
+// ------------------------------------- causal context: rotary positions, causal convolution, selective scan
+namespace {
+
+// need with the operator's name in front, put together only where it is thrown.
+void need_in(bool ok, const char* what, const char* msg) {
+    if (!ok) throw Error(ZJAI_E_INVALID_ARGUMENT, std::string(what) + msg);
+}
+// What the descriptors of the operators on sequences have in common.
+struct SeqSide {
+    const void* p;
+    int64_t position, sequence, width;  // width: elements of a position
+};
+void check_sequences(int precision, int sequences, int length, const char* what) {
+    need(precision >= DT_F32 && precision <= DT_BF16, "precision");
+    need_in(sequences >= 0 && length >= 0, what, ": negative count");
+    if (length > LIN_MAX_LENGTH) throw Error(ZJAI_E_LIMIT, std::string(what) + ": more than 2^30 positions");
+}
+void check_side(const SeqSide& b, int es, const char* what) {
+    need_in(b.p != nullptr, what, ": null buffer");
+    need_in(((uintptr_t)b.p & (uintptr_t)(es - 1)) == 0, what, ": buffers not aligned to their element");
+    need_in(b.position >= 0 && b.sequence >= 0, what, ": negative stride");
+}
+// Outputs of two positions must not share elements: sequence after sequence, or position after position.
+void check_out(const SeqSide& o, int sequences, int length, const char* what) {
+    need_in(length == 1 || o.position >= o.width, what, ": output positions overlap");
+    need_in(sequences == 1 || o.sequence >= o.width, what, ": output sequences overlap");
+    const __int128 along = (__int128)(length - 1) * o.position + o.width, across = (__int128)(sequences - 1) * o.sequence + o.width;
+    need_in(sequences == 1 || length == 1 || o.sequence >= along || o.position >= across, what, ": output sequences overlap");
+}
+// The states of a call: `bytes` each.
+void check_states(bool step, int sequences, int length, const int32_t* lengths, const int32_t* slots, int num_slots, const void* in,
+                  const void* out, int es, uintptr_t bytes, const char* what) {
+    need_in(((uintptr_t)lengths & (uintptr_t)(4 - 1)) == 0, what, ": lengths not aligned");
+    need_in(((uintptr_t)slots & (uintptr_t)(4 - 1)) == 0, what, ": slots not aligned");
+    need_in(((uintptr_t)in & (uintptr_t)(es - 1)) == 0, what, ": states not aligned");
+    need_in(((uintptr_t)out & (uintptr_t)(es - 1)) == 0, what, ": states not aligned");
+    if (step) {
+        need_in(length == 1 && !lengths, what, " step: one position a sequence, no lengths");
+        need_in(bytes == 0 || (in && out), what, " step: null states");
+        need_in(num_slots >= 0 && (slots || num_slots == 0 || num_slots >= sequences), what, " step: slots");
+        need_in(!slots || num_slots > 0 || sequences == 0, what, " step: slots without their number");
+    } else {
+        need_in(!slots && num_slots == 0, what, ": slots are the recurrent form's");
+    }
+    if (in && out && in != out) {
+        const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out, n = (uintptr_t)(step && slots ? num_slots : sequences) * bytes;
+        need_in(a + n <= b || b + n <= a, what, ": states overlap");
+    }
+}
+LinRows rows_of(const SeqSide& b) { return LinRows{b.p, b.sequence, 0, b.position}; }
+
+void check_rotary(int heads, int dim, int turned, int layout, int inverse, bool map, float magnitude) {
+    need(heads > 0 && dim > 0, "rotary: head count and size");
+    if (dim > ROTARY_MAX_DIM) throw Error(ZJAI_E_UNSUPPORTED, "rotary: heads of more than 1024 channels");
+    if ((long long)heads * dim > 1 << 30) throw Error(ZJAI_E_LIMIT, "rotary: more than 2^30 channels");
+    need(turned > 0 && turned <= dim && turned % (map ? 4 : 2) == 0, "rotary: turned channels are not pairs (of each half) of a head's");
+    need(layout == ZJAI_ROTARY_INTERLEAVED || layout == ZJAI_ROTARY_HALVES, "rotary: layout");
+    need(inverse == 0 || inverse == 1, "rotary: inverse");
+    need(std::isfinite(magnitude), "rotary: magnitude");
+}
+void run_rotary(Context& C, const RotaryArgs& a, int dtype) {
+    const double n = (double)a.seqs * a.length * a.heads;
+    LaunchScope sc(C, rotary_name(a, dtype), 3.0 * n * a.turned, 2.0 * dtype_size(dtype) * n * (a.x.p == a.o.p ? a.turned : a.dim));
+    ZJAI_HIP(launch_rotary(a, dtype, C.stream));
+}
+
+void check_conv(int channels, int taps, int act) {
+    need(channels > 0 && taps > 0, "causal conv: channel and tap counts");
+    if (channels > SEQUENCE_MAX_CHANNELS) throw Error(ZJAI_E_UNSUPPORTED, "causal conv: more than 2^20 channels");
+    if (taps > CAUSAL_CONV_MAX_TAPS) throw Error(ZJAI_E_UNSUPPORTED, "causal conv: more than 8 taps");
+    need(act >= GATE_LINEAR && act <= GATE_SILU, "causal conv: act");
+}
+void run_conv(Context& C, const CausalConvArgs& a, int dtype, bool step) {
+    const double n = (double)a.seqs * a.length * a.channels;
+    // A step's grid has a lane for each channel of each sequence, which the launch counts in 32 bits.
+    if (step && (double)a.seqs * round_up(a.channels, 256) >= 4294967296.0) throw Error(ZJAI_E_LIMIT, "causal conv step: too many sequences");
+    LaunchScope sc(C, causal_conv_name(a, dtype, step), 2.0 * n * a.taps, 2.0 * dtype_size(dtype) * n);
+    if (step) ZJAI_HIP(launch_causal_conv_step(a, dtype, C.stream));
+    else ZJAI_HIP(launch_causal_conv(a, dtype, C.stream));
+}
+CausalConvArgs conv_args(const zjai_causal_conv_desc& d, bool step) {
+    check_sequences(d.precision, d.sequences, d.length, "causal conv");
+    check_conv(d.channels, d.taps, d.act);
+    need(d.reserved == 0, "causal conv: reserved");
+    const int es = dtype_size(d.precision);
+    const SeqSide x{d.x, d.x_position, d.x_sequence, d.channels}, o{d.out, d.out_position, d.out_sequence, d.channels};
+    if (d.sequences > 0 && d.length > 0) {
+        check_side(x, es, "causal conv");
+        check_side(o, es, "causal conv");
+        check_out(o, d.sequences, d.length, "causal conv");
+        need(d.x != d.out, "causal conv: out is x");
+    }
+    need(d.weight != nullptr, "causal conv: null weight");
+    need_aligned(d.weight, 4, "causal conv: weights not aligned");
+    need_aligned(d.bias, 4, "causal conv: weights not aligned");
+    check_states(step, d.sequences, d.length, d.lengths, d.slots, d.num_slots, d.state_in, d.state_out, es,
+                 (uintptr_t)(d.taps - 1) * d.channels * es, "causal conv");
+    CausalConvArgs a{};
+    a.x = rows_of(x);
+    a.o = rows_of(o);
+    a.seqs = d.sequences;
+    a.length = d.length;
+    a.channels = d.channels;
+    a.taps = d.taps;
+    a.act = d.act;
+    a.weight = d.weight;
+    a.bias = d.bias;
+    a.lengths = d.lengths;
+    a.slots = d.slots;
+    a.num_slots = d.num_slots;
+    a.s_in = d.state_in;
+    a.s_out = d.state_out;
+    return a;
+}
+
+void check_scan(int channels, int groups, int n, int softplus) {
+    need(channels > 0 && groups > 0 && n > 0 && channels % groups == 0, "selective scan: channel, group and state counts");
+    if (channels > SEQUENCE_MAX_CHANNELS) throw Error(ZJAI_E_UNSUPPORTED, "selective scan: more than 2^20 channels");
+    if (n > SCAN_MAX_STATES) throw Error(ZJAI_E_UNSUPPORTED, "selective scan: more than 256 states a channel");
+    need(softplus == 0 || softplus == 1, "selective scan: softplus");
+}
+double scan_bytes(const ScanArgs& a, int dtype) {
+    const double states = 4.0 * a.seqs * a.channels * a.n * ((a.s_in != nullptr) + (a.s_out != nullptr));
+    return (double)a.seqs * a.length * dtype_size(dtype) * ((3.0 + (a.z.p != nullptr)) * a.channels + 2.0 * a.groups * a.n) + states;
+}
+// SCAN_MAX_WAVES keeps a grid below 2^32 lanes where two waves a SIMD are cut into segments, the longest positions
+// (LIN_MAX_LENGTH) a position plus a segment in an int.
+void run_scan(Context& C, const ScanArgs& a, int dtype) {
+    const ScanPlan p = scan_plan(a, dtype, CONTEXT_SCRATCH_BYTES);
+    if ((double)a.seqs * a.groups * p.blocks > SCAN_MAX_WAVES) throw Error(ZJAI_E_LIMIT, "selective scan: more than 2^22 waves of sequences");
+    const double elems = (double)a.seqs * a.length * a.channels * a.n, ends = 4.0 * a.seqs * p.segments * a.channels * (a.n + 1.0);
+    float* scratch = (float*)C.top().scratch;
+    if (p.segments > 1) {
+        {
+            LaunchScope sc(C, scan_name(p, dtype, false), 5.0 * elems, scan_bytes(a, dtype) / 2 + ends);
+            ZJAI_HIP(launch_scan_ends(a, p, dtype, scratch, C.stream));
+        }
+        LaunchScope sc(C, "k_scan_starts", 0.75 * ends, 2.0 * ends);
+        ZJAI_HIP(launch_scan_starts(a, p, scratch, C.stream));
+    }
+    LaunchScope sc(C, scan_name(p, dtype, true), 7.0 * elems, scan_bytes(a, dtype) + (p.segments > 1 ? ends : 0.0));
+    ZJAI_HIP(launch_scan_outputs(a, p, dtype, scratch, C.stream));
+}
+void run_scan_step(Context& C, const ScanArgs& a, int dtype) {
+    // The grid's lanes, which the launch counts in 32 bits: one for four states, a power of two to a channel.
+    int lanes = 1;
+    while (lanes * 4 < a.n) lanes *= 2;
+    if (a.seqs * ((double)a.channels * lanes + 256) >= 4294967296.0) throw Error(ZJAI_E_LIMIT, "selective scan step: too many sequences");
+    LaunchScope sc(C, scan_step_name(a, dtype), 7.0 * a.seqs * a.channels * a.n, scan_bytes(a, dtype));
+    ZJAI_HIP(launch_scan_step(a, dtype, C.stream));
+}
+ScanArgs scan_args(const zjai_selective_scan_desc& d, bool step) {
+    check_sequences(d.precision, d.sequences, d.length, "selective scan");
+    check_scan(d.channels, d.groups, d.state_dim, d.softplus);
+    const int es = dtype_size(d.precision);
+    const int64_t bc = (int64_t)d.groups * d.state_dim;
+    const SeqSide x{d.x, d.x_position, d.x_sequence, d.channels}, delta{d.delta, d.delta_position, d.delta_sequence, d.channels},
+        b{d.b, d.b_position, d.b_sequence, bc}, c{d.c, d.c_position, d.c_sequence, bc}, z{d.z, d.z_position, d.z_sequence, d.channels},
+        o{d.out, d.out_position, d.out_sequence, d.channels};
+    if (d.sequences > 0 && d.length > 0) {
+        for (const SeqSide* side : {&x, &delta, &b, &c, &o}) check_side(*side, es, "selective scan");
+        if (d.z) check_side(z, es, "selective scan");
+        check_out(o, d.sequences, d.length, "selective scan");
+        for (const void* p : {d.x, d.delta, d.b, d.c, d.z}) need(p != d.out, "selective scan: out is an input");
+    }
+    need(d.a != nullptr, "selective scan: null a");
+    for (const float* p : {d.a, d.d, d.delta_bias}) need_aligned(p, 4, "selective scan: weights not aligned");
+    check_states(step, d.sequences, d.length, d.lengths, d.slots, d.num_slots, d.state_in, d.state_out, 4,
+                 (uintptr_t)d.channels * d.state_dim * 4, "selective scan");
+    ScanArgs a{};
+    a.x = rows_of(x);
+    a.delta = rows_of(delta);
+    a.b = rows_of(b);
+    a.c = rows_of(c);
+    a.z = rows_of(z);
+    a.o = rows_of(o);
+    a.seqs = d.sequences;
+    a.length = d.length;
+    a.channels = d.channels;
+    a.groups = d.groups;
+    a.n = d.state_dim;
+    a.softplus = d.softplus;
+    a.a = d.a;
+    a.d = d.d;
+    a.bias = d.delta_bias;
+    a.lengths = d.lengths;
+    a.slots = d.slots;
+    a.num_slots = d.num_slots;
+    a.s_in = d.state_in;
+    a.s_out = d.state_out;
+    return a;
+}
+
+// A map's positions as sequences: all of them in raster order, or row by row.
+struct MapRows {
+    int rows, width, seqs, length;  // width: of the rows, where they do not follow one another without a gap
+    MapRows(const Tensor& x, int rows_) : rows(rows_) {
+        need(x.n == 1, "one map");
+        need(rows == 0 || rows == 1, "rows");
+        need(rows || (long long)x.h * x.w <= LIN_MAX_LENGTH, "too many positions");
+        width = 0;
+        seqs = rows ? x.h : 1;
+        length = rows ? x.w : x.h * x.w;
+    }
+    // x's channels from c0 on.
+    LinRows part(const Tensor& x, int c0 = 0) {
+        if (!rows && x.v.row != (long long)x.w * x.v.cs) width = x.w;
+        return LinRows{(const char*)x.v.p + (size_t)(x.v.c_off + c0) * dtype_size(x.dtype), rows ? x.v.row : x.v.bstride, rows ? 0 : x.v.row, x.v.cs};
+    }
+};
+// Host arrays on the device for the time of a call, one behind the other, each from 16 bytes on.
+struct CallArrays {
+    Context& c;
+    std::shared_ptr<void> keep;
+    char* base = nullptr;
+    size_t used = 0;
+    CallArrays(Context& ctx, size_t bytes) : c(ctx) {
+        base = (char*)ctx.pool.alloc(bytes);
+        keep = std::shared_ptr<void>(base, [&ctx](void* q) { ctx.pool.release(q); });
+    }
+    template <typename E>
+    const E* put(const E* host, size_t n) {
+        if (!host) return nullptr;
+        char* to = base + used;
+        used += (n * sizeof(E) + 15) / 16 * 16;
+        ZJAI_HIP(hipMemcpyAsync(to, host, n * sizeof(E), hipMemcpyHostToDevice, c.stream));
+        return (const E*)to;
+    }
+};
+
+}  // namespace
+
+extern "C" int32_t zjai_rotary(zjai_ctx* ctx, zjai_tensor* x, int32_t heads, int32_t head_dim, int32_t rotary_dim, int32_t layout,
+                               int32_t by, int32_t inverse, const double* frequencies, float magnitude) {
+    if (!ctx || !x || !frequencies) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const Tensor& t = *x->t;
+        need(by >= ZJAI_ROTARY_BY_RASTER && by <= ZJAI_ROTARY_BY_BOTH, "rotary: by");
+        check_rotary(heads, head_dim, rotary_dim, layout, inverse, by == ZJAI_ROTARY_BY_BOTH, magnitude);
+        need((long long)heads * head_dim <= t.c, "rotary: more channels than the map has");
+        MapRows m(t, by == ZJAI_ROTARY_BY_COLUMN);
+        if (t.h == 0 || t.w == 0) return;
+        CallArrays arrays(ctx->c, sizeof(double) * rotary_dim / 2 + 16);
+        RotaryArgs a{};
+        a.freq = arrays.put(frequencies, rotary_dim / 2);
+        a.x = a.o = m.part(t);
+        a.width = m.width;
+        a.seqs = m.seqs;
+        a.length = m.length;
+        a.heads = heads;
+        a.dim = head_dim;
+        a.turned = rotary_dim;
+        a.halves = layout == ZJAI_ROTARY_HALVES;
+        a.inverse = inverse;
+        a.map = by == ZJAI_ROTARY_BY_BOTH ? t.w : 0;
+        a.magnitude = magnitude;
+        run_rotary(ctx->c, a, t.dtype);
+        count_f16_range(ctx->c, *channel_view(x->t, 0, heads * head_dim));
+        ZJAI_HIP(hipStreamSynchronize(ctx->c.stream));
+    });
+}
+
+extern "C" int32_t zjai_rotary_noalloc(zjai_ctx* ctx, const zjai_rotary_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const zjai_rotary_desc& d = *desc;
+        check_sequences(d.precision, d.sequences, d.length, "rotary");
+        need(d.width >= 0, "rotary: width");
+        check_rotary(d.heads, d.head_dim, d.rotary_dim, d.layout, d.inverse, d.width > 0, d.magnitude);
+        need(d.frequencies != nullptr, "rotary: null frequencies");
+        need_aligned(d.frequencies, 8, "rotary: frequencies not aligned");
+        for (const int32_t* p : {d.positions, d.starts, d.lengths}) need_aligned(p, 4, "rotary: positions, starts or lengths not aligned");
+        if (d.sequences == 0 || d.length == 0) return;
+        const int es = dtype_size(d.precision), ch = d.heads * d.head_dim;
+        const SeqSide x{d.x, d.x_position, d.x_sequence, ch}, o{d.out, d.out_position, d.out_sequence, ch};
+        check_side(x, es, "rotary");
+        check_side(o, es, "rotary");
+        check_out(o, d.sequences, d.length, "rotary");
+        need(d.x != d.out || ((d.length == 1 || d.x_position == d.out_position) && (d.sequences == 1 || d.x_sequence == d.out_sequence)),
+             "rotary: in place with another stride");
+        RotaryArgs a{};
+        a.x = rows_of(x);
+        a.o = rows_of(o);
+        a.seqs = d.sequences;
+        a.length = d.length;
+        a.heads = d.heads;
+        a.dim = d.head_dim;
+        a.turned = d.rotary_dim;
+        a.halves = d.layout == ZJAI_ROTARY_HALVES;
+        a.inverse = d.inverse;
+        a.map = d.width;
+        a.magnitude = d.magnitude;
+        a.freq = d.frequencies;
+        a.positions = d.positions;
+        a.starts = d.starts;
+        a.lengths = d.lengths;
+        run_rotary(ctx->c, a, d.precision);
+    });
+}
+
+extern "C" int32_t zjai_rotary_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor, double trained_length,
+                                           double* frequencies, float* magnitude) {
+    return guard(nullptr, [&] {
+        need(frequencies && magnitude, "rotary frequencies: null output");
+        need(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= ROTARY_MAX_DIM, "rotary frequencies: rotary_dim");
+        need(scaling >= ZJAI_ROTARY_SCALE_NONE && scaling <= ZJAI_ROTARY_SCALE_YARN, "rotary frequencies: scaling");
+        need(std::isfinite(base) && base > 0.0, "rotary frequencies: base");
+        const bool yarn = scaling == ZJAI_ROTARY_SCALE_YARN;
+        need(scaling == ZJAI_ROTARY_SCALE_NONE || (std::isfinite(factor) && factor >= 1.0), "rotary frequencies: factor");
+        need(!yarn || (std::isfinite(trained_length) && trained_length > 0.0), "rotary frequencies: trained_length");
+        need(scaling != ZJAI_ROTARY_SCALE_NTK || rotary_dim >= 4, "rotary frequencies: one pair has no base to scale");
+        if (scaling == ZJAI_ROTARY_SCALE_NTK) base *= std::pow(factor, rotary_dim / (rotary_dim - 2.0));
+        for (int i = 0; i < rotary_dim / 2; ++i) {
+            double f = std::pow(base, -2.0 * i / rotary_dim);
+            if (scaling == ZJAI_ROTARY_SCALE_LINEAR) f /= factor;
+            if (yarn) {
+                const double turns = trained_length * f / 6.28318530717958647693, g = std::min(1.0, std::max(0.0, (turns - 1.0) / 31.0));
+                f = g * f + (1.0 - g) * f / factor;
+            }
+            frequencies[i] = f;
+        }
+        *magnitude = yarn ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    });
+}
+
+extern "C" int32_t zjai_causal_conv(zjai_ctx* ctx, const zjai_tensor* x, int32_t taps, const float* weight, const float* bias,
+                                    int32_t act, int32_t rows, zjai_tensor** out) {
+    if (!ctx || !x || !weight || !out) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const Tensor& t = *x->t;
+        check_conv(t.c, taps, act);
+        MapRows m(t, rows);
+        TensorP y = ctx->c.alloc(1, t.c, t.h, t.w, t.dtype);
+        if (t.h > 0 && t.w > 0) {
+            CallArrays arrays(ctx->c, sizeof(float) * t.c * (taps + 1) + 32);
+            CausalConvArgs a{};
+            a.weight = arrays.put(weight, (size_t)t.c * taps);
+            a.bias = arrays.put(bias, t.c);
+            a.x = m.part(t);
+            a.o = m.part(*y);
+            a.width = m.width;
+            a.seqs = m.seqs;
+            a.length = m.length;
+            a.channels = t.c;
+            a.taps = taps;
+            a.act = act;
+            run_conv(ctx->c, a, t.dtype, false);
+            count_f16_range(ctx->c, *y);
+            ZJAI_HIP(hipStreamSynchronize(ctx->c.stream));
+        }
+        *out = new zjai_tensor{y};
+    });
+}
+
+extern "C" int32_t zjai_causal_conv_noalloc(zjai_ctx* ctx, const zjai_causal_conv_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const CausalConvArgs a = conv_args(*desc, false);
+        if (a.seqs > 0 && (a.length > 0 || (a.s_out && a.taps > 1))) run_conv(ctx->c, a, desc->precision, false);
+    });
+}
+
+extern "C" int32_t zjai_causal_conv_step(zjai_ctx* ctx, const zjai_causal_conv_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const CausalConvArgs a = conv_args(*desc, true);
+        if (a.seqs > 0) run_conv(ctx->c, a, desc->precision, true);
+    });
+}
+
+extern "C" int32_t zjai_selective_scan(zjai_ctx* ctx, const zjai_tensor* x, const zjai_tensor* delta, const zjai_tensor* bc,
+                                       const zjai_tensor* z, int32_t groups, int32_t state_dim, const float* a_, const float* d,
+                                       const float* delta_bias, int32_t softplus, int32_t rows, zjai_tensor** out) {
+    if (!ctx || !x || !delta || !bc || !a_ || !out) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const Tensor& t = *x->t;
+        check_scan(t.c, groups, state_dim, softplus);
+        for (const zjai_tensor* o : {delta, bc, z})
+            need(!o || (o->t->n == t.n && o->t->h == t.h && o->t->w == t.w && o->t->dtype == t.dtype &&
+                        (o == bc ? (long long)o->t->c == 2LL * groups * state_dim : o->t->c == t.c)),
+                 "selective scan: shapes differ");
+        MapRows m(t, rows);
+        TensorP y = ctx->c.alloc(1, t.c, t.h, t.w, t.dtype);
+        if (t.h > 0 && t.w > 0) {
+            CallArrays arrays(ctx->c, sizeof(float) * t.c * (state_dim + 2) + 48);
+            ScanArgs a{};
+            a.a = arrays.put(a_, (size_t)t.c * state_dim);
+            a.d = arrays.put(d, t.c);
+            a.bias = arrays.put(delta_bias, t.c);
+            a.x = m.part(t);
+            a.delta = m.part(*delta->t);
+            a.b = m.part(*bc->t);
+            a.c = m.part(*bc->t, groups * state_dim);
+            if (z) a.z = m.part(*z->t);
+            a.o = m.part(*y);
+            a.width = m.width;
+            a.seqs = m.seqs;
+            a.length = m.length;
+            a.channels = t.c;
+            a.groups = groups;
+            a.n = state_dim;
+            a.softplus = softplus;
+            run_scan(ctx->c, a, t.dtype);
+            count_f16_range(ctx->c, *y);
+            ZJAI_HIP(hipStreamSynchronize(ctx->c.stream));
+        }
+        *out = new zjai_tensor{y};
+    });
+}
+
+extern "C" int32_t zjai_selective_scan_noalloc(zjai_ctx* ctx, const zjai_selective_scan_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const ScanArgs a = scan_args(*desc, false);
+        if (a.seqs > 0 && (a.length > 0 || a.s_out)) run_scan(ctx->c, a, desc->precision);
+    });
+}
+
+extern "C" int32_t zjai_selective_scan_step(zjai_ctx* ctx, const zjai_selective_scan_desc* desc) {
+    if (!ctx || !desc) return ZJAI_E_INVALID_ARGUMENT;
+    return guard(ctx, [&] {
+        const OnDevice on(ctx->c.device);
+        const ScanArgs a = scan_args(*desc, true);
+        if (a.seqs > 0) run_scan_step(ctx->c, a, desc->precision);
+    });
+}
+
 // --------------------------------------------------- the join of two blocks: norms, gate, residual
 namespace {
 

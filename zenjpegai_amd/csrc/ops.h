@@ -165,6 +165,64 @@ hipError_t launch_linear_outputs(const LinAttnArgs& a, const LinChunkPlan& p, in
 // The recurrent form: a workgroup keeps its part of a state in registers over the positions.
 std::string linear_recurrent_name(const LinAttnArgs& a, int dtype);
 hipError_t launch_linear_recurrent(const LinAttnArgs& a, int dtype, hipStream_t s);
+// Rotary positions (zjai_rotary): `heads` heads of `dim` channels, the first `turned` of each in pairs. Position t of
+// sequence s has rotary position positions[s * length + t] + starts[s] (t and 0 where they are absent).
+struct RotaryArgs {
+    LinRows x, o;  // o.p may be x.p
+    int width;     // of the rows x and o are laid out in (0: none)
+    int seqs, length, heads, dim, turned;
+    bool halves;  // pairs (i, i + turned / 2), not (2i, 2i + 1)
+    bool inverse;
+    int map;  // columns of the map whose rows and columns turn one half of the pairs each (0: none)
+    float magnitude;
+    const double* freq;
+    const int *positions, *starts, *lengths;
+};
+constexpr int ROTARY_MAX_DIM = 1024;
+std::string rotary_name(const RotaryArgs& a, int dtype);
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s);
+// Short causal convolution of each channel (zjai_causal_conv); states [..][taps - 1][channels] of the storage type.
+struct CausalConvArgs {
+    LinRows x, o;
+    int width;
+    int seqs, length, channels, taps, act;  // act: GateAct
+    const float *weight, *bias;             // bias may be null
+    const int *lengths, *slots;
+    int num_slots;
+    const void* s_in;
+    void* s_out;
+};
+constexpr int CAUSAL_CONV_MAX_TAPS = 8, SEQUENCE_MAX_CHANNELS = 1 << 20;
+std::string causal_conv_name(const CausalConvArgs& a, int dtype, bool step);
+hipError_t launch_causal_conv(const CausalConvArgs& a, int dtype, hipStream_t s);
+hipError_t launch_causal_conv_step(const CausalConvArgs& a, int dtype, hipStream_t s);
+// Selective state-space scan (zjai_selective_scan); states [..][channels][n] f32.
+struct ScanArgs {
+    LinRows x, delta, b, c, z, o;  // z.p may be null
+    int width;
+    int seqs, length, channels, groups, n;
+    int softplus;
+    const float *a, *d, *bias;  // d, bias may be null
+    const int *lengths, *slots;
+    int num_slots;
+    const float* s_in;
+    float* s_out;
+};
+constexpr int SCAN_MAX_STATES = 256, SCAN_MAX_WAVES = 1 << 22;  // waves: of all sequences, for one stretch of positions
+// `segments` stretches of seg_len positions of each sequence (the last one shorter) run side by side; a lane keeps `ns`
+// states of a channel, `lanes` lanes have one channel.
+struct ScanPlan {
+    int ns = 16, lanes = 1;
+    int blocks = 0;  // waves of a group's channels
+    int segments = 1, seg_len = 0;
+};
+ScanPlan scan_plan(const ScanArgs& a, int dtype, size_t scratch_bytes);
+std::string scan_name(const ScanPlan& p, int dtype, bool outputs);
+hipError_t launch_scan_ends(const ScanArgs& a, const ScanPlan& p, int dtype, float* scratch, hipStream_t s);
+hipError_t launch_scan_starts(const ScanArgs& a, const ScanPlan& p, float* scratch, hipStream_t s);
+hipError_t launch_scan_outputs(const ScanArgs& a, const ScanPlan& p, int dtype, const float* scratch, hipStream_t s);
+std::string scan_step_name(const ScanArgs& a, int dtype);
+hipError_t launch_scan_step(const ScanArgs& a, int dtype, hipStream_t s);
 // Norm, gate, residual scale, residual sum and norm of each position (zjai_norm_gate_residual): views of
 // N x [h][w][C] (x_out may be x; h may be y, g or x).
 enum NormKind : int { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };

@@ -411,6 +411,127 @@ def linear_attention_step(eng: Engine, desc: _lib.ZjaiLinearAttentionDesc) -> No
     check(lib().zjai_linear_attention_step(eng.handle, desc), eng.handle)
 
 
+# ------------------------------------------------------------- causal context: rotary positions
+_f64p = ctypes.POINTER(ctypes.c_double)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = "none", factor: float = 1.0,
+                       trained_length: float = 0.0):
+    """``zjai_rotary_frequencies``: ``(frequencies, magnitude)``, float64 [rotary_dim / 2] in radians a position, for
+    contexts ``factor`` times as long as those trained on (``scaling`` none, linear, ntk or yarn)."""
+    f, m = np.empty(max(rotary_dim // 2, 1), np.float64), ctypes.c_float()
+    check(lib().zjai_rotary_frequencies(rotary_dim, base, _lib.ROTARY_SCALES[scaling], factor, trained_length,
+                                        f.ctypes.data_as(_f64p), ctypes.byref(m)))
+    return f, m.value
+
+
+def rotary(eng: Engine, x: BTensor, heads: int, head_dim: int, frequencies, *, layout: str = "interleaved", by: str = "raster",
+           magnitude: float = 1.0, inverse: bool = False) -> None:
+    """Turns the first ``heads * head_dim`` channels of a map in place, ``2 * len(frequencies)`` channels of each head, by
+    the positions in raster order, by the column or (``both``) by row and column (``zjai_rotary``)."""
+    f = np.ascontiguousarray(np.ravel(frequencies), np.float64)
+    check(lib().zjai_rotary(eng.handle, x._h, heads, head_dim, 2 * f.size, _lib.ROTARY_LAYOUTS[layout], _lib.ROTARY_BY[by],
+                            int(inverse), f.ctypes.data_as(_f64p), magnitude), eng.handle)
+
+
+def _strides(length: int, given: dict, **positions) -> dict:
+    """Strides of dense buffers whose positions have the given sizes, with those that the caller gives in their place."""
+    st = {n + "_position": p for n, p in positions.items()}
+    st.update({n + "_sequence": p * length for n, p in positions.items()})
+    st.update(given)
+    return st
+
+
+def rotary_desc(precision: str, x, out, *, heads: int, head_dim: int, sequences: int, length: int, frequencies,
+                rotary_dim: int | None = None, layout: str = "interleaved", width: int = 0, magnitude: float = 1.0,
+                inverse: bool = False, positions=None, starts=None, lengths=None, **strides) -> _lib.ZjaiRotaryDesc:
+    """A descriptor for ``rotary_noalloc`` over device buffers (addresses, or objects with ``data_ptr()``, which the caller
+    keeps alive; ``frequencies``: float64), dense unless ``strides`` (``x_position=...``) says otherwise."""
+    c = heads * head_dim
+    return _lib.ZjaiRotaryDesc(
+        precision=_lib.PRECISIONS[precision], heads=heads, head_dim=head_dim,
+        rotary_dim=head_dim if rotary_dim is None else rotary_dim, layout=_lib.ROTARY_LAYOUTS[layout], inverse=int(inverse),
+        width=width, sequences=sequences, length=length, magnitude=magnitude, x=_address(x), out=_address(out),
+        frequencies=_address(frequencies), positions=_address(positions), starts=_address(starts),
+        lengths=_address(lengths), **_strides(length, strides, x=c, out=c))
+
+
+def rotary_noalloc(eng: Engine, desc: _lib.ZjaiRotaryDesc) -> None:
+    """``zjai_rotary_noalloc``: enqueued as ``linear_attention_noalloc``."""
+    check(lib().zjai_rotary_noalloc(eng.handle, desc), eng.handle)
+
+
+# ------------------------------ causal context: short causal convolution, selective state-space scan
+def causal_conv(eng: Engine, x: BTensor, weight, bias=None, *, act: str = "linear", rows: bool = False) -> BTensor:
+    """A convolution of each channel over the last positions, in raster order or (``rows``) row by row; weight
+    ``[channels][taps]`` (``zjai_causal_conv``)."""
+    w, b = _f32(weight), _f32(bias)
+    if w.ndim != 2 or w.shape[0] != x.c or (b is not None and b.shape != (x.c,)):
+        raise HipError(_lib.E_INVALID_ARGUMENT, "causal conv: weight is [channels][taps], bias [channels]")
+    out = ctypes.c_void_p()
+    check(lib().zjai_causal_conv(eng.handle, x._h, w.shape[1], _fp(w), _fp(b), _lib.GATES[act], int(rows), ctypes.byref(out)),
+          eng.handle)
+    return BTensor(eng, out)
+
+
+def causal_conv_desc(precision: str, x, out, *, channels: int, taps: int, sequences: int, length: int, weight, bias=None,
+                     act: str = "linear", lengths=None, slots=None, num_slots: int = 0, state_in=None, state_out=None,
+                     **strides) -> _lib.ZjaiCausalConvDesc:
+    """A descriptor for ``causal_conv_noalloc`` / ``causal_conv_step`` over device buffers (as for ``rotary_desc``)."""
+    return _lib.ZjaiCausalConvDesc(
+        precision=_lib.PRECISIONS[precision], channels=channels, taps=taps, act=_lib.GATES[act], sequences=sequences,
+        length=length, x=_address(x), out=_address(out), weight=_address(weight), bias=_address(bias),
+        lengths=_address(lengths), slots=_address(slots), num_slots=num_slots if slots is not None else 0, reserved=0,
+        state_in=_address(state_in), state_out=_address(state_out), **_strides(length, strides, x=channels, out=channels))
+
+
+def causal_conv_noalloc(eng: Engine, desc: _lib.ZjaiCausalConvDesc) -> None:
+    """``zjai_causal_conv_noalloc``: enqueued as ``linear_attention_noalloc``."""
+    check(lib().zjai_causal_conv_noalloc(eng.handle, desc), eng.handle)
+
+
+def causal_conv_step(eng: Engine, desc: _lib.ZjaiCausalConvDesc) -> None:
+    """``zjai_causal_conv_step``: enqueued as ``linear_attention_noalloc``."""
+    check(lib().zjai_causal_conv_step(eng.handle, desc), eng.handle)
+
+
+def selective_scan(eng: Engine, x: BTensor, delta: BTensor, bc: BTensor, a, z: BTensor | None = None, *, groups: int = 1,
+                   d=None, delta_bias=None, softplus: bool = True, rows: bool = False) -> BTensor:
+    """The selective state-space scan of a map, in raster order or (``rows``) row by row; ``bc`` holds b and c behind one another,
+    a is ``[channels][states]`` (``zjai_selective_scan``)."""
+    a, d, delta_bias = _f32(a), _f32(d), _f32(delta_bias)
+    if a.ndim != 2 or a.shape[0] != x.c or any(v is not None and v.shape != (x.c,) for v in (d, delta_bias)):
+        raise HipError(_lib.E_INVALID_ARGUMENT, "selective scan: a is [channels][states], d and delta_bias [channels]")
+    out = ctypes.c_void_p()
+    check(lib().zjai_selective_scan(eng.handle, x._h, delta._h, bc._h, z._h if z else None, groups, a.shape[1], _fp(a), _fp(d),
+                                    _fp(delta_bias), int(softplus), int(rows), ctypes.byref(out)), eng.handle)
+    return BTensor(eng, out)
+
+
+def selective_scan_desc(precision: str, x, delta, b, c, out, *, channels: int, state_dim: int, sequences: int, length: int, a,
+                        z=None, groups: int = 1, d=None, delta_bias=None, softplus: bool = True, lengths=None, slots=None,
+                        num_slots: int = 0, state_in=None, state_out=None, **strides) -> _lib.ZjaiSelectiveScanDesc:
+    """A descriptor for ``selective_scan_noalloc`` / ``selective_scan_step`` over device buffers (as for ``rotary_desc``)."""
+    bc = groups * state_dim
+    return _lib.ZjaiSelectiveScanDesc(
+        precision=_lib.PRECISIONS[precision], channels=channels, groups=groups, state_dim=state_dim, sequences=sequences,
+        length=length, softplus=int(softplus), num_slots=num_slots if slots is not None else 0, x=_address(x),
+        delta=_address(delta), b=_address(b), c=_address(c), z=_address(z), out=_address(out), a=_address(a), d=_address(d),
+        delta_bias=_address(delta_bias), lengths=_address(lengths), slots=_address(slots), state_in=_address(state_in),
+        state_out=_address(state_out),
+        **_strides(length, strides, x=channels, delta=channels, b=bc, c=bc, z=channels, out=channels))
+
+
+def selective_scan_noalloc(eng: Engine, desc: _lib.ZjaiSelectiveScanDesc) -> None:
+    """``zjai_selective_scan_noalloc``: enqueued as ``linear_attention_noalloc``."""
+    check(lib().zjai_selective_scan_noalloc(eng.handle, desc), eng.handle)
+
+
+def selective_scan_step(eng: Engine, desc: _lib.ZjaiSelectiveScanDesc) -> None:
+    """``zjai_selective_scan_step``: enqueued as ``linear_attention_noalloc``."""
+    check(lib().zjai_selective_scan_step(eng.handle, desc), eng.handle)
+
+
 # ---------------------------------------------- the join of two blocks: norms, gate, residual
 def norm_gate_residual(eng: Engine, x: BTensor, y: BTensor, gate: BTensor | None = None, *,
                        gate_act: str = "linear", post_norm: str = "none", post_groups: int = 1,
