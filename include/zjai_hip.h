@@ -463,8 +463,9 @@ ZJAI_API int32_t zjai_selective_scan(zjai_ctx* ctx, const zjai_tensor* x, const 
 typedef struct zjai_selective_scan_desc {
     int32_t precision, channels;   /* channels 1..2^20 */
     int32_t groups, state_dim;     /* groups divides channels; state_dim 1..256 */
-    int32_t sequences, length;     /* length: up to 2^30; sequences * groups * (waves of a group's channels): up to
-                                      2^22 (else ZJAI_E_LIMIT) */
+    int32_t sequences, length;     /* length: up to 2^30; sequences * groups * (workgroups of a group's
+                                      channels, of 256 / ceil(state_dim / 16) or a quarter of that): up to 2^20
+                                      (else ZJAI_E_LIMIT) */
     int32_t softplus;              /* 1: the steps are taken through softplus */
     int32_t num_slots;             /* step: states in state_in / state_out (0: as many as sequences) */
     const void *x, *delta, *b, *c;

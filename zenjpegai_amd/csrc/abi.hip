@@ -867,11 +867,11 @@ double scan_bytes(const ScanArgs& a, int dtype) {
     const double states = 4.0 * a.seqs * a.channels * a.n * ((a.s_in != nullptr) + (a.s_out != nullptr));
     return (double)a.seqs * a.length * dtype_size(dtype) * ((3.0 + (a.z.p != nullptr)) * a.channels + 2.0 * a.groups * a.n) + states;
 }
-// SCAN_MAX_WAVES keeps a grid below 2^32 lanes where two waves a SIMD are cut into segments, the longest positions
-// (LIN_MAX_LENGTH) a position plus a segment in an int.
+// SCAN_MAX_BLOCKS keeps a grid below 2^32 lanes (few workgroups alone are cut into segments), LIN_MAX_LENGTH a position
+// plus a segment in an int.
 void run_scan(Context& C, const ScanArgs& a, int dtype) {
-    const ScanPlan p = scan_plan(a, dtype, CONTEXT_SCRATCH_BYTES);
-    if ((double)a.seqs * a.groups * p.blocks > SCAN_MAX_WAVES) throw Error(ZJAI_E_LIMIT, "selective scan: more than 2^22 waves of sequences");
+    const ScanPlan p = scan_plan(a, CONTEXT_SCRATCH_BYTES);
+    if ((double)a.seqs * a.groups * p.blocks > SCAN_MAX_BLOCKS) throw Error(ZJAI_E_LIMIT, "selective scan: more than 2^20 workgroups of sequences");
     const double elems = (double)a.seqs * a.length * a.channels * a.n, ends = 4.0 * a.seqs * p.segments * a.channels * (a.n + 1.0);
     float* scratch = (float*)C.top().scratch;
     if (p.segments > 1) {
@@ -952,6 +952,20 @@ struct MapRows {
         return LinRows{(const char*)x.v.p + (size_t)(x.v.c_off + c0) * dtype_size(x.dtype), rows ? x.v.row : x.v.bstride, rows ? 0 : x.v.row, x.v.cs};
     }
 };
+// A map whose rows follow one another without a gap: t itself, or a copy.
+TensorP without_gaps(Context& c, const TensorP& t) {
+    if (t->v.row == (long long)t->w * t->v.cs || t->h <= 1 || t->w == 0) return t;
+    const size_t es = dtype_size(t->dtype), row = (size_t)t->w * t->v.cs * es;
+    char* base = (char*)c.pool.alloc(row * t->h);
+    auto d = std::make_shared<Tensor>(*t);
+    d->keep = std::shared_ptr<void>(base, [pool = c.pool_owner](void* q) { pool->release(q); });
+    d->base = base;
+    d->v.p = base;
+    d->v.row = (long long)t->w * t->v.cs;
+    d->v.bstride = d->v.row * t->h;
+    ZJAI_HIP(hipMemcpy2DAsync(base, row, t->v.p, t->v.row * es, row, t->h, hipMemcpyDeviceToDevice, c.stream));
+    return d;
+}
 // Host arrays on the device for the time of a call, one behind the other, each from 16 bytes on.
 struct CallArrays {
     Context& c;
@@ -1137,13 +1151,14 @@ extern "C" int32_t zjai_selective_scan(zjai_ctx* ctx, const zjai_tensor* x, cons
             a.a = arrays.put(a_, (size_t)t.c * state_dim);
             a.d = arrays.put(d, t.c);
             a.bias = arrays.put(delta_bias, t.c);
-            a.x = m.part(t);
-            a.delta = m.part(*delta->t);
-            a.b = m.part(*bc->t);
-            a.c = m.part(*bc->t, groups * state_dim);
-            if (z) a.z = m.part(*z->t);
+            const auto sequence = [&](const TensorP& v) { return rows ? v : without_gaps(ctx->c, v); };
+            const TensorP tx = sequence(x->t), td = sequence(delta->t), tb = sequence(bc->t), tz = z ? sequence(z->t) : nullptr;
+            a.x = m.part(*tx);
+            a.delta = m.part(*td);
+            a.b = m.part(*tb);
+            a.c = m.part(*tb, groups * state_dim);
+            if (z) a.z = m.part(*tz);
             a.o = m.part(*y);
-            a.width = m.width;
             a.seqs = m.seqs;
             a.length = m.length;
             a.channels = t.c;

@@ -198,8 +198,7 @@ hipError_t launch_causal_conv(const CausalConvArgs& a, int dtype, hipStream_t s)
 hipError_t launch_causal_conv_step(const CausalConvArgs& a, int dtype, hipStream_t s);
 // Selective state-space scan (zjai_selective_scan); states [..][channels][n] f32.
 struct ScanArgs {
-    LinRows x, delta, b, c, z, o;  // z.p may be null
-    int width;
+    LinRows x, delta, b, c, z, o;  // z.p may be null; no gaps between rows
     int seqs, length, channels, groups, n;
     int softplus;
     const float *a, *d, *bias;  // d, bias may be null
@@ -208,15 +207,15 @@ struct ScanArgs {
     const float* s_in;
     float* s_out;
 };
-constexpr int SCAN_MAX_STATES = 256, SCAN_MAX_WAVES = 1 << 22;  // waves: of all sequences, for one stretch of positions
+constexpr int SCAN_MAX_STATES = 256, SCAN_MAX_BLOCKS = 1 << 20;  // workgroups: of all sequences, for one stretch of positions
 // `segments` stretches of seg_len positions of each sequence (the last one shorter) run side by side; a lane keeps `ns`
 // states of a channel, `lanes` lanes have one channel.
 struct ScanPlan {
     int ns = 16, lanes = 1;
-    int blocks = 0;  // waves of a group's channels
+    int blocks = 0;  // workgroups of a group's channels
     int segments = 1, seg_len = 0;
 };
-ScanPlan scan_plan(const ScanArgs& a, int dtype, size_t scratch_bytes);
+ScanPlan scan_plan(const ScanArgs& a, size_t scratch_bytes);
 std::string scan_name(const ScanPlan& p, int dtype, bool outputs);
 hipError_t launch_scan_ends(const ScanArgs& a, const ScanPlan& p, int dtype, float* scratch, hipStream_t s);
 hipError_t launch_scan_starts(const ScanArgs& a, const ScanPlan& p, float* scratch, hipStream_t s);

@@ -2,12 +2,18 @@
 //   s_t = softplus(delta_t + bias),  h_t = exp(s_t a) h_(t-1) + s_t b_t x_t,
 //   out_t = (sum over the states of c_t h_t + d x_t) * silu(z_t).
 //
-// A wave has 64 / `lanes` channels of one group, a lane `ns` states of one of them, in registers over the positions. b and c
-// of a tile of positions, which all channels of a group share, go through LDS as f32.
+// A lane has NS states of one channel, in registers over the positions; LANES neighbouring lanes have a channel, four waves
+// of a workgroup 256 / LANES channels of one group. Positions pass in tiles of eight. What a tile needs for each channel
+// and position (the step, its softplus, the gate) is shared out among the channel's lanes and handed round by lane
+// exchanges; b and c, which all channels of a group share, go through LDS as f32. The next tile's loads are in
+// flight meanwhile.
+// Bound by the vector ALUs: five instructions and a 2^x for each position, channel and state.
 // Sequences that leave SIMDs idle are cut into segments: what each leaves behind when it starts from nothing (its end
-// states and the sum of its steps, which is all that its decays depend on), from those the states that each starts from, then the outputs of all.
+// states and the sum of its steps, which is all that its decays depend on), from those the states that each starts from, then
+// the outputs of all.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sequence.h"
 
@@ -15,38 +21,40 @@ namespace zjai {
 
 namespace {
 
-constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int SCAN_TILE = 8;  // positions whose loads are issued together
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int SCAN_TILE = 8, SCAN_WAVES = 4;
+constexpr int SCAN_RUN = 16, SCAN_MAX_SEGMENTS = 256;  // segments of a thread, and of 16 threads
 
-// ln(1 + exp(s)) = max(s, 0) + 2 artanh(e / (2 + e)) with e = exp(-|s|), by the series up to the fifteenth power of
-// an argument of at most 1/3 (what follows is below 2^-29 of it): small steps keep their accuracy, the hardware's 2^x
-// leaves (|s| + 2) 2^-24 of e.
+// ln(1 + exp(s)) = max(s, 0) + ln(1 + e) with e = exp(-|s|): the logarithm of the rounded 1 + e, and what the rounding left
+// of e beside it, so that small steps keep their accuracy (the hardware's 2^x leaves (|s| + 2) 2^-24 of e, its logarithm
+// 2^-23 of itself next to one, too).
 __device__ __forceinline__ float softplus(float s) {
     const float e = __builtin_amdgcn_exp2f(fabsf(s) * -LOG2E);
-    const float q = e * __builtin_amdgcn_rcpf(2.0f + e), q2 = q * q;
-    float p = fmaf(q2, 1.0f / 15.0f, 1.0f / 13.0f);
-    p = fmaf(p, q2, 1.0f / 11.0f);
-    p = fmaf(p, q2, 1.0f / 9.0f);
-    p = fmaf(p, q2, 1.0f / 7.0f);
-    p = fmaf(p, q2, 1.0f / 5.0f);
-    p = fmaf(p, q2, 1.0f / 3.0f);
-    p = fmaf(p, q2, 1.0f);
-    return fmaxf(s, 0.0f) + 2.0f * q * p;
+    const float u = 1.0f + e;
+    return __builtin_amdgcn_fmed3f(s, 0.0f, __builtin_inff()) + fmaf(__builtin_amdgcn_logf(u), LN2, e - (u - 1.0f));
 }
 
-// Sum over the 2^k neighbouring lanes of one channel; every one of them gets it.
+// Sum over the `lanes` neighbouring lanes of one channel; every one of them gets it.
 template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 __device__ __forceinline__ float lane_sum(float v, int lanes) {
-    if (lanes >= 2) v = dpp_add<0xb1>(v);    // quad_perm 1 0 3 2
-    if (lanes >= 4) v = dpp_add<0x4e>(v);    // quad_perm 2 3 0 1
-    if (lanes >= 8) v = dpp_add<0x141>(v);   // the other half of eight lanes
-    if (lanes >= 16) v = dpp_add<0x140>(v);  // ... of sixteen
+    if (lanes >= 2) v += dpp<0xb1>(v);    // quad_perm 1 0 3 2
+    if (lanes >= 4) v += dpp<0x4e>(v);    // quad_perm 2 3 0 1
+    if (lanes >= 8) v += dpp<0x141>(v);   // the other half of eight lanes
+    if (lanes >= 16) v += dpp<0x140>(v);  // ... of sixteen
     if (lanes >= 32) v += __shfl_xor(v, 16);
     if (lanes >= 64) v += __shfl_xor(v, 32);
     return v;
+}
+// The value of lane `owner` of the LANES neighbouring ones.
+template <int LANES, int OWNER>
+__device__ __forceinline__ float lane_value(float v) {
+    if constexpr (LANES == 1) return v;
+    else if constexpr (LANES == 2) return dpp<OWNER == 0 ? 0xa0 : 0xf5>(v);  // quad_perm 0 0 2 2, 1 1 3 3
+    else if constexpr (LANES == 4) return dpp<OWNER * 0x55>(v);
+    else return __shfl(v, (threadIdx.x & 63 & ~(LANES - 1)) | OWNER);
 }
 
 // A segment's states in the scratch: [sequences][segments][n][channels], then the sums of steps [sequences][segments][channels].
@@ -58,28 +66,42 @@ __device__ __forceinline__ long long step_slot(const ScanArgs& a, const ScanPlan
 }
 __device__ __forceinline__ int live_segments(const ScanPlan& p, int len) { return max(1, (len + p.seg_len - 1) / p.seg_len); }
 
-// OUT: the outputs of a segment; else what it leaves behind.
-template <typename T, int NS, bool OUT>
-__global__ void __launch_bounds__(64) k_scan(ScanArgs a, ScanPlan p, float* scratch) {
-    extern __shared__ float s_bc[];  // [SCAN_TILE][2][np]
-    const int lane = threadIdx.x, np = NS * p.lanes, per_seg = a.groups * p.blocks, grid_segs = OUT ? p.segments : p.segments - 1;
+// Compile-time loop: f(0), f(1), .. as constants.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each<N, I + 1>(f);
+    }
+}
+
+// OUT: the outputs of a segment; else what it leaves behind. Z: whether there is a gate.
+template <typename T, int NS, int LANES, bool OUT>
+__global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPlan p, float* scratch) {
+    constexpr int NP = NS * LANES < 4 ? 4 : NS * LANES;  // floats of a row of b or c in LDS
+    constexpr int SIDES = OUT ? 2 : 1, ITEMS = SCAN_TILE * SIDES * NP / 4, PER_LANE = (ITEMS + 64 * SCAN_WAVES - 1) / (64 * SCAN_WAVES);
+    constexpr int OWNERS = LANES < SCAN_TILE ? LANES : SCAN_TILE, OWN = SCAN_TILE / OWNERS;  // positions of a tile that a lane looks after
+    __shared__ float s_bc[2][SCAN_TILE][SIDES][NP];
+    const int tid = threadIdx.x, lane = tid & 63, per_seg = a.groups * p.blocks, grid_segs = OUT ? p.segments : p.segments - 1;
     int id = blockIdx.x;
     const int s = id / (per_seg * grid_segs);
     id -= s * per_seg * grid_segs;
     const int seg = id / per_seg;
     id -= seg * per_seg;
     const int g = id / p.blocks, cg = a.channels / a.groups;
-    const int at = (id - g * p.blocks) * (64 / p.lanes) + lane / p.lanes, part = lane & (p.lanes - 1);
+    const int at = (id - g * p.blocks) * (64 * SCAN_WAVES / LANES) + tid / LANES, part = lane & (LANES - 1);
     const bool on = at < cg;
     const int c = g * cg + (on ? at : 0);
     const int len = seq_length(a.lengths, s, a.length), live = live_segments(p, len);
     if (seg >= live || (!OUT && seg + 1 >= live)) return;
     const int t0 = seg * p.seg_len, t1 = min(len, t0 + p.seg_len);
 
+    // The lane's state i: quads of states go round the channel's lanes, so that those read neighbouring quads.
+    const auto state = [&](int i) { return NS < 4 ? i : ((i >> 2) * LANES + part) * 4 + (i & 3); };
     float rate[NS], h[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        const int n = part * NS + i;
+        const int n = state(i);
         rate[i] = n < a.n ? a.a[(long long)c * a.n + n] * LOG2E : 0.0f;
         h[i] = 0.0f;
         if (OUT && n < a.n) {
@@ -88,53 +110,208 @@ __global__ void __launch_bounds__(64) k_scan(ScanArgs a, ScanPlan p, float* scra
         }
     }
     const float bias = a.bias ? a.bias[c] : 0.0f, d = OUT && a.d ? a.d[c] : 0.0f;
+    const bool gate = OUT && a.z.p;
     double steps = 0.0;  // its rounding would grow with the positions, and what a segment keeps of its start with it
-    for (int t = t0; t < t1; t += SCAN_TILE) {
-        T xv[SCAN_TILE], dv[SCAN_TILE], zv[SCAN_TILE];
+
+    // A tile's inputs: the lane's share of x, delta and z, and of b and c in quads. Lanes without a channel or a quad of
+    // their own load the first ones: nothing here branches, so that loads and stores stay in flight over the tiles.
+    struct Tile {
+        T x[OWN], delta[OWN], z[OWN];
+        SeqVec<T, 4> bc[PER_LANE];
+    };
+    const int own = part & (OWNERS - 1);
+    const unsigned c_bytes = (unsigned)c * (unsigned)sizeof(T);
+    const auto item_of = [&](int k) { return min(tid + k * 64 * SCAN_WAVES, ITEMS - 1); };
+    // The channel's offset, made anew where it is added to a place that all lanes share: as the address's own 32 bits.
+    const auto channel = [&]() __attribute__((always_inline)) {
+        unsigned off = c_bytes;
+        asm volatile("" : "+v"(off));
+        return off;
+    };
+    const auto load = [&](const T* at, long long pos, T (&to)[OWN]) __attribute__((always_inline)) {
+        const unsigned off = channel();
 #pragma unroll
-        for (int i = 0; i < SCAN_TILE; ++i) {
-            const int u = min(t + i, t1 - 1);
-            xv[i] = ((const T*)a.x.p)[seq_at(a.x, a.width, s, u) + c];
-            dv[i] = ((const T*)a.delta.p)[seq_at(a.delta, a.width, s, u) + c];
-            if (OUT && a.z.p) zv[i] = ((const T*)a.z.p)[seq_at(a.z, a.width, s, u) + c];
+        for (int k = 0; k < OWN; ++k, at += OWNERS * pos) to[k] = *(const T*)((const char*)at + off);
+    };
+    const auto load_quad = [&](const T* at, int q, SeqVec<T, 4>& to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to.e[e] = at[min(q + e, a.n - 1)];
+    };
+    // Places of the next whole tile to load; they stay at the last one.
+    const LinRows& gate_rows = gate ? a.z : a.x;
+    const auto place = [&](const LinRows& r, long long t) { return (const T*)r.p + s * r.seq + t * r.pos; };
+    const long long own_at = LANES == 1 ? t0 : t0 + own;  // (one lane: the same for all of them)
+    const T *xp = place(a.x, own_at), *dp = place(a.delta, own_at), *zp = place(gate_rows, own_at), *bp[PER_LANE];
+    long long b_move[PER_LANE];
+#pragma unroll
+    for (int k = 0; k < PER_LANE; ++k) {
+        const int row = item_of(k) / (NP / 4);
+        const LinRows& r = row % SIDES ? a.c : a.b;
+        bp[k] = place(r, t0 + row / SIDES) + (long long)g * a.n;
+        b_move[k] = SCAN_TILE * r.pos;
+    }
+    const int whole = (t1 - t0) / SCAN_TILE;
+    int ahead = 0;  // whole tiles whose loads have been issued
+    const auto fetch = [&](Tile& v) __attribute__((always_inline)) {
+        load(xp, a.x.pos, v.x);
+        load(dp, a.delta.pos, v.delta);
+        if (OUT) load(zp, gate_rows.pos, v.z);
+#pragma unroll
+        for (int k = 0; k < PER_LANE; ++k) load_quad(bp[k], item_of(k) % (NP / 4) * 4, v.bc[k]);
+        const bool more = ++ahead < whole;
+        xp += more ? SCAN_TILE * a.x.pos : 0;
+        dp += more ? SCAN_TILE * a.delta.pos : 0;
+        if (OUT) zp += more ? SCAN_TILE * gate_rows.pos : 0;
+#pragma unroll
+        for (int k = 0; k < PER_LANE; ++k) bp[k] += more ? b_move[k] : 0;
+    };
+    T* op = OUT ? (T*)a.o.p + s * a.o.seq + own_at * a.o.pos : nullptr;
+    // n positions from t on (SCAN_TILE but for the last tile), with b and c in s_bc[buf].
+    const auto tile = [&](const Tile& v, auto buf_, int n, auto next) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_)::value;
+#pragma unroll
+        for (int k = 0; k < PER_LANE; ++k) {
+            const int item = tid + k * 64 * SCAN_WAVES, q = item_of(k) % (NP / 4) * 4, row = item_of(k) / (NP / 4);
+            f32x4 f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = q + e < a.n ? to_f32(v.bc[k].e[e]) : 0.0f;  // states past the last one: zeros
+            if (ITEMS >= (k + 1) * 64 * SCAN_WAVES || item < ITEMS) *(f32x4*)&s_bc[buf][row / SIDES][row % SIDES][q] = f;
         }
-        __syncthreads();
-        for (int e = lane; e < SCAN_TILE * np; e += 64) {
-            const int i = e / np, n = e - i * np, u = min(t + i, t1 - 1);
-            const bool there = n < a.n;
-            const long long k = (long long)g * a.n + (there ? n : 0);
-            const float b = to_f32(((const T*)a.b.p)[seq_at(a.b, a.width, s, u) + k]);
-            s_bc[2 * i * np + n] = there ? b : 0.0f;
+        float step[OWN], in[OWN], z[OWN], y[OWN];  // y: begins with d x
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            step[k] = to_f32(v.delta[k]) + bias;
+            in[k] = to_f32(v.x[k]);
             if (OUT) {
-                const float w = to_f32(((const T*)a.c.p)[seq_at(a.c, a.width, s, u) + k]);
-                s_bc[(2 * i + 1) * np + n] = there ? w : 0.0f;
+                y[k] = d * in[k];
+                z[k] = to_f32(v.z[k]);
             }
         }
+        if (a.softplus) {
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) step[k] = softplus(step[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) in[k] *= step[k];
         __syncthreads();
+        next();
+        if (!OUT) {
+            float sum[OWN];
 #pragma unroll
-        for (int i = 0; i < SCAN_TILE; ++i) {
-            if (t + i >= t1) break;
-            float step = to_f32(dv[i]) + bias;
-            if (a.softplus) step = softplus(step);
-            if (!OUT) steps += step;
-            const float x = to_f32(xv[i]), u = step * x;
-            const float* b = s_bc + 2 * i * np + part * NS;
-            float y = 0.0f;
+            for (int k = 0; k < OWN; ++k) sum[k] = part < OWNERS && k * OWNERS + own < n ? step[k] : 0.0f;
 #pragma unroll
-            for (int k = 0; k < NS; ++k) {
-                h[k] = fmaf(__builtin_amdgcn_exp2f(step * rate[k]), h[k], u * b[k]);
-                if (OUT) y = fmaf(b[np + k], h[k], y);
+            for (int m = OWN / 2; m > 0; m /= 2)
+#pragma unroll
+                for (int k = 0; k < m; ++k) sum[k] += sum[k + m];
+            steps += sum[0];
+        }
+        // A position's quads of states one after another. The quads of b and c are read from LDS AHEAD quads before
+        // they are used (the barriers keep the compiler from reading them where it needs them, and waiting).
+        constexpr int QUADS = NS < 4 ? 1 : NS / 4, AHEAD = 2;
+        f32x4 b[AHEAD + 1], w[AHEAD + 1];
+        const auto read = [&](auto at_) __attribute__((always_inline)) {
+            constexpr int at = decltype(at_)::value, i = at / QUADS, q = at % QUADS;
+            if constexpr (i < SCAN_TILE) {
+                b[at % (AHEAD + 1)] = *(const f32x4*)&s_bc[buf][i][0][(q * LANES + part) * 4];
+                if (OUT) w[at % (AHEAD + 1)] = *(const f32x4*)&s_bc[buf][i][SIDES - 1][(q * LANES + part) * 4];
             }
-            if (OUT) {
-                y = lane_sum(y, p.lanes);
-                if (a.d) y = fmaf(d, x, y);
-                if (a.z.p) {
-                    const float z = to_f32(zv[i]);
-                    y *= z * fast_sigmoid(z);
+        };
+        each<AHEAD>(read);
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int REGION = NS > 4 ? 1 : 4;  // quads between which the compiler may move things about
+        float st, u, o[SCAN_TILE];
+        each<SCAN_TILE * QUADS>([&](auto at_) __attribute__((always_inline)) {
+            constexpr int at = decltype(at_)::value, i = at / QUADS, q = at % QUADS, owner = i % OWNERS, k = i / OWNERS;
+            read(std::integral_constant<int, at + AHEAD>{});
+            if (q == 0) o[i] = 0.0f;
+            if (n < SCAN_TILE && i >= n) return;
+            if (q == 0) {
+                st = lane_value<LANES, owner>(step[k]);
+                u = lane_value<LANES, owner>(in[k]);
+                asm volatile("" : "+v"(st));  // its products and powers are formed here, not with all of the tile's
+                if (OUT && LANES == 1) o[i] = y[k];
+            }
+#pragma unroll
+            for (int e = 0; e < 4 && q * 4 + e < NS; ++e) {
+                float& x = h[q * 4 + e];
+                x = fmaf(__builtin_amdgcn_exp2f(st * rate[q * 4 + e]), x, u * b[at % (AHEAD + 1)][e]);
+                if (OUT) o[i] = fmaf(w[at % (AHEAD + 1)][e], x, o[i]);
+            }
+            if (at % REGION == REGION - 1) __builtin_amdgcn_sched_barrier(0);
+        });
+        if (OUT) {  // each position's sum over the channel's lanes, for the lane that looks after it
+            const bool p0 = part & 1, p1 = part & 2;
+            const auto pair = [&](float v0, float v1) { return (p0 ? v1 : v0) + dpp<0xb1>(p0 ? v0 : v1); };
+#pragma unroll
+            for (int k = 0; k < OWN; ++k) {
+                if constexpr (LANES == 1) y[k] = o[k];
+                else if constexpr (LANES == 2) y[k] += pair(o[2 * k], o[2 * k + 1]);
+                else if constexpr (LANES == 4) {
+                    const float v0 = pair(o[4 * k], o[4 * k + 1]), v1 = pair(o[4 * k + 2], o[4 * k + 3]);
+                    y[k] += (p1 ? v1 : v0) + dpp<0x4e>(p1 ? v0 : v1);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < OWNERS; ++i) {
+                        const float v = lane_sum(o[k * OWNERS + i], LANES);
+                        y[k] += own == i ? v : 0.0f;
+                    }
                 }
-                if (on && part == 0) ((T*)a.o.p)[seq_at(a.o, a.width, s, t + i) + c] = from_f32<T>(y);
             }
         }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) asm volatile("" : "+v"(h[i]));  // done here, not behind the next tile's branches
+        if (OUT) {
+            if (gate)
+#pragma unroll
+                for (int k = 0; k < OWN; ++k) y[k] *= z[k] * fast_sigmoid(z[k]);
+            T* o = op;
+            const unsigned off = channel();
+#pragma unroll
+            for (int k = 0; k < OWN; ++k, o += OWNERS * a.o.pos) {
+                // (A lane without a channel of its own has the first one's results, and writes them once more.)
+                if (LANES <= SCAN_TILE && n == SCAN_TILE) *(T*)((char*)o + off) = from_f32<T>(y[k]);
+                else if (on && part < OWNERS && k * OWNERS + own < n) o[c] = from_f32<T>(y[k]);
+            }
+            op += SCAN_TILE * a.o.pos;
+        }
+    };
+    typedef std::integral_constant<int, 0> Even;
+    typedef std::integral_constant<int, 1> Odd;
+    Tile even, odd;
+    if (whole > 0) {
+        fetch(even);
+        fetch(odd);
+    }
+    int j = 0;
+    for (; j + 1 < whole; j += 2) {
+        Tile v = even;
+        tile(v, Even(), SCAN_TILE, [&]() __attribute__((always_inline)) { fetch(even); });
+        v = odd;
+        tile(v, Odd(), SCAN_TILE, [&]() __attribute__((always_inline)) { fetch(odd); });
+    }
+    if (j < whole) tile(even, Even(), SCAN_TILE, []() {});
+    if (const int n = (t1 - t0) - whole * SCAN_TILE; n > 0) {
+        // Positions past the last one: its values, not used.
+        Tile v;
+        const int first = t0 + whole * SCAN_TILE;
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int t = min(first + k * OWNERS + own, t1 - 1);
+            v.x[k] = place(a.x, t)[c];
+            v.delta[k] = place(a.delta, t)[c];
+            if (OUT) v.z[k] = place(gate_rows, t)[c];
+        }
+#pragma unroll
+        for (int k = 0; k < PER_LANE; ++k) {
+            const int row = item_of(k) / (NP / 4);
+            load_quad(place(row % SIDES ? a.c : a.b, min(first + row / SIDES, t1 - 1)) + (long long)g * a.n, item_of(k) % (NP / 4) * 4, v.bc[k]);
+        }
+        if (j < whole) tile(v, Odd(), n, []() {});
+        else tile(v, Even(), n, []() {});
+    }
+    if (!OUT) {
+        const float sum = lane_sum((float)steps, LANES);
+        if (on && part == 0) scratch[step_slot(a, p, s, seg) + c] = sum;
     }
     if (!on) return;
     float* to = nullptr;
@@ -143,28 +320,49 @@ __global__ void __launch_bounds__(64) k_scan(ScanArgs a, ScanPlan p, float* scra
     if (!to) return;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        const int n = part * NS + i;
+        const int n = state(i);
         if (n < a.n) to[OUT ? ((long long)s * a.channels + c) * a.n + n : (long long)n * a.channels + c] = h[i];
     }
-    if (!OUT && part == 0) scratch[step_slot(a, p, s, seg) + c] = (float)steps;
 }
 
-// Each segment's end states become the states that it starts from.
-__global__ void __launch_bounds__(256) k_scan_starts(ScanArgs a, ScanPlan p, float* scratch) {
-    const long long each = (long long)a.n * a.channels, i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.seqs * each) return;
-    const int s = (int)(i / each);
-    const long long in_slot = i - s * each;
+// Each segment's end states become the states that it starts from. `parts` threads of a workgroup have a state, each
+// SCAN_RUN consecutive segments of it, whose loads are issued together; what a run makes of its start (a decay and an
+// end) goes to the later ones through LDS.
+__global__ void __launch_bounds__(256) k_scan_starts(ScanArgs a, ScanPlan p, int parts, float* scratch) {
+    __shared__ float s_keep[256], s_end[256];
+    const int items = 256 / parts, part = threadIdx.x / items, first = part * SCAN_RUN;
+    const long long size = (long long)a.n * a.channels, i = (long long)blockIdx.x * items + threadIdx.x % items;
+    const bool on = i < a.seqs * size;
+    const int s = on ? (int)(i / size) : 0;
+    const long long in_slot = on ? i - s * size : 0;
     const int n = (int)(in_slot / a.channels), c = (int)(in_slot - (long long)n * a.channels);
-    const int live = live_segments(p, seq_length(a.lengths, s, a.length));
-    const float rate = a.a[(long long)c * a.n + n] * LOG2E;
-    float h = a.s_in ? a.s_in[((long long)s * a.channels + c) * a.n + n] : 0.0f;
+    const int left = live_segments(p, seq_length(a.lengths, s, a.length)) - first;  // segments of the run, or none
     float* state = scratch + scan_slot(a, p, s, 0) + in_slot;
     const float* steps = scratch + step_slot(a, p, s, 0) + c;
-    for (int k = 0; k < live; ++k) {
-        const float end = k + 1 < live ? state[k * each] : 0.0f, sum = k + 1 < live ? steps[(long long)k * a.channels] : 0.0f;
-        state[k * each] = h;
-        h = fmaf(__builtin_amdgcn_exp2f(sum * rate), h, end);
+    float end[SCAN_RUN], keep[SCAN_RUN];
+#pragma unroll
+    for (int k = 0; k < SCAN_RUN; ++k) {  // the last segment leaves nothing behind (the first one's values in its place, not used)
+        const long long from = k + 1 < left ? first + k : 0;
+        end[k] = state[from * size];
+        keep[k] = steps[from * a.channels];
+    }
+    const float rate = a.a[(long long)c * a.n + n] * LOG2E;
+    float h = a.s_in ? a.s_in[((long long)s * a.channels + c) * a.n + n] : 0.0f, all = 1.0f, e = 0.0f;
+#pragma unroll
+    for (int k = 0; k < SCAN_RUN; ++k) {
+        keep[k] = __builtin_amdgcn_exp2f(keep[k] * rate);
+        e = fmaf(keep[k], e, end[k]);
+        all *= keep[k];
+    }
+    s_keep[threadIdx.x] = all;
+    s_end[threadIdx.x] = e;
+    __syncthreads();  // (and every state has been read before one is written)
+    for (int q = 0; q < part; ++q) h = fmaf(s_keep[threadIdx.x + (q - part) * items], h, s_end[threadIdx.x + (q - part) * items]);
+#pragma unroll
+    for (int k = 0; k < SCAN_RUN; ++k) {
+        if (!on || k >= left) break;
+        state[(first + k) * size] = h;
+        h = fmaf(keep[k], h, end[k]);
     }
 }
 
@@ -240,13 +438,18 @@ hipError_t scan_step(const ScanArgs& a, hipStream_t s) {
 template <typename T, bool OUT>
 hipError_t scan(const ScanArgs& a, const ScanPlan& p, float* scratch, hipStream_t s) {
     const unsigned grid = (unsigned)(a.seqs * (OUT ? p.segments : p.segments - 1) * a.groups * p.blocks);
-    const size_t lds = sizeof(float) * SCAN_TILE * 2 * p.ns * p.lanes;
-    switch (p.ns) {
-        case 1: k_scan<T, 1, OUT><<<grid, 64, lds, s>>>(a, p, scratch); break;
-        case 2: k_scan<T, 2, OUT><<<grid, 64, lds, s>>>(a, p, scratch); break;
-        case 4: k_scan<T, 4, OUT><<<grid, 64, lds, s>>>(a, p, scratch); break;
-        case 8: k_scan<T, 8, OUT><<<grid, 64, lds, s>>>(a, p, scratch); break;
-        default: k_scan<T, 16, OUT><<<grid, 64, lds, s>>>(a, p, scratch);
+    const dim3 block(64 * SCAN_WAVES);
+    switch (p.ns * 100 + p.lanes) {
+        case 101: k_scan<T, 1, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 401: k_scan<T, 4, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 404: k_scan<T, 4, 4, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 801: k_scan<T, 8, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1601: k_scan<T, 16, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1602: k_scan<T, 16, 2, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1604: k_scan<T, 16, 4, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1608: k_scan<T, 16, 8, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1616: k_scan<T, 16, 16, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        default: return hipErrorInvalidValue;
     }
     return hipGetLastError();
 }
@@ -259,19 +462,26 @@ hipError_t scan_any(const ScanArgs& a, const ScanPlan& p, int dtype, float* scra
 
 }  // namespace
 
-ScanPlan scan_plan(const ScanArgs& a, int dtype, size_t scratch_bytes) {
+ScanPlan scan_plan(const ScanArgs& a, size_t scratch_bytes) {
     ScanPlan p{};
     const int cg = a.channels / a.groups;
-    p.ns = 1;
-    while (p.ns < 16 && p.ns < a.n) p.ns *= 2;
+    p.ns = a.n == 1 ? 1 : a.n <= 4 ? 4 : a.n <= 8 ? 8 : 16;
     p.lanes = 1;
     while (p.ns * p.lanes < a.n) p.lanes *= 2;
-    p.blocks = (cg + 64 / p.lanes - 1) / (64 / p.lanes);
-    const double waves = (double)a.seqs * a.groups * p.blocks;
+    const auto waves = [&]() { return std::max(1.0, (double)a.seqs * a.groups * ((cg + 64 / p.lanes - 1) / (64 / p.lanes))); };
+    // Nine to sixteen states in one lane, or, where that leaves SIMDs idle even with segments of 64 positions, in four
+    // (64 x 64 positions of 320 channels x 16 states f32 36 -> 27 us, 24 of 64 11.1 -> 5.4).
+    if (p.ns == 16 && p.lanes == 1 && waves() * (a.length / 64.0) < 1024.0) {
+        p.ns = 4;
+        p.lanes = 4;
+    }
+    p.blocks = (cg + 64 * SCAN_WAVES / p.lanes - 1) / (64 * SCAN_WAVES / p.lanes);
+    // Segments for four waves a SIMD (65536 positions of 2048 channels x 16 states bf16: two 864 us, four 832, eight 879) or,
+    // where lengths may differ, which only the device knows, for eight (12 sequences of 0-3001, 1024 channels x 64 f16: two
+    // 939 us, four 640, eight 518), but none of less than 32 positions (the 64 x 64 map: 64 positions 31 us, 32 27, 16 29).
     const long long slot = 4LL * a.seqs * a.channels * (a.n + 1);
-    // Two waves a SIMD, of 32 positions at least.
-    long long segments = waves < 1 ? 1 : (long long)std::min(2048.0 / waves, a.length / 32.0);
-    segments = std::min<long long>(segments, (long long)scratch_bytes / std::max(slot, 1LL));
+    long long segments = (long long)std::min((a.lengths ? 8192 : 4096) / waves(), a.length / 32.0);
+    segments = std::min<long long>({segments, (long long)scratch_bytes / std::max(slot, 1LL), SCAN_MAX_SEGMENTS});
     p.segments = (int)std::max(1LL, segments);
     p.seg_len = std::max(1, (a.length + p.segments - 1) / p.segments);
     p.seg_len = (p.seg_len + SCAN_TILE - 1) / SCAN_TILE * SCAN_TILE;
@@ -280,14 +490,16 @@ ScanPlan scan_plan(const ScanArgs& a, int dtype, size_t scratch_bytes) {
 }
 
 std::string scan_name(const ScanPlan& p, int dtype, bool outputs) {
-    return std::string("k_scan<") + type_name(dtype) + ", " + std::to_string(p.ns) + (outputs ? ", true>" : ", false>");
+    return std::string("k_scan<") + type_name(dtype) + ", " + std::to_string(p.ns) + ", " + std::to_string(p.lanes) + (outputs ? ", true>" : ", false>");
 }
 hipError_t launch_scan_ends(const ScanArgs& a, const ScanPlan& p, int dtype, float* scratch, hipStream_t s) {
     return scan_any<false>(a, p, dtype, scratch, s);
 }
 hipError_t launch_scan_starts(const ScanArgs& a, const ScanPlan& p, float* scratch, hipStream_t s) {
-    const long long n = (long long)a.seqs * a.n * a.channels;
-    k_scan_starts<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, p, scratch);
+    int parts = 1;
+    while (parts * SCAN_RUN < p.segments) parts *= 2;
+    const long long n = (long long)a.seqs * a.n * a.channels, items = 256 / parts;
+    k_scan_starts<<<(unsigned)((n + items - 1) / items), 256, 0, s>>>(a, p, parts, scratch);
     return hipGetLastError();
 }
 hipError_t launch_scan_outputs(const ScanArgs& a, const ScanPlan& p, int dtype, const float* scratch, hipStream_t s) {
