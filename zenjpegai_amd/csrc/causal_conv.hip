@@ -2,7 +2,11 @@
 //   out_t = act(bias + sum_j w_j x_(t - taps + 1 + j)).
 //
 // HBM bound: inputs and outputs pass once. A lane owns four channels and walks a run of positions, the last
-// inputs kept in registers.
+// inputs kept in registers, the next eight positions' loads issued together. Runs of 16 positions: longer ones leave SIMDs
+// without work (135 rows of 240 positions of 384 channels bf16: 64 positions 18.2 us, 32 14.3, 16 11.9, 8 12.9, a copy
+// of as many bytes 9.9), shorter ones read more of the inputs twice (12 sequences of 0-3001 of 2048 f16: 51, 44, 42, 45).
+// Eight channels of 16 bits a lane halve the lanes (14.9 and 45 us); taking neighbouring runs to one XCD's L2 gains
+// nothing (11.8 and 43) or leaves XCDs without work where lengths differ (48).
 
 #include <algorithm>
 
@@ -17,13 +21,29 @@ constexpr int CONV_AHEAD = 8;  // positions whose loads are issued together
 struct ConvPlan {
     int vecs;       // accesses of a position
     int run, runs;  // positions of a run, runs of a sequence
+    bool wide;      // weights and bias 16-byte aligned
 };
 
 // Weights and bias of VE channels.
 template <int VE, int K>
 struct ConvWeights {
     float w[VE][K], b[VE];
-    __device__ __forceinline__ ConvWeights(const CausalConvArgs& a, int c) {
+    __device__ __forceinline__ ConvWeights(const CausalConvArgs& a, int c, bool wide) {
+        if (VE % 4 == 0 && wide) {  // 16 bytes at a time
+#pragma unroll
+            for (int i = 0; i < VE * K; i += 4) {
+                const f32x4 v = *(const f32x4*)(a.weight + (long long)c * K + i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[(i + k) / K][(i + k) % K] = v[k];
+            }
+#pragma unroll
+            for (int e = 0; e < VE; e += 4) {
+                const f32x4 v = a.bias ? *(const f32x4*)(a.bias + c + e) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) b[e + k] = v[k];
+            }
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
 #pragma unroll
@@ -70,7 +90,7 @@ __global__ void __launch_bounds__(256) k_causal_conv(CausalConvArgs a, ConvPlan 
             return v;
         };
         if (t0 < t1) {
-            const ConvWeights<VE, K> w(a, c);
+            const ConvWeights<VE, K> w(a, c, p.wide);
             float in[K + CONV_AHEAD - 1][VE];  // the last K - 1 inputs, then the new ones
 #pragma unroll
             for (int j = 0; j < K - 1; ++j) {
@@ -115,7 +135,7 @@ __global__ void __launch_bounds__(256) k_causal_conv(CausalConvArgs a, ConvPlan 
 
 // One position of each sequence: a workgroup takes a block of channels of one (or of all that share a slot).
 template <typename T, int VE, int K>
-__global__ void __launch_bounds__(256) k_causal_conv_step(CausalConvArgs a, int vecs, int blocks) {
+__global__ void __launch_bounds__(256) k_causal_conv_step(CausalConvArgs a, int vecs, int blocks, bool wide) {
     typedef SeqVec<T, VE> V;
     __shared__ int s_next;
     const int first = blockIdx.x / blocks, cv = (blockIdx.x - first * blocks) * blockDim.x + threadIdx.x;
@@ -123,7 +143,7 @@ __global__ void __launch_bounds__(256) k_causal_conv_step(CausalConvArgs a, int 
     if (!chain.begin(first)) return;
     const bool on = cv < vecs;
     const int c = on ? cv * VE : 0;
-    const ConvWeights<VE, K> w(a, c);
+    const ConvWeights<VE, K> w(a, c, wide);
     const long long sbase = (long long)chain.slot * (K - 1) * a.channels + c;
     V in[K];
 #pragma unroll
@@ -162,14 +182,16 @@ int conv_vector(const CausalConvArgs& a, int es) {
 template <typename T, int VE, int K>
 void conv_taps(const CausalConvArgs& a, bool step, hipStream_t s) {
     const int vecs = a.channels / VE;
+    const bool wide = (((uintptr_t)a.weight | (uintptr_t)a.bias) & 15) == 0;
     if (step) {
         const int threads = std::min(256, (vecs + 63) / 64 * 64), blocks = (vecs + threads - 1) / threads;
-        k_causal_conv_step<T, VE, K><<<(unsigned)(a.seqs * blocks), threads, 0, s>>>(a, vecs, blocks);
+        k_causal_conv_step<T, VE, K><<<(unsigned)(a.seqs * blocks), threads, 0, s>>>(a, vecs, blocks, wide);
         return;
     }
     ConvPlan p{};
     p.vecs = vecs;
-    p.run = 32;
+    p.run = 16;
+    p.wide = wide;
     p.runs = std::max(1, (a.length + p.run - 1) / p.run);
     const long long items = (long long)a.seqs * p.runs * vecs;
     k_causal_conv<T, VE, K><<<(unsigned)std::min<long long>((items + 255) / 256, 1 << 20), 256, 0, s>>>(a, p);

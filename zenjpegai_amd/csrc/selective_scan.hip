@@ -54,7 +54,10 @@ __device__ __forceinline__ float lane_value(float v) {
     if constexpr (LANES == 1) return v;
     else if constexpr (LANES == 2) return dpp<OWNER == 0 ? 0xa0 : 0xf5>(v);  // quad_perm 0 0 2 2, 1 1 3 3
     else if constexpr (LANES == 4) return dpp<OWNER * 0x55>(v);
-    else return __shfl(v, (threadIdx.x & 63 & ~(LANES - 1)) | OWNER);
+    else if constexpr (LANES == 8) {
+        const float mine = dpp<(OWNER & 3) * 0x55>(v), other = dpp<0x141>(mine);  // of the lane's four, of the other four
+        return ((threadIdx.x >> 2) & 1) == OWNER >> 2 ? mine : other;
+    } else return dpp<0x150 + OWNER>(v);  // row_newbcast
 }
 
 // A segment's states in the scratch: [sequences][segments][n][channels], then the sums of steps [sequences][segments][channels].
@@ -138,17 +141,17 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
         for (int e = 0; e < 4; ++e) to.e[e] = at[min(q + e, a.n - 1)];
     };
     // Places of the next whole tile to load; they stay at the last one.
-    const LinRows& gate_rows = gate ? a.z : a.x;
+    const LinRows gate_rows = gate ? a.z : a.x;
     const auto place = [&](const LinRows& r, long long t) { return (const T*)r.p + s * r.seq + t * r.pos; };
+    const auto side = [&](int row, long long t) { return (row % SIDES ? place(a.c, t) : place(a.b, t)) + (long long)g * a.n; };
     const long long own_at = LANES == 1 ? t0 : t0 + own;  // (one lane: the same for all of them)
     const T *xp = place(a.x, own_at), *dp = place(a.delta, own_at), *zp = place(gate_rows, own_at), *bp[PER_LANE];
     long long b_move[PER_LANE];
 #pragma unroll
     for (int k = 0; k < PER_LANE; ++k) {
         const int row = item_of(k) / (NP / 4);
-        const LinRows& r = row % SIDES ? a.c : a.b;
-        bp[k] = place(r, t0 + row / SIDES) + (long long)g * a.n;
-        b_move[k] = SCAN_TILE * r.pos;
+        bp[k] = side(row, t0 + row / SIDES);
+        b_move[k] = SCAN_TILE * (row % SIDES ? a.c.pos : a.b.pos);
     }
     const int whole = (t1 - t0) / SCAN_TILE;
     int ahead = 0;  // whole tiles whose loads have been issued
@@ -237,6 +240,10 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
                 x = fmaf(__builtin_amdgcn_exp2f(st * rate[q * 4 + e]), x, u * b[at % (AHEAD + 1)][e]);
                 if (OUT) o[i] = fmaf(w[at % (AHEAD + 1)][e], x, o[i]);
             }
+            if constexpr (OUT && LANES > 4 && q + 1 == QUADS) {
+                const float v = lane_sum(o[i], LANES);
+                y[k] += own == owner ? v : 0.0f;
+            }
             if (at % REGION == REGION - 1) __builtin_amdgcn_sched_barrier(0);
         });
         if (OUT) {  // each position's sum over the channel's lanes, for the lane that looks after it
@@ -249,12 +256,6 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
                 else if constexpr (LANES == 4) {
                     const float v0 = pair(o[4 * k], o[4 * k + 1]), v1 = pair(o[4 * k + 2], o[4 * k + 3]);
                     y[k] += (p1 ? v1 : v0) + dpp<0x4e>(p1 ? v0 : v1);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < OWNERS; ++i) {
-                        const float v = lane_sum(o[k * OWNERS + i], LANES);
-                        y[k] += own == i ? v : 0.0f;
-                    }
                 }
             }
         }
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
 #pragma unroll
         for (int k = 0; k < PER_LANE; ++k) {
             const int row = item_of(k) / (NP / 4);
-            load_quad(place(row % SIDES ? a.c : a.b, min(first + row / SIDES, t1 - 1)) + (long long)g * a.n, item_of(k) % (NP / 4) * 4, v.bc[k]);
+            load_quad(side(row, min(first + row / SIDES, t1 - 1)), item_of(k) % (NP / 4) * 4, v.bc[k]);
         }
         if (j < whole) tile(v, Odd(), n, []() {});
         else tile(v, Even(), n, []() {});
