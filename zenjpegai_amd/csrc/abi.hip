@@ -1097,9 +1097,9 @@ extern "C" int32_t zjai_causal_conv(zjai_ctx* ctx, const zjai_tensor* x, int32_t
             CausalConvArgs a{};
             a.weight = arrays.put(weight, (size_t)t.c * taps);
             a.bias = arrays.put(bias, t.c);
-            a.x = m.part(t);
+            const TensorP tx = rows ? x->t : without_gaps(ctx->c, x->t);
+            a.x = m.part(*tx);
             a.o = m.part(*y);
-            a.width = m.width;
             a.seqs = m.seqs;
             a.length = m.length;
             a.channels = t.c;

@@ -73,14 +73,13 @@ __global__ void __launch_bounds__(256) k_causal_conv(CausalConvArgs a, ConvPlan 
         const int c = cv * VE, len = seq_length(a.lengths, s, a.length), t0 = run * p.run, t1 = min(t0 + p.run, len);
         const bool keeps = run == 0 && K > 1 && a.s_out;  // a sequence's first run takes its state on as well
         if (t0 >= t1 && !keeps) continue;
-        const T* x = (const T*)a.x.p + c;
-        T* o = (T*)a.o.p + c;
+        const T* x = (const T*)a.x.p + s * a.x.seq + c;
         const T* before = a.s_in && K > 1 ? (const T*)a.s_in + (long long)s * (K - 1) * a.channels + c : nullptr;
         // The input at position t of the sequence, which may lie up to K - 1 positions before the first.
         const auto input = [&](int t) {
             V v;
             if (t >= 0) {
-                v = *(const V*)(x + seq_at(a.x, a.width, s, t));
+                v = *(const V*)(x + t * a.x.pos);
             } else if (before) {
                 v = *(const V*)(before + (long long)(t + K - 1) * a.channels);
             } else {
@@ -98,10 +97,15 @@ __global__ void __launch_bounds__(256) k_causal_conv(CausalConvArgs a, ConvPlan 
 #pragma unroll
                 for (int e = 0; e < VE; ++e) in[j][e] = to_f32(v.e[e]);
             }
+            const T* from = x + t0 * a.x.pos;
+            T* o = (T*)a.o.p + s * a.o.seq + t0 * a.o.pos + c;
             for (int t = t0; t < t1; t += CONV_AHEAD) {
                 V v[CONV_AHEAD];
 #pragma unroll
-                for (int i = 0; i < CONV_AHEAD; ++i) v[i] = *(const V*)(x + seq_at(a.x, a.width, s, min(t + i, t1 - 1)));
+                for (int i = 0; i < CONV_AHEAD; ++i) {
+                    v[i] = *(const V*)from;
+                    if (t + i + 1 < t1) from += a.x.pos;  // past the run's last position: it once more, not used
+                }
 #pragma unroll
                 for (int i = 0; i < CONV_AHEAD; ++i) {
                     V y;
@@ -113,7 +117,8 @@ __global__ void __launch_bounds__(256) k_causal_conv(CausalConvArgs a, ConvPlan 
                         for (int j = 0; j < K; ++j) sum = fmaf(w.w[e][j], in[i + j][e], sum);
                         y.e[e] = from_f32<T>(gate_act(sum, a.act));
                     }
-                    if (t + i < t1) *(V*)(o + seq_at(a.o, a.width, s, t + i)) = y;
+                    if (t + i < t1) *(V*)o = y;
+                    o += a.o.pos;
                 }
 #pragma unroll
                 for (int j = 0; j < K - 1; ++j)
@@ -172,7 +177,7 @@ int conv_vector(const CausalConvArgs& a, int es) {
     const auto fits = [&](int v) {
         if (a.channels % v) return false;
         for (const LinRows* r : {&a.x, &a.o})
-            if ((uintptr_t)r->p % (v * es) || r->pos % v || r->seq % v || (a.width && r->row % v)) return false;
+            if ((uintptr_t)r->p % (v * es) || r->pos % v || r->seq % v) return false;
         return ((uintptr_t)a.s_in | (uintptr_t)a.s_out) % (v * es) == 0;
     };
     if (fits(4)) return 4;

@@ -183,8 +183,7 @@ std::string rotary_name(const RotaryArgs& a, int dtype);
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s);
 // Short causal convolution of each channel (zjai_causal_conv); states [..][taps - 1][channels] of the storage type.
 struct CausalConvArgs {
-    LinRows x, o;
-    int width;
+    LinRows x, o;  // no gaps between rows
     int seqs, length, channels, taps, act;  // act: GateAct
     const float *weight, *bias;             // bias may be null
     const int *lengths, *slots;
