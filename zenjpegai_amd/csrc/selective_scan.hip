@@ -7,10 +7,11 @@
 // and position (the step, its softplus, the gate) is shared out among the channel's lanes and handed round by lane
 // exchanges; b and c, which all channels of a group share, go through LDS as f32. The next tile's loads are in
 // flight meanwhile.
-// Bound by the vector ALUs: five instructions and a 2^x for each position, channel and state.
+// Bound by the vector ALUs: four instructions of 4 cycles and a 2^x of 8 for each position, channel and state of a wave's lanes. 65536
+// positions of 2048 channels x 16 states bf16: outputs 483 us with the ALUs 90 % busy, ends 347 with 98 %.
 // Sequences that leave SIMDs idle are cut into segments: what each leaves behind when it starts from nothing (its end
 // states and the sum of its steps, which is all that its decays depend on), from those the states that each starts from, then
-// the outputs of all.
+// the outputs of all. The ends cost nearly as much again, so whole sequences stay whole where they fill the card.
 
 #include <algorithm>
 #include <type_traits>
@@ -78,7 +79,7 @@ __device__ __forceinline__ void each(F&& f) {
     }
 }
 
-// OUT: the outputs of a segment; else what it leaves behind. Z: whether there is a gate.
+// OUT: the outputs of a segment; else what it leaves behind.
 template <typename T, int NS, int LANES, bool OUT>
 __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPlan p, float* scratch) {
     constexpr int NP = NS * LANES < 4 ? 4 : NS * LANES;  // floats of a row of b or c in LDS
@@ -209,7 +210,8 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
             steps += sum[0];
         }
         // A position's quads of states one after another. The quads of b and c are read from LDS AHEAD quads before
-        // they are used (the barriers keep the compiler from reading them where it needs them, and waiting).
+        // they are used (the barriers keep the compiler from reading them where it needs them, and waiting: outputs of the long
+        // sequence above 552 us, with them 511).
         constexpr int QUADS = NS < 4 ? 1 : NS / 4, AHEAD = 2;
         f32x4 b[AHEAD + 1], w[AHEAD + 1];
         const auto read = [&](auto at_) __attribute__((always_inline)) {
@@ -367,7 +369,8 @@ __global__ void __launch_bounds__(256) k_scan_starts(ScanArgs a, ScanPlan p, int
     }
 }
 
-// One position of each sequence. `lanes` lanes have a channel, four states each.
+// One position of each sequence. `lanes` lanes have a channel, four states each: HBM bound (257 sequences of 2048
+// channels x 16 states: 23 us for 135 MB of states).
 template <typename T, bool V4>
 __global__ void __launch_bounds__(256) k_scan_step(ScanArgs a, int lanes, int blocks) {
     __shared__ int s_next;
