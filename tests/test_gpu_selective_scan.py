@@ -130,6 +130,18 @@ def test_states_updated_in_place_over_many_segments(eng, prec):
 
 
 @pytest.mark.parametrize("prec", PRECS)
+@pytest.mark.parametrize("channels,n", [(300, 16), (515, 8), (70, 64), (257, 1)])
+def test_states_in_place_with_workgroups_of_part_of_the_channels(eng, prec, channels, n):
+    """The lanes of a channel's last workgroup that have no channel leave the first one, whose state has been replaced, alone:
+    the same bits as with states of their own, in sequences whose workgroups do not all run at once."""
+    k = Case(25, prec, 600, 33, channels, n)
+    want = run(eng, k, only=[0, 599])
+    for _ in range(2):
+        got = run(eng, k, in_place=True, only=[])
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("prec", PRECS)
 def test_buffers_off_16_bytes(eng, prec):
     run(eng, Case(15, prec, 2, 45, 64, 16), offset=4 if prec == "f32" else 2)
 

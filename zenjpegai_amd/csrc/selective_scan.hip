@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
     double steps = 0.0;  // its rounding would grow with the positions, and what a segment keeps of its start with it
 
     // A tile's inputs: the lane's share of x, delta and z, and of b and c in quads. Lanes without a channel or a quad of
-    // their own load the first ones: nothing here branches, so that loads and stores stay in flight over the tiles.
+    // their own load the first ones, which nothing uses: no load is in a branch, so that they stay in flight over the tiles.
     struct Tile {
         T x[OWN], delta[OWN], z[OWN];
         SeqVec<T, 4> bc[PER_LANE];
@@ -271,9 +271,11 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
             const unsigned off = channel();
 #pragma unroll
             for (int k = 0; k < OWN; ++k, o += OWNERS * a.o.pos) {
-                // (A lane without a channel of its own has the first one's results, and writes them once more.)
-                if (LANES <= SCAN_TILE && n == SCAN_TILE) *(T*)((char*)o + off) = from_f32<T>(y[k]);
-                else if (on && part < OWNERS && k * OWNERS + own < n) o[c] = from_f32<T>(y[k]);
+                if (LANES <= SCAN_TILE && n == SCAN_TILE) {
+                    if (on) *(T*)((char*)o + off) = from_f32<T>(y[k]);
+                } else if (on && part < OWNERS && k * OWNERS + own < n) {
+                    o[c] = from_f32<T>(y[k]);
+                }
             }
             op += SCAN_TILE * a.o.pos;
         }
