@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
     const int g = id / p.blocks, cg = a.channels / a.groups;
     const int at = (id - g * p.blocks) * (64 * SCAN_WAVES / LANES) + tid / LANES, part = lane & (LANES - 1);
     const bool on = at < cg;
+    const bool idle = __builtin_amdgcn_readfirstlane(at) >= cg;  // a wave without channels: it loads, and waits at the barriers
     const int c = g * cg + (on ? at : 0);
     const int len = seq_length(a.lengths, s, a.length), live = live_segments(p, len);
     if (seg >= live || (!OUT && seg + 1 >= live)) return;
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
         for (int k = 0; k < OWN; ++k) in[k] *= step[k];
         __syncthreads();
         next();
+        if (idle) return;
         if (!OUT) {
             float sum[OWN];
 #pragma unroll
