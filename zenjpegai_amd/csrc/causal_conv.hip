@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256) k_causal_conv_step(CausalConvArgs a, int 
     __shared__ int s_next;
     const int first = blockIdx.x / blocks, cv = (blockIdx.x - first * blocks) * blockDim.x + threadIdx.x;
     SlotChain chain{a.slots, a.num_slots, a.seqs, &s_next};
-    if (!chain.begin(first)) return;
+    if (!chain.enter(first)) return;
     const bool on = cv < vecs;
     const int c = on ? cv * VE : 0;
     const ConvWeights<VE, K> w(a, c, wide);
@@ -153,8 +153,10 @@ __global__ void __launch_bounds__(256) k_causal_conv_step(CausalConvArgs a, int 
     V in[K];
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) in[j] = *(const V*)((const T*)a.s_in + sbase + (long long)j * a.channels);
-    for (int s = first; s != INT_MAX; s = chain.next()) {
-        in[K - 1] = *(const V*)((const T*)a.x.p + (long long)s * a.x.seq + c);
+    in[K - 1] = *(const V*)((const T*)a.x.p + (long long)first * a.x.seq + c);
+    // (All these are in flight while the sequences of the slot are looked for.)
+    if (!chain.alone_or_first(first)) return;
+    for (int s = first; s != INT_MAX;) {
         V y;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
@@ -166,6 +168,8 @@ __global__ void __launch_bounds__(256) k_causal_conv_step(CausalConvArgs a, int 
         if (on) *(V*)((T*)a.o.p + (long long)s * a.o.seq + c) = y;
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) in[j] = in[j + 1];
+        s = chain.next();
+        if (s != INT_MAX) in[K - 1] = *(const V*)((const T*)a.x.p + (long long)s * a.x.seq + c);
     }
     if (!on) return;
 #pragma unroll

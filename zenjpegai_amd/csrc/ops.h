@@ -211,7 +211,7 @@ constexpr int SCAN_MAX_STATES = 256, SCAN_MAX_BLOCKS = 1 << 20;  // workgroups: 
 // states of a channel, `lanes` lanes have one channel.
 struct ScanPlan {
     int ns = 16, lanes = 1;
-    int blocks = 0;  // workgroups of a group's channels
+    int waves = 4, blocks = 0;  // waves of a workgroup, workgroups of a group's channels
     int segments = 1, seg_len = 0;
 };
 ScanPlan scan_plan(const ScanArgs& a, size_t scratch_bytes);

@@ -4,7 +4,7 @@
 // HBM bound: every channel passes once. A workgroup takes a tile of positions: its lanes first form the tile's sines and
 // cosines, one for each pair and position however many heads there are, in LDS, then walk over the channels of the
 // tile's positions, which lie behind one another, 16 bytes a lane (65536 positions of 32 heads of 128 channels, 64 of them turned, bf16:
-// 222 us, 4.8 TB/s, a copy 213; the 64 x 64 map of 10 heads of 32 f32: 4.5 us, a launch).
+// 216 us, 5.0 TB/s, a copy 213; the 64 x 64 map of 10 heads of 32 f32: 4.5 us, a launch).
 
 #include <algorithm>
 
@@ -70,39 +70,43 @@ __global__ void __launch_bounds__(256) k_rotary(RotaryArgs a, RotaryPlan p) {
             s_turn[e] = rotary_turn(at, a.freq[i], a.magnitude);
         }
         __syncthreads();
-        for (int e = tid; e < n * per_pos; e += 256) {
-            const int t = e / per_pos, in_pos = e - t * per_pos, h = in_pos / per_head, k = in_pos - h * per_head;
-            const T* x = (const T*)a.x.p + seq_at(a.x, a.width, s, t0 + t) + (long long)h * a.dim;
-            T* o = (T*)a.o.p + seq_at(a.o, a.width, s, t0 + t) + (long long)h * a.dim;
-            if (k >= p.turn) {
-                const int c = a.turned + (k - p.turn) * VE;
-                *(V*)(o + c) = *(const V*)(x + c);
-                continue;
-            }
-            if constexpr (HALVES || VE == 1) {  // two accesses, the pairs across them
-                const float2* cs = s_turn + t * pairs + k * VE;
-                const int c0 = HALVES ? k * VE : 2 * k, c1 = HALVES ? pairs + k * VE : 2 * k + 1;
-                const V va = *(const V*)(x + c0), vb = *(const V*)(x + c1);
-                V oa, ob;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const float u = to_f32(va.e[i]), v = to_f32(vb.e[i]), sn = a.inverse ? -cs[i].y : cs[i].y;
-                    oa.e[i] = from_f32<T>(fmaf(u, cs[i].x, -(v * sn)));
-                    ob.e[i] = from_f32<T>(fmaf(u, sn, v * cs[i].x));
+        // A lane keeps its channels over the tile's positions: `beside` of these lie side by side in the workgroup.
+        const int beside = max(1, 256 / per_pos), t_first = beside > 1 ? tid / per_pos : 0;
+        for (int in_pos = t_first < beside ? tid - t_first * per_pos : per_pos; in_pos < per_pos; in_pos += 256) {
+            const int h = in_pos / per_head, k = in_pos - h * per_head;
+            for (int t = t_first; t < n; t += beside) {
+                const T* x = (const T*)a.x.p + seq_at(a.x, a.width, s, t0 + t) + (long long)h * a.dim;
+                T* o = (T*)a.o.p + seq_at(a.o, a.width, s, t0 + t) + (long long)h * a.dim;
+                if (k >= p.turn) {
+                    const int c = a.turned + (k - p.turn) * VE;
+                    *(V*)(o + c) = *(const V*)(x + c);
+                    continue;
                 }
-                *(V*)(o + c0) = oa;
-                *(V*)(o + c1) = ob;
-            } else {  // one, the pairs within it
-                const float2* cs = s_turn + t * pairs + k * (VE / 2);
-                const V va = *(const V*)(x + k * VE);
-                V oa;
+                if constexpr (HALVES || VE == 1) {  // two accesses, the pairs across them
+                    const float2* cs = s_turn + t * pairs + k * VE;
+                    const int c0 = HALVES ? k * VE : 2 * k, c1 = HALVES ? pairs + k * VE : 2 * k + 1;
+                    const V va = *(const V*)(x + c0), vb = *(const V*)(x + c1);
+                    V oa, ob;
 #pragma unroll
-                for (int i = 0; i < VE / 2; ++i) {
-                    const float u = to_f32(va.e[2 * i]), v = to_f32(va.e[2 * i + 1]), sn = a.inverse ? -cs[i].y : cs[i].y;
-                    oa.e[2 * i] = from_f32<T>(fmaf(u, cs[i].x, -(v * sn)));
-                    oa.e[2 * i + 1] = from_f32<T>(fmaf(u, sn, v * cs[i].x));
+                    for (int i = 0; i < VE; ++i) {
+                        const float u = to_f32(va.e[i]), v = to_f32(vb.e[i]), sn = a.inverse ? -cs[i].y : cs[i].y;
+                        oa.e[i] = from_f32<T>(fmaf(u, cs[i].x, -(v * sn)));
+                        ob.e[i] = from_f32<T>(fmaf(u, sn, v * cs[i].x));
+                    }
+                    *(V*)(o + c0) = oa;
+                    *(V*)(o + c1) = ob;
+                } else {  // one, the pairs within it
+                    const float2* cs = s_turn + t * pairs + k * (VE / 2);
+                    const V va = *(const V*)(x + k * VE);
+                    V oa;
+#pragma unroll
+                    for (int i = 0; i < VE / 2; ++i) {
+                        const float u = to_f32(va.e[2 * i]), v = to_f32(va.e[2 * i + 1]), sn = a.inverse ? -cs[i].y : cs[i].y;
+                        oa.e[2 * i] = from_f32<T>(fmaf(u, cs[i].x, -(v * sn)));
+                        oa.e[2 * i + 1] = from_f32<T>(fmaf(u, sn, v * cs[i].x));
+                    }
+                    *(V*)(o + k * VE) = oa;
                 }
-                *(V*)(o + k * VE) = oa;
             }
         }
     }
@@ -126,8 +130,9 @@ RotaryPlan rotary_plan(const RotaryArgs& a, int ve) {
     p.turn = a.halves ? a.turned / 2 / ve : a.turned / std::max(ve, 2);
     p.copy = a.x.p == a.o.p ? 0 : (a.dim - a.turned) / ve;
     const long long per_pos = (long long)(p.turn + p.copy) * a.heads;
-    // Four accesses a lane, unless that leaves CUs idle; 16 KB of turns at most.
-    const long long want = std::max<long long>(1, 1024 / per_pos), spread = std::max<long long>(1, (long long)a.seqs * a.length / 1024);
+    // Eight accesses a lane (65536 positions of 32 heads of 128 bf16: four 221 us, eight 216, sixteen 230; 20000 of 8 of 100 in
+    // single channels f16: 56, 40, 39), unless that leaves CUs idle; 16 KB of turns at most.
+    const long long want = std::max<long long>(1, 2048 / per_pos), spread = std::max<long long>(1, (long long)a.seqs * a.length / 1024);
     p.tp = (int)std::min({want, spread, (long long)(2048 / (a.turned / 2)), (long long)a.length});
     p.tiles = (a.length + p.tp - 1) / p.tp;
     return p;

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
     const int seg = id / per_seg;
     id -= seg * per_seg;
     const int g = id / p.blocks, cg = a.channels / a.groups;
-    const int at = (id - g * p.blocks) * (64 * SCAN_WAVES / LANES) + tid / LANES, part = lane & (LANES - 1);
+    const int at = (id - g * p.blocks) * ((int)blockDim.x / LANES) + tid / LANES, part = lane & (LANES - 1);
     const bool on = at < cg;
     const bool idle = __builtin_amdgcn_readfirstlane(at) >= cg;  // a wave without channels: it loads, and waits at the barriers
     const int c = g * cg + (on ? at : 0);
@@ -373,72 +373,88 @@ __global__ void __launch_bounds__(256) k_scan_starts(ScanArgs a, ScanPlan p, int
     }
 }
 
-// One position of each sequence. `lanes` lanes have a channel, four states each: HBM bound (257 sequences of 2048
-// channels x 16 states: 23 us for 135 MB of states).
-template <typename T, bool V4>
+// One position of each sequence. `lanes` lanes have a channel, four states each. WIDE: states, rates, b and c in aligned
+// quads. A workgroup for every 256 / lanes channels: four times as many states a lane gain nothing (25 us instead of 23).
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) k_scan_step(ScanArgs a, int lanes, int blocks) {
+    typedef SeqVec<T, 4> Quad;
     __shared__ int s_next;
     const int first = blockIdx.x / blocks, at = (blockIdx.x - first * blocks) * (256 / lanes) + threadIdx.x / lanes;
     const int n0 = (threadIdx.x & (lanes - 1)) * 4;
-    const bool on = at < a.channels && n0 < a.n;
+    const bool on = at < a.channels && n0 < a.n, gate = a.z.p != nullptr;
     const int c = min(at, a.channels - 1), n_first = n0 < a.n ? n0 : 0;
     const long long g = c / (a.channels / a.groups) * a.n;
     SlotChain chain{a.slots, a.num_slots, a.seqs, &s_next};
-    if (!chain.begin(first)) return;
+    if (!chain.enter(first)) return;
     const long long sbase = ((long long)chain.slot * a.channels + c) * a.n;
-    f32x4 h, rate;
-    if (V4) {
-        h = *(const f32x4*)(a.s_in + sbase + n_first);
-        rate = *(const f32x4*)(a.a + (long long)c * a.n + n_first);
-    } else {
+    // Quads, or their values one by one: of states past the last one, the last one's (not used).
+    const auto quad = [&](const float* p) __attribute__((always_inline)) {
+        if (WIDE) return *(const f32x4*)(p + n_first);
+        f32x4 v;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int n = min(n_first + k, a.n - 1);
-            h[k] = a.s_in[sbase + n];
-            rate[k] = a.a[(long long)c * a.n + n];
-        }
-    }
+        for (int k = 0; k < 4; ++k) v[k] = p[min(n_first + k, a.n - 1)];
+        return v;
+    };
+    const auto quad_t = [&](const T* p) __attribute__((always_inline)) {
+        if (WIDE) return *(const Quad*)(p + n_first);
+        Quad v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v.e[k] = p[min(n_first + k, a.n - 1)];
+        return v;
+    };
+    T dr, xr, zr;
+    Quad b, w;
+    const auto fetch = [&](long long s) __attribute__((always_inline)) {
+        dr = ((const T*)a.delta.p)[s * a.delta.seq + c];
+        xr = ((const T*)a.x.p)[s * a.x.seq + c];
+        zr = gate ? ((const T*)a.z.p)[s * a.z.seq + c] : xr;
+        b = quad_t((const T*)a.b.p + s * a.b.seq + g);
+        w = quad_t((const T*)a.c.p + s * a.c.seq + g);
+    };
+    f32x4 h = quad(a.s_in + sbase);
+    fetch(first);
+    const f32x4 rate = quad(a.a + (long long)c * a.n) * LOG2E;
     const float bias = a.bias ? a.bias[c] : 0.0f, d = a.d ? a.d[c] : 0.0f;
-    for (int s = first; s != INT_MAX; s = chain.next()) {
-        float step = to_f32(((const T*)a.delta.p)[(long long)s * a.delta.seq + c]) + bias;
-        const float x = to_f32(((const T*)a.x.p)[(long long)s * a.x.seq + c]);
-        const float z = a.z.p ? to_f32(((const T*)a.z.p)[(long long)s * a.z.seq + c]) : 0.0f;
-        float b[4], w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int n = min(n_first + k, a.n - 1);
-            b[k] = to_f32(((const T*)a.b.p)[(long long)s * a.b.seq + g + n]);
-            w[k] = to_f32(((const T*)a.c.p)[(long long)s * a.c.seq + g + n]);
-        }
+    // (All these are in flight while the sequences of the slot are looked for.)
+    if (!chain.alone_or_first(first)) return;
+    for (int s = first; s != INT_MAX;) {
+        float step = to_f32(dr) + bias;
+        const float x = to_f32(xr), z = to_f32(zr);
         if (a.softplus) step = softplus(step);
         const float u = step * x;
         float y = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            h[k] = fmaf(__builtin_amdgcn_exp2f(step * (rate[k] * LOG2E)), h[k], u * b[k]);
-            if (n0 + k < a.n) y = fmaf(w[k], h[k], y);
+            h[k] = fmaf(__builtin_amdgcn_exp2f(step * rate[k]), h[k], u * to_f32(b.e[k]));
+            if (n0 + k < a.n) y = fmaf(to_f32(w.e[k]), h[k], y);
         }
         y = lane_sum(y, lanes);
         if (a.d) y = fmaf(d, x, y);
-        if (a.z.p) y *= z * fast_sigmoid(z);
+        if (gate) y *= z * fast_sigmoid(z);
         if (on && n0 == 0) ((T*)a.o.p)[(long long)s * a.o.seq + c] = from_f32<T>(y);
+        s = chain.next();
+        if (s != INT_MAX) fetch(s);
     }
     if (!on) return;
-    if (V4) *(f32x4*)(a.s_out + sbase + n0) = h;
+    if (WIDE) *(f32x4*)(a.s_out + sbase + n0) = h;
     else
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (n0 + k < a.n) a.s_out[sbase + n0 + k] = h[k];
 }
 
-bool step_wide(const ScanArgs& a) { return a.n % 4 == 0 && (((uintptr_t)a.s_in | (uintptr_t)a.s_out | (uintptr_t)a.a) & 15) == 0; }
+bool step_wide(const ScanArgs& a, int es) {
+    for (const LinRows* r : {&a.b, &a.c})
+        if ((uintptr_t)r->p % (4 * es) || r->seq % 4) return false;
+    return a.n % 4 == 0 && (((uintptr_t)a.s_in | (uintptr_t)a.s_out | (uintptr_t)a.a) & 15) == 0;
+}
 
 template <typename T>
 hipError_t scan_step(const ScanArgs& a, hipStream_t s) {
     int lanes = 1;
     while (lanes * 4 < a.n) lanes *= 2;
     const int blocks = (a.channels + 256 / lanes - 1) / (256 / lanes);
-    if (step_wide(a)) k_scan_step<T, true><<<(unsigned)(a.seqs * blocks), 256, 0, s>>>(a, lanes, blocks);
+    if (step_wide(a, sizeof(T))) k_scan_step<T, true><<<(unsigned)(a.seqs * blocks), 256, 0, s>>>(a, lanes, blocks);
     else k_scan_step<T, false><<<(unsigned)(a.seqs * blocks), 256, 0, s>>>(a, lanes, blocks);
     return hipGetLastError();
 }
@@ -446,12 +462,15 @@ hipError_t scan_step(const ScanArgs& a, hipStream_t s) {
 template <typename T, bool OUT>
 hipError_t scan(const ScanArgs& a, const ScanPlan& p, float* scratch, hipStream_t s) {
     const unsigned grid = (unsigned)(a.seqs * (OUT ? p.segments : p.segments - 1) * a.groups * p.blocks);
-    const dim3 block(64 * SCAN_WAVES);
+    const dim3 block(64 * p.waves);
     switch (p.ns * 100 + p.lanes) {
         case 101: k_scan<T, 1, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
         case 401: k_scan<T, 4, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
         case 404: k_scan<T, 4, 4, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
         case 801: k_scan<T, 8, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1201: k_scan<T, 12, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1202: k_scan<T, 12, 2, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
+        case 1204: k_scan<T, 12, 4, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
         case 1601: k_scan<T, 16, 1, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
         case 1602: k_scan<T, 16, 2, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
         case 1604: k_scan<T, 16, 4, OUT><<<grid, block, 0, s>>>(a, p, scratch); break;
@@ -476,14 +495,23 @@ ScanPlan scan_plan(const ScanArgs& a, size_t scratch_bytes) {
     p.ns = a.n == 1 ? 1 : a.n <= 4 ? 4 : a.n <= 8 ? 8 : 16;
     p.lanes = 1;
     while (p.ns * p.lanes < a.n) p.lanes *= 2;
+    if (p.ns == 16 && p.lanes <= 4 && 12 * p.lanes >= a.n) p.ns = 12;
     const auto waves = [&]() { return std::max(1.0, (double)a.seqs * a.groups * ((cg + 64 / p.lanes - 1) / (64 / p.lanes))); };
     // Nine to sixteen states in one lane, or, where that leaves SIMDs idle even with segments of 64 positions, in four
     // (64 x 64 positions of 320 channels x 16 states f32 36 -> 27 us, 24 of 64 11.1 -> 5.4).
-    if (p.ns == 16 && p.lanes == 1 && waves() * (a.length / 64.0) < 1024.0) {
+    if (p.ns >= 12 && p.lanes == 1 && waves() * (a.length / 64.0) < 1024.0) {
         p.ns = 4;
         p.lanes = 4;
     }
-    p.blocks = (cg + 64 * SCAN_WAVES / p.lanes - 1) / (64 * SCAN_WAVES / p.lanes);
+    // Waves of a workgroup: few without a channel, and few workgroups, each of which loads b and c (half a wave's worth): 64 sequences
+    // of 1000 positions of 100 channels x 16 f32 four waves 122 us, two 95. (More than sixteen states' b and c take four waves.)
+    const int needed = (int)(((long long)cg * p.lanes + 63) / 64);
+    const auto cost = [&](int w) { return (needed + w - 1) / w * (w + 0.5); };
+    p.waves = SCAN_WAVES;
+    if (p.ns * p.lanes <= 16)
+        for (int w = SCAN_WAVES - 1; w > 0; --w)
+            if (cost(w) < cost(p.waves)) p.waves = w;
+    p.blocks = (needed + p.waves - 1) / p.waves;
     // Segments for four waves a SIMD (65536 positions of 2048 channels x 16 states bf16: two 864 us, four 832, eight 879) or,
     // where lengths may differ, which only the device knows, for eight (12 sequences of 0-3001, 1024 channels x 64 f16: two
     // 939 us, four 640, eight 518), but none of less than 32 positions (the 64 x 64 map: 64 positions 31 us, 32 27, 16 29).
@@ -515,7 +543,7 @@ hipError_t launch_scan_outputs(const ScanArgs& a, const ScanPlan& p, int dtype, 
 }
 
 std::string scan_step_name(const ScanArgs& a, int dtype) {
-    return std::string("k_scan_step<") + type_name(dtype) + (step_wide(a) ? ", true>" : ", false>");
+    return std::string("k_scan_step<") + type_name(dtype) + (step_wide(a, dtype == DT_F32 ? 4 : 2) ? ", true>" : ", false>");
 }
 hipError_t launch_scan_step(const ScanArgs& a, int dtype, hipStream_t s) {
     if (dtype == DT_F32) return scan_step<float>(a, s);

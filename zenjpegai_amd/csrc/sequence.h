@@ -33,21 +33,21 @@ __device__ __forceinline__ float gate_act(float v, int act) {
 }
 
 // The sequences of one slot, for a workgroup that starts at sequence `first`: the first of them takes them all, in
-// order. begin: whether this workgroup has any (all lanes get the same answer); next: the sequence after `cur`, or INT_MAX.
+// order. enter: its slot, and whether there is one; alone_or_first: whether this workgroup has them (all lanes get the same
+// answer); next: the sequence after the current one, or INT_MAX.
 struct SlotChain {
     const int* slots;
     int num_slots, seqs;
     int* s_next;  // shared
-    int slot, after;
-    bool alone;
+    int slot = 0, after = INT_MAX;
+    bool alone = false;
 
-    __device__ __forceinline__ bool begin(int first) {
-        slot = first;
-        after = INT_MAX;
+    __device__ __forceinline__ bool enter(int first) {
+        slot = slots ? slots[first] : first;
         alone = !slots || seqs == 1;
-        if (!slots) return true;
-        slot = slots[first];
-        if ((unsigned)slot >= (unsigned)num_slots) return false;
+        return !slots || (unsigned)slot < (unsigned)num_slots;
+    }
+    __device__ __forceinline__ bool alone_or_first(int first) {
         if (alone) return true;
         if (threadIdx.x == 0) *s_next = INT_MAX;
         __syncthreads();
