@@ -371,12 +371,19 @@ def _address(a):
     return a.data_ptr() if hasattr(a, "data_ptr") else a
 
 
+def _holding(desc, *buffers):
+    """A descriptor, which has addresses alone, together with the objects that they are of."""
+    desc.buffers = [b for b in buffers if hasattr(b, "data_ptr")]
+    return desc
+
+
 def linear_attention_desc(precision: str, qkv, out, *, heads: int, key_dim: int, value_dim: int,
                           sequences: int, length: int, decay, scale: float = 1.0, lengths=None,
                           slots=None, num_slots: int = 0, state_in=None, state_out=None,
                           **strides) -> _lib.ZjaiLinearAttentionDesc:
     """A descriptor for ``linear_attention_noalloc`` / ``linear_attention_step`` over device buffers
-    (addresses, or objects with ``data_ptr()``, which the caller keeps alive). ``qkv`` is one
+    (addresses, or objects with ``data_ptr()``, which the descriptor keeps alive; the caller keeps
+    the descriptor until the device has done its calls). ``qkv`` is one
     buffer of packed channels, dense over positions and sequences, or a tuple ``(q, k, v)`` of
     dense buffers; ``strides`` (``q_position=...``, ``out_sequence=...``) replaces single ones."""
     kc, vc = heads * key_dim, heads * value_dim
@@ -392,11 +399,12 @@ def linear_attention_desc(precision: str, qkv, out, *, heads: int, key_dim: int,
     st = {n + "_position": p for n, p in pos.items()}
     st.update({n + "_sequence": p * length for n, p in pos.items()})
     st.update(strides)
-    return _lib.ZjaiLinearAttentionDesc(
+    desc = _lib.ZjaiLinearAttentionDesc(
         precision=_lib.PRECISIONS[precision], heads=heads, key_dim=key_dim, value_dim=value_dim,
         sequences=sequences, length=length, q=q, k=k, v=v, out=_address(out), decay=_address(decay), scale=scale,
         num_slots=num_slots if slots is not None else 0, lengths=_address(lengths), slots=_address(slots),
         state_in=_address(state_in), state_out=_address(state_out), **st)
+    return _holding(desc, *(qkv if isinstance(qkv, (tuple, list)) else [qkv]), out, decay, lengths, slots, state_in, state_out)
 
 
 def linear_attention_noalloc(eng: Engine, desc: _lib.ZjaiLinearAttentionDesc) -> None:
@@ -445,15 +453,16 @@ def _strides(length: int, given: dict, **positions) -> dict:
 def rotary_desc(precision: str, x, out, *, heads: int, head_dim: int, sequences: int, length: int, frequencies,
                 rotary_dim: int | None = None, layout: str = "interleaved", width: int = 0, magnitude: float = 1.0,
                 inverse: bool = False, positions=None, starts=None, lengths=None, **strides) -> _lib.ZjaiRotaryDesc:
-    """A descriptor for ``rotary_noalloc`` over device buffers (addresses, or objects with ``data_ptr()``, which the caller
-    keeps alive; ``frequencies``: float64), dense unless ``strides`` (``x_position=...``) says otherwise."""
+    """A descriptor for ``rotary_noalloc`` over device buffers (as for ``linear_attention_desc``; ``frequencies``: float64),
+    dense unless ``strides`` (``x_position=...``) says otherwise."""
     c = heads * head_dim
-    return _lib.ZjaiRotaryDesc(
+    desc = _lib.ZjaiRotaryDesc(
         precision=_lib.PRECISIONS[precision], heads=heads, head_dim=head_dim,
         rotary_dim=head_dim if rotary_dim is None else rotary_dim, layout=_lib.ROTARY_LAYOUTS[layout], inverse=int(inverse),
         width=width, sequences=sequences, length=length, magnitude=magnitude, x=_address(x), out=_address(out),
         frequencies=_address(frequencies), positions=_address(positions), starts=_address(starts),
         lengths=_address(lengths), **_strides(length, strides, x=c, out=c))
+    return _holding(desc, x, out, frequencies, positions, starts, lengths)
 
 
 def rotary_noalloc(eng: Engine, desc: _lib.ZjaiRotaryDesc) -> None:
@@ -477,12 +486,13 @@ def causal_conv(eng: Engine, x: BTensor, weight, bias=None, *, act: str = "linea
 def causal_conv_desc(precision: str, x, out, *, channels: int, taps: int, sequences: int, length: int, weight, bias=None,
                      act: str = "linear", lengths=None, slots=None, num_slots: int = 0, state_in=None, state_out=None,
                      **strides) -> _lib.ZjaiCausalConvDesc:
-    """A descriptor for ``causal_conv_noalloc`` / ``causal_conv_step`` over device buffers (as for ``rotary_desc``)."""
-    return _lib.ZjaiCausalConvDesc(
+    """A descriptor for ``causal_conv_noalloc`` / ``causal_conv_step`` over device buffers (as for ``linear_attention_desc``)."""
+    desc = _lib.ZjaiCausalConvDesc(
         precision=_lib.PRECISIONS[precision], channels=channels, taps=taps, act=_lib.GATES[act], sequences=sequences,
         length=length, x=_address(x), out=_address(out), weight=_address(weight), bias=_address(bias),
         lengths=_address(lengths), slots=_address(slots), num_slots=num_slots if slots is not None else 0, reserved=0,
         state_in=_address(state_in), state_out=_address(state_out), **_strides(length, strides, x=channels, out=channels))
+    return _holding(desc, x, out, weight, bias, lengths, slots, state_in, state_out)
 
 
 def causal_conv_noalloc(eng: Engine, desc: _lib.ZjaiCausalConvDesc) -> None:
@@ -511,15 +521,16 @@ def selective_scan(eng: Engine, x: BTensor, delta: BTensor, bc: BTensor, a, z: B
 def selective_scan_desc(precision: str, x, delta, b, c, out, *, channels: int, state_dim: int, sequences: int, length: int, a,
                         z=None, groups: int = 1, d=None, delta_bias=None, softplus: bool = True, lengths=None, slots=None,
                         num_slots: int = 0, state_in=None, state_out=None, **strides) -> _lib.ZjaiSelectiveScanDesc:
-    """A descriptor for ``selective_scan_noalloc`` / ``selective_scan_step`` over device buffers (as for ``rotary_desc``)."""
+    """A descriptor for ``selective_scan_noalloc`` / ``selective_scan_step`` over device buffers (as for ``linear_attention_desc``)."""
     bc = groups * state_dim
-    return _lib.ZjaiSelectiveScanDesc(
+    desc = _lib.ZjaiSelectiveScanDesc(
         precision=_lib.PRECISIONS[precision], channels=channels, groups=groups, state_dim=state_dim, sequences=sequences,
         length=length, softplus=int(softplus), num_slots=num_slots if slots is not None else 0, x=_address(x),
         delta=_address(delta), b=_address(b), c=_address(c), z=_address(z), out=_address(out), a=_address(a), d=_address(d),
         delta_bias=_address(delta_bias), lengths=_address(lengths), slots=_address(slots), state_in=_address(state_in),
         state_out=_address(state_out),
         **_strides(length, strides, x=channels, delta=channels, b=bc, c=bc, z=channels, out=channels))
+    return _holding(desc, x, delta, b, c, z, out, a, d, delta_bias, lengths, slots, state_in, state_out)
 
 
 def selective_scan_noalloc(eng: Engine, desc: _lib.ZjaiSelectiveScanDesc) -> None:
@@ -555,17 +566,17 @@ def norm_gate_residual_desc(precision: str, x, y, gate, x_out, h, *, positions: 
                             post_eps: float = 1e-5, post_weight=None, post_bias=None, residual_scale=None,
                             pre_norm: str = "none", pre_eps: float = 1e-5, pre_weight=None, pre_bias=None,
                             **strides) -> _lib.ZjaiNormGateResidualDesc:
-    """A descriptor for ``norm_gate_residual_noalloc`` over device buffers (addresses, or objects
-    with ``data_ptr()``, which the caller keeps alive), dense unless ``strides`` (``x_stride=...``)
-    says otherwise."""
+    """A descriptor for ``norm_gate_residual_noalloc`` over device buffers (as for ``linear_attention_desc``),
+    dense unless ``strides`` (``x_stride=...``) says otherwise."""
     st = {n + "_stride": channels for n in ("x", "y", "gate", "x_out", "h")}
     st.update(strides)
-    return _lib.ZjaiNormGateResidualDesc(
+    desc = _lib.ZjaiNormGateResidualDesc(
         precision=_lib.PRECISIONS[precision], channels=channels, positions=positions, x=_address(x), y=_address(y),
         gate=_address(gate), x_out=_address(x_out), h=_address(h), gate_act=_lib.GATES[gate_act],
         post_norm=_lib.NORMS[post_norm], post_groups=post_groups, pre_norm=_lib.NORMS[pre_norm],
         post_eps=post_eps, pre_eps=pre_eps, post_weight=_address(post_weight), post_bias=_address(post_bias),
         residual_scale=_address(residual_scale), pre_weight=_address(pre_weight), pre_bias=_address(pre_bias), **st)
+    return _holding(desc, x, y, gate, x_out, h, post_weight, post_bias, residual_scale, pre_weight, pre_bias)
 
 
 def norm_gate_residual_noalloc(eng: Engine, desc: _lib.ZjaiNormGateResidualDesc) -> None:
