@@ -444,7 +444,10 @@ ZJAI_API int32_t zjai_causal_conv_step(zjai_ctx* ctx, const zjai_causal_conv_des
  * state_in. Like zjai_linear_attention it runs over a whole map of known latents at once or position by position
  * (zjai_selective_scan_step), with the same result up to rounding. Sums, products and states are f32 whatever
  * the precision, and an output is rounded once; the decay of a position is rounded to f32 like any factor, so
- * that a memory of 2^k positions is kept to 2^(k - 23) of itself at worst. A non-finite x, delta or z of a
+ * that a memory of 2^k positions is kept to 2^(k - 23) of itself at worst. States may grow (a > 0, or negative
+ * steps without softplus) as long as they stay within f32's range, and exp(s_t a) of each position with them; long
+ * sequences are worked in stretches, so what a stretch takes on and what it adds should not cancel beyond
+ * f32's accuracy. A non-finite x, delta or z of a
  * channel reaches the outputs of this channel at its own position (z) and at later ones only, b or c those of its
  * group's channels (infinities may arrive there as NaN), a state_in those of its channel. No counterpart in the
  * reference.

@@ -332,11 +332,22 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
     }
 }
 
+// The decay 2^x of many positions together, as m 2^n: where states grow it may lie past f32's range although what comes of it
+// does not, and a zero stays zero. (x: past the range of an exponent for sure, or no number, which the ends show.)
+__device__ __forceinline__ void split_power(float x, float& m, int& n) {
+    x = __builtin_amdgcn_fmed3f(x, -1024.0f, 1024.0f);
+    const float whole = floorf(x);
+    m = __builtin_amdgcn_exp2f(x - whole);
+    n = (int)whole;
+}
+__device__ __forceinline__ float pass_on(float start, float m, int n, float end) { return fmaf(__builtin_amdgcn_ldexpf(start, n), m, end); }
+
 // Each segment's end states become the states that it starts from. `parts` threads of a workgroup have a state, each
 // SCAN_RUN consecutive segments of it, whose loads are issued together; what a run makes of its start (a decay and an
 // end) goes to the later ones through LDS.
 __global__ void __launch_bounds__(256) k_scan_starts(ScanArgs a, ScanPlan p, int parts, float* scratch) {
-    __shared__ float s_keep[256], s_end[256];
+    __shared__ float s_power[256], s_end[256];
+    __shared__ int s_whole[256];
     const int items = 256 / parts, part = threadIdx.x / items, first = part * SCAN_RUN;
     const long long size = (long long)a.n * a.channels, i = (long long)blockIdx.x * items + threadIdx.x % items;
     const bool on = i < a.seqs * size;
@@ -346,30 +357,32 @@ __global__ void __launch_bounds__(256) k_scan_starts(ScanArgs a, ScanPlan p, int
     const int left = live_segments(p, seq_length(a.lengths, s, a.length)) - first;  // segments of the run, or none
     float* state = scratch + scan_slot(a, p, s, 0) + in_slot;
     const float* steps = scratch + step_slot(a, p, s, 0) + c;
-    float end[SCAN_RUN], keep[SCAN_RUN];
+    float end[SCAN_RUN], power[SCAN_RUN];
 #pragma unroll
     for (int k = 0; k < SCAN_RUN; ++k) {  // the last segment leaves nothing behind (the first one's values in its place, not used)
         const long long from = k + 1 < left ? first + k : 0;
         end[k] = state[from * size];
-        keep[k] = steps[from * a.channels];
+        power[k] = steps[from * a.channels];
     }
     const float rate = a.a[(long long)c * a.n + n] * LOG2E;
-    float h = a.s_in ? a.s_in[((long long)s * a.channels + c) * a.n + n] : 0.0f, all = 1.0f, e = 0.0f;
+    float h = a.s_in ? a.s_in[((long long)s * a.channels + c) * a.n + n] : 0.0f, all = 0.0f, e = 0.0f;
+    int whole[SCAN_RUN];
 #pragma unroll
     for (int k = 0; k < SCAN_RUN; ++k) {
-        keep[k] = __builtin_amdgcn_exp2f(keep[k] * rate);
-        e = fmaf(keep[k], e, end[k]);
-        all *= keep[k];
+        const float x = power[k] * rate;
+        all += x;
+        split_power(x, power[k], whole[k]);
+        e = pass_on(e, power[k], whole[k], end[k]);
     }
-    s_keep[threadIdx.x] = all;
+    split_power(all, s_power[threadIdx.x], s_whole[threadIdx.x]);
     s_end[threadIdx.x] = e;
     __syncthreads();  // (and every state has been read before one is written)
-    for (int q = 0; q < part; ++q) h = fmaf(s_keep[threadIdx.x + (q - part) * items], h, s_end[threadIdx.x + (q - part) * items]);
+    for (int q = threadIdx.x - part * items; q < (int)threadIdx.x; q += items) h = pass_on(h, s_power[q], s_whole[q], s_end[q]);
 #pragma unroll
     for (int k = 0; k < SCAN_RUN; ++k) {
         if (!on || k >= left) break;
         state[(first + k) * size] = h;
-        h = fmaf(keep[k], h, end[k]);
+        h = pass_on(h, power[k], whole[k], end[k]);
     }
 }
 
