@@ -4,7 +4,7 @@
 // HBM bound: every channel passes once. A workgroup takes a tile of positions: its lanes first form the tile's sines and
 // cosines, one for each pair and position however many heads there are, in LDS, then walk over the channels of the
 // tile's positions, which lie behind one another, 16 bytes a lane (65536 positions of 32 heads of 128 channels, 64 of them turned, bf16:
-// 216 us, 5.0 TB/s, a copy 213; the 64 x 64 map of 10 heads of 32 f32: 4.5 us, a launch).
+// 215 us, 5.0 TB/s, a copy 213; the 64 x 64 map of 10 heads of 32 f32: 4.5 us, a launch).
 
 #include <algorithm>
 
@@ -125,14 +125,17 @@ int rotary_vector(const RotaryArgs& a, int es) {
     return ve;
 }
 
-RotaryPlan rotary_plan(const RotaryArgs& a, int ve) {
+RotaryPlan rotary_plan(const RotaryArgs& a, int ve, int es) {
     RotaryPlan p{};
     p.turn = a.halves ? a.turned / 2 / ve : a.turned / std::max(ve, 2);
     p.copy = a.x.p == a.o.p ? 0 : (a.dim - a.turned) / ve;
     const long long per_pos = (long long)(p.turn + p.copy) * a.heads;
-    // Eight accesses a lane (65536 positions of 32 heads of 128 bf16: four 221 us, eight 216, sixteen 230; 20000 of 8 of 100 in
-    // single channels f16: 56, 40, 39), unless that leaves CUs idle; 16 KB of turns at most.
-    const long long want = std::max<long long>(1, 2048 / per_pos), spread = std::max<long long>(1, (long long)a.seqs * a.length / 1024);
+    // Accesses a lane: five of 16 bytes, eight of fewer. 512 MB into as many, us with four, five, eight: heads of 128 (32, bf16, from
+    // packed channels) 220, 215, 215, of 160 (13, f16) 199, 204, 217, both 16 bytes; 10 heads of 100 in 8 bytes (f16) 258, 244, 237, 8 in
+    // 4 bytes 297, 304, 277. Fewer where that leaves CUs idle; 16 KB of turns at most. A count that leaves lanes idle costs
+    // little, as HBM is what bounds them (heads of 80 f16: 16, 160 accesses a position, 200 us; 13, 130 of them, 222).
+    const long long lane = ve * es == 16 ? 5 : 8;
+    const long long want = std::max<long long>(1, 256 * lane / per_pos), spread = std::max<long long>(1, (long long)a.seqs * a.length / 1024);
     p.tp = (int)std::min({want, spread, (long long)(2048 / (a.turned / 2)), (long long)a.length});
     p.tiles = (a.length + p.tp - 1) / p.tp;
     return p;
@@ -140,7 +143,7 @@ RotaryPlan rotary_plan(const RotaryArgs& a, int ve) {
 
 template <typename T, int VE>
 void rotary_of(const RotaryArgs& a, hipStream_t s) {
-    const RotaryPlan p = rotary_plan(a, VE);
+    const RotaryPlan p = rotary_plan(a, VE, sizeof(T));
     const unsigned grid = (unsigned)std::min<long long>((long long)a.seqs * p.tiles, 1 << 16);
     const size_t lds = sizeof(float2) * p.tp * (a.turned / 2);
     if (a.halves) k_rotary<T, VE, true><<<grid, 256, lds, s>>>(a, p);
