@@ -1069,10 +1069,10 @@ extern "C" int32_t zjai_rotary_frequencies(int32_t rotary_dim, double base, int3
         need(scaling == ZJAI_ROTARY_SCALE_NONE || (std::isfinite(factor) && factor >= 1.0), "rotary frequencies: factor");
         need(!yarn || (std::isfinite(trained_length) && trained_length > 0.0), "rotary frequencies: trained_length");
         need(scaling != ZJAI_ROTARY_SCALE_NTK || rotary_dim >= 4, "rotary frequencies: one pair has no base to scale");
-        if (scaling == ZJAI_ROTARY_SCALE_NTK) base *= std::pow(factor, rotary_dim / (rotary_dim - 2.0));
         for (int i = 0; i < rotary_dim / 2; ++i) {
             double f = std::pow(base, -2.0 * i / rotary_dim);
             if (scaling == ZJAI_ROTARY_SCALE_LINEAR) f /= factor;
+            if (scaling == ZJAI_ROTARY_SCALE_NTK) f *= std::pow(factor, -2.0 * i / (rotary_dim - 2));  // the larger base may be past a double
             if (yarn) {
                 const double turns = trained_length * f / 6.28318530717958647693, g = std::min(1.0, std::max(0.0, (turns - 1.0) / 31.0));
                 f = g * f + (1.0 - g) * f / factor;
