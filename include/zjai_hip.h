@@ -408,7 +408,8 @@ ZJAI_API int32_t zjai_causal_conv(zjai_ctx* ctx, const zjai_tensor* x, int32_t t
 typedef struct zjai_causal_conv_desc {
     int32_t precision, channels;  /* channels 1..2^20 */
     int32_t taps, act;            /* taps 1..8 */
-    int32_t sequences, length;    /* length: up to 2^30 */
+    int32_t sequences, length;    /* length: up to 2^30. Step: sequences * (channels, up to a multiple of 256) below
+                                     2^32 (else ZJAI_E_LIMIT) */
     const void* x;
     void* out;
     int64_t x_position, out_position; /* from one position to the next */
@@ -466,9 +467,10 @@ ZJAI_API int32_t zjai_selective_scan(zjai_ctx* ctx, const zjai_tensor* x, const 
 typedef struct zjai_selective_scan_desc {
     int32_t precision, channels;   /* channels 1..2^20 */
     int32_t groups, state_dim;     /* groups divides channels; state_dim 1..256 */
-    int32_t sequences, length;     /* length: up to 2^30; sequences * groups * (workgroups of a group's
-                                      channels, of 256 / ceil(state_dim / 16) or a quarter of that): up to 2^20
-                                      (else ZJAI_E_LIMIT) */
+    int32_t sequences, length;     /* length: up to 2^30; sequences * groups * ceil(channels / groups / k): up to
+                                      2^20, with k = 128 for state_dim up to 32, 64 up to 64, 32 up to 128, 16 above
+                                      (beyond it the call may end with ZJAI_E_LIMIT). Step: sequences * (channels *
+                                      (state_dim / 4, up to a power of two) + 256) below 2^32 */
     int32_t softplus;              /* 1: the steps are taken through softplus */
     int32_t num_slots;             /* step: states in state_in / state_out (0: as many as sequences) */
     const void *x, *delta, *b, *c;

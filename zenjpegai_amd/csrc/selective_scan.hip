@@ -512,7 +512,7 @@ ScanPlan scan_plan(const ScanArgs& a, size_t scratch_bytes) {
     const auto waves = [&]() { return std::max(1.0, (double)a.seqs * a.groups * ((cg + 64 / p.lanes - 1) / (64 / p.lanes))); };
     // Nine to sixteen states in one lane, or, where that leaves SIMDs idle even with segments of 64 positions, in four
     // (64 x 64 positions of 320 channels x 16 states f32 36 -> 27 us, 24 of 64 11.1 -> 5.4).
-    if (p.ns >= 12 && p.lanes == 1 && waves() * (a.length / 64.0) < 1024.0) {
+    if (p.ns >= 12 && p.lanes == 1 && waves() * (std::max(a.length, 1) / 64.0) < 1024.0) {
         p.ns = 4;
         p.lanes = 4;
     }
