@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(64 * SCAN_WAVES, 2) k_scan(ScanArgs a, ScanPla
     constexpr int NP = NS * LANES < 4 ? 4 : NS * LANES;  // floats of a row of b or c in LDS
     constexpr int SIDES = OUT ? 2 : 1, ITEMS = SCAN_TILE * SIDES * NP / 4, PER_LANE = (ITEMS + 64 * SCAN_WAVES - 1) / (64 * SCAN_WAVES);
     constexpr int OWNERS = LANES < SCAN_TILE ? LANES : SCAN_TILE, OWN = SCAN_TILE / OWNERS;  // positions of a tile that a lane looks after
-    __shared__ float s_bc[2][SCAN_TILE][SIDES][NP];
+    __shared__ alignas(16) float s_bc[2][SCAN_TILE][SIDES][NP];  // read and written in quads
     const int tid = threadIdx.x, lane = tid & 63, per_seg = a.groups * p.blocks, grid_segs = OUT ? p.segments : p.segments - 1;
     int id = blockIdx.x;
     const int s = id / (per_seg * grid_segs);
