@@ -329,8 +329,8 @@ ZJAI_API int32_t zjai_linear_attention_step(zjai_ctx* ctx, const zjai_linear_att
  * (i < rotary_dim / 2) at rotary position p becomes
  *     (a, b) -> magnitude * (a cos(p f_i) - b sin(p f_i), a sin(p f_i) + b cos(p f_i))
  * with the frequency f_i in radians a position; the other channels stay as they are. Stands in front of
- * zjai_linear_attention, for its queries and keys. Angles are formed in 64 bits (a position's rounding stays
- * 2^-53 of its angle however far it is), sines and products in f32, and each result is rounded once. No
+ * zjai_linear_attention, for its queries and keys. Angles are formed in 64 bits (off by 2^-51 of themselves at
+ * most, however far a position is), sines and products in f32, and each result is rounded once. No
  * counterpart in the reference. */
 #define ZJAI_ROTARY_INTERLEAVED 0 /* pair i: channels 2i, 2i + 1 */
 #define ZJAI_ROTARY_HALVES 1      /* pair i: channels i, i + rotary_dim / 2 */

@@ -20,8 +20,8 @@ struct RotaryPlan {
     int tiles;            // of a sequence
 };
 
-// (magnitude cos, magnitude sin) of p f. The angle loses its whole turns in 64 bits (relative error 2^-52: 2^-34 of a
-// radian at 2^18), down to an eighth of a turn to either side; there the power series up to the ninth and
+// (magnitude cos, magnitude sin) of p f. The angle loses its whole turns in 64 bits (two products and a constant, each off by
+// 2^-53 of itself, are within 2^-51 of the angle: 2^-33 of a radian at 2^18), down to an eighth of a turn to either side; there the power series up to the ninth and
 // tenth order are exact to 2^-27 and 2^-31.
 __device__ __forceinline__ float2 rotary_turn(int p, double f, float magnitude) {
     const double turns = (double)p * f * 0.15915494309189533577;  // 1 / (2 pi)
