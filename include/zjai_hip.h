@@ -432,7 +432,9 @@ ZJAI_API int32_t zjai_causal_conv_noalloc(zjai_ctx* ctx, const zjai_causal_conv_
 /* One position of each sequence (length 1, lengths NULL; both states given unless taps is 1). Sequence i reads
  * state_in[slots[i]] and writes state_out[slots[i]]; states of other slots stay as they were. A slot
  * outside 0..num_slots-1 marks an idle sequence, whose output stays as it was. Sequences with the same slot
- * follow one another in their order, as consecutive positions. */
+ * follow one another in their order, as consecutive positions; they are looked for among all of the call's, in
+ * a time that grows with the square of the sequences (some thousands cost as much as the states' traffic), so that
+ * more than a few thousand are better split into calls. */
 ZJAI_API int32_t zjai_causal_conv_step(zjai_ctx* ctx, const zjai_causal_conv_desc* desc);
 
 /* ------------------------------------------- causal context: selective state-space scan */

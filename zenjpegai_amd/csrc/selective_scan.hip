@@ -2,10 +2,10 @@
 //   s_t = softplus(delta_t + bias),  h_t = exp(s_t a) h_(t-1) + s_t b_t x_t,
 //   out_t = (sum over the states of c_t h_t + d x_t) * silu(z_t).
 //
-// A lane has NS states of one channel, in registers over the positions; LANES neighbouring lanes have a channel, four waves
-// of a workgroup 256 / LANES channels of one group. Positions pass in tiles of eight. What a tile needs for each channel
+// A lane has NS states of one channel, in registers over the positions; LANES neighbouring lanes have a channel, a workgroup of
+// one to four waves 64 / LANES channels of one group for each of them. Positions pass in tiles of eight. What a tile needs for each channel
 // and position (the step, its softplus, the gate) is shared out among the channel's lanes and handed round by lane
-// exchanges; b and c, which all channels of a group share, go through LDS as f32. The next tile's loads are in
+// exchanges; b and c, which all channels of a group share, go through LDS as f32. The next two tiles' loads are in
 // flight meanwhile.
 // Bound by the vector ALUs: four instructions of 4 cycles and a 2^x of 8 for each position, channel and state of a wave's lanes. 65536
 // positions of 2048 channels x 16 states bf16: outputs 483 us with the ALUs 90 % busy, ends 347 with 98 %.
