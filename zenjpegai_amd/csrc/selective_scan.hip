@@ -12,7 +12,8 @@ namespace {
 constexpr int SCAN_RUN = 16, SCAN_MAX_SEGMENTS = 256;  // segments of a thread, and of 16 threads
 
 // The decay 2^x of many positions together, as m 2^n: where states grow it may lie past f32's range although what comes of it
-// does not, and a zero stays zero. (x: past the range of an exponent for sure, or no number, which the ends show.)
+// does not, and a zero stays zero. (x is cut off well past the range of an exponent. Where it is no number, neither is the end
+// state that is added.)
 __device__ __forceinline__ void split_power(float x, float& m, int& n) {
     x = __builtin_amdgcn_fmed3f(x, -1024.0f, 1024.0f);
     const float whole = floorf(x);
